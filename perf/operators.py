@@ -70,14 +70,14 @@ def draw(rng):
     train = kind.endswith("train")
     k, n = _log_int(rng, 64, 2048), _log_int(rng, 40, 4096)
     # below the largest listed case in products and in bytes
-    products = 2.0e10 if dtype == "f32" else 6.0e10
-    rows = 5.0e8 / (_SIZE[dtype] * (k + n) * (2 if train else 1))
+    products = 2.0e10 if dtype == "f32" else 5.0e10
+    rows = 6.0e8 / (_SIZE[dtype] * (k + 2 * n) * (2 if train else 1))
     m = _log_int(rng, 1, max(1, min(262144, int(products / (k * n)), int(rows))))
     case = {"op": "grouped" if kind.startswith("grouped") else "linear", "train": train, "dtype": dtype, "m": m, "k": k,
             "n": n, "act": rng.choice(["none", "relu", "prelu", "silu", "gelu_tanh"]),
             "bias": rng.random() < 0.7, "residual": rng.random() < 0.4}
     if case["op"] == "grouped":
-        case["groups"] = _log_int(rng, 2, max(2, min(64, (1 << 26) // (k * n))))
+        case["groups"] = _log_int(rng, 2, max(2, min(64, (1 << 25) // (k * n))))
     return case
 
 
