@@ -22,6 +22,19 @@ class TensorDesc(C.Structure):
     _fields_ = [("name", C.c_char_p), ("data", C.c_void_p), ("ndim", C.c_int32), ("shape", C.c_int64 * 4)]
 
 
+class RowGroupsDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("n_groups", C.c_int32), ("tile_rows", C.c_int32), ("n_tiles", C.c_int32),
+                ("order", C.c_void_p), ("offsets", C.c_void_p), ("tiles", C.c_void_p), ("tile_offsets", C.c_void_p)]
+
+
+class LinearDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("act", C.c_int32), ("bias_dtype", C.c_int32), ("slope_dtype", C.c_int32),
+                ("M", C.c_int64), ("K", C.c_int32), ("N", C.c_int32), ("x", C.c_void_p), ("w", C.c_void_p),
+                ("bias", C.c_void_p), ("slope", C.c_void_p), ("resid", C.c_void_p), ("ldx", C.c_int64),
+                ("ldw", C.c_int64), ("ldr", C.c_int64), ("w_group_stride", C.c_int64),
+                ("groups", C.POINTER(RowGroupsDesc))]
+
+
 # name -> (restype, argtypes); every symbol include/face_recognition_amd.h declares
 _P, _I, _L, _D = C.c_void_p, C.c_int, C.c_int64, C.c_double
 SIGNATURES = {
@@ -74,6 +87,13 @@ SIGNATURES = {
     "fb_match_nearest": (_I, [_P, _P, _I, _D, _P, _P, _P, _P]),
     "fb_destroy": (_I, [_P]),
     "ev_fold_scores": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _P, _P]),
+    "fra_group_tile_rows": (_I, [_L, _I]),
+    "fra_group_tiles": (_I, [_L, _I]),
+    "fra_group_rows_workspace_bytes": (_I, [_L, _I, C.POINTER(C.c_size_t)]),
+    "fra_group_rows": (_I, [_P, _I, C.POINTER(RowGroupsDesc), _P, C.c_size_t, _P]),
+    "fra_linear": (_I, [C.POINTER(LinearDesc), _P, _P, _P]),
+    "fra_linear_backward_workspace_bytes": (_I, [C.POINTER(LinearDesc), _I, _I, _I, _I, C.POINTER(C.c_size_t)]),
+    "fra_linear_backward": (_I, [C.POINTER(LinearDesc), _P, _P, _L, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "fa_align_warp": (_I, [_P, _I, _I, _P, _I, _P, _I, _I, _P]),
 }
 

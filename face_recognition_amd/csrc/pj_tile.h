@@ -1,0 +1,234 @@
+// The tiled matrix product behind the projections: C[i][j] = sum_k A(i,k) B(j,k) on one workgroup, fp32 accumulation.
+//
+// Either operand may lie row by row ("row-major": k is the contiguous index) or contraction by contraction
+// ("contraction-major": i or j is contiguous); the four combinations are the forward product, the two gradients and the
+// Gram products, with no transposed copy in memory.  A step covers 128 bytes of k per row: 64 sixteen-bit values (two
+// 16x16x32 MFMAs deep) or 32 floats (eight 16x16x4 MFMAs deep).
+//
+// LDS images, in 16-byte chunks:
+//   row-major          [DIM rows][8 chunks of k], chunk c of row r at slot c ^ (r & 7): the sixteen rows a fragment read
+//                      touches fall on all banks;
+//   contraction-major  [KSTEP rows of k][DIM], 16 bit: chunk pair p of row k at p ^ ((k & 3) | (k >> 1 & 4)) (128 columns;
+//                      with 64, two rows of k fill a row of banks: p ^ ((k >> 1 & 1) | (k >> 2 & 2))), so the eight 32-byte
+//                      pieces that half a wave's transposing read (ds_read_b64_tr_b16) takes are on different banks;
+//                      float: chunk c at c ^ 4 (k >> 2 & 3).
+#pragma once
+
+#include "common.h"
+
+namespace fra {
+
+template <typename T> struct Elem {                 // 16-bit element types
+    static constexpr int EPC = 8;                   // elements per 16-byte chunk
+    static constexpr int KSTEP = 64;                // contraction per step
+    typedef typename vec8<T>::type Frag;            // one lane's operand of an MFMA group: 16 bytes
+    typedef typename vec4<T>::type Quad;
+};
+template <> struct Elem<float> {
+    static constexpr int EPC = 4;
+    static constexpr int KSTEP = 32;
+    typedef f32x4 Frag;
+    typedef f32x4 Quad;
+};
+
+template <typename T> __device__ __forceinline__ f32x4 pj_mma(typename Elem<T>::Frag a, typename Elem<T>::Frag b, f32x4 c) {
+    if constexpr (sizeof(T) == 2) {
+        return mfma16(a, b, c);
+    } else {
+        // a lane of k-group g holds k = 4 g + s in element s: step s multiplies the four k = 4 g + s of the groups
+#pragma unroll
+        for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// 16 bytes from any address an element may have
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Chunk { typename Elem<T>::Frag v; };
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Four { typename Elem<T>::Quad v; };
+
+// `n` valid elements (at most a chunk; none if n <= 0) from p, the rest zero
+template <typename T> __device__ __forceinline__ typename Elem<T>::Frag load_chunk(const T* p, int n) {
+    typename Elem<T>::Frag v;
+    if (n >= Elem<T>::EPC) return reinterpret_cast<const Chunk<T>*>(p)->v;
+#pragma unroll
+    for (int e = 0; e < Elem<T>::EPC; ++e) v[e] = (T)0.0f;
+    if (n > 0) {
+#pragma unroll
+        for (int e = 0; e < Elem<T>::EPC; ++e)
+            if (e < n) v[e] = p[e];
+    }
+    return v;
+}
+template <typename T> __device__ __forceinline__ void load_four(const T* p, int n, float (&o)[4]) {
+    if (n >= 4) {
+        const typename Elem<T>::Quad v = reinterpret_cast<const Four<T>*>(p)->v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (float)v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = e < n ? (float)p[e] : 0.0f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store_four(T* p, int n, const float (&v)[4]) {
+    if (n >= 4) {
+        typename Elem<T>::Quad q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = (T)v[e];
+        reinterpret_cast<Four<T>*>(p)->v = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < n) p[e] = (T)v[e];
+    }
+}
+// a parameter vector that is float or of the product's own type
+template <typename T> __device__ __forceinline__ void load_param4(const void* p, bool is_f32, int64_t at, int n, float (&o)[4]) {
+    if (is_f32) load_four<float>(reinterpret_cast<const float*>(p) + at, n, o);
+    else load_four<T>(reinterpret_cast<const T*>(p) + at, n, o);
+}
+
+template <typename T> __device__ __forceinline__ int swz_row_major(int row, int c) { return c ^ (row & 7); }
+template <typename T, int CPR> __device__ __forceinline__ int swz_k_major(int k, int c) {
+    if constexpr (sizeof(T) == 4) return c ^ (((k >> 2) & 3) << 2);
+    else if constexpr (CPR >= 16) return c ^ (((k & 3) | ((k >> 1) & 4)) << 1);
+    else return c ^ ((((k >> 1) & 1) | ((k >> 2) & 2)) << 1);       // two rows of k share a row of banks
+}
+
+// One operand of a workgroup's tile: where its chunks come from and how a wave reads its fragments.
+//   row-major: `rows` tile rows start at row0 of a row list (`order`, or the rows themselves), each `klen` long from k = 0;
+//   contraction-major: columns col0 .. col0 + DIM of an array whose rows (through `order`) k0 .. k0 + klen are summed over.
+template <typename T, bool KMAJOR, int DIM, int NT> struct Operand {
+    static constexpr int EPC = Elem<T>::EPC, KSTEP = Elem<T>::KSTEP;
+    static constexpr int CPR = KMAJOR ? DIM / EPC : 8;              // chunks per LDS row
+    static constexpr int CHUNKS = DIM * 8;                          // 16-byte chunks per tile
+    static constexpr int BYTES = CHUNKS * 16;
+    static constexpr int NLD = CHUNKS / NT;                         // per thread
+    static_assert(CHUNKS % NT == 0 && NT % CPR == 0, "whole chunks per thread, whole rows per pass");
+    typedef typename Elem<T>::Frag Frag;
+
+    const T* base;
+    const int* order;
+    int64_t ld;
+    int row0, rows, klen, cols;     // k-major: row0 = first contraction row, cols = valid columns from `base`
+
+    // row-major: rows >= 1; tile row r stands for list entry row0 + min(r, rows - 1) (rows past the end repeat the last:
+    // their results are not stored)
+    __device__ __forceinline__ const T* row_ptr(int r) const {
+        const int at = row0 + (r < rows ? r : rows - 1);
+        return base + (int64_t)(order ? order[at] : at) * ld;
+    }
+    __device__ __forceinline__ void load(Frag (&v)[NLD], int step, int tid) const {
+#pragma unroll
+        for (int j = 0; j < NLD; ++j) {
+            const int slot = j * NT + tid, r = slot / CPR, s = slot % CPR;
+            if constexpr (!KMAJOR) {
+                const int k = step * KSTEP + swz_row_major<T>(r, s) * EPC;
+                const int n = klen - k;
+                v[j] = load_chunk<T>(row_ptr(r) + (n > 0 ? k : 0), n);
+            } else {
+                const int k = step * KSTEP + r, col = swz_k_major<T, CPR>(r, s) * EPC;
+                const int n = k < klen ? cols - col : 0;
+                const T* p = base;
+                if (n > 0) {
+                    const int at = row0 + k;
+                    p = base + (int64_t)(order ? order[at] : at) * ld + col;
+                }
+                v[j] = load_chunk<T>(p, n);
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(char* tile, const Frag (&v)[NLD], int tid) {
+#pragma unroll
+        for (int j = 0; j < NLD; ++j) *reinterpret_cast<Frag*>(tile + (j * NT + tid) * 16) = v[j];
+    }
+    // fragment of the 16 rows / columns from `d0`, k half `ks` (0, 1) of the step
+    static __device__ __forceinline__ Frag frag(const char* tile, int d0, int ks, int lane) {
+        const int m = lane & 15, g = lane >> 4;
+        if constexpr (!KMAJOR) {
+            const int r = d0 + m;
+            return *reinterpret_cast<const Frag*>(tile + (r * 8 + swz_row_major<T>(r, ks * 4 + g)) * 16);
+        } else if constexpr (sizeof(T) == 2) {
+            // sixteen lanes take four rows of k x sixteen columns and receive one column of four k each
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            typedef __attribute__((address_space(3))) s16x4* LP;
+            const int k = ks * 32 + g * 8 + (m >> 2);
+            const int c0 = d0 / EPC + ((m >> 1) & 1);
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (LP)(tile + (k * CPR + swz_k_major<T, CPR>(k, c0)) * 16 + (m & 1) * 8));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (LP)(tile + ((k + 4) * CPR + swz_k_major<T, CPR>(k + 4, c0)) * 16 + (m & 1) * 8));
+            const s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(Frag, v);
+        } else {
+            Frag v;
+            const int col = d0 + m;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int k = ks * 16 + g * 4 + s;
+                v[s] = *reinterpret_cast<const float*>(tile + (k * CPR + swz_k_major<T, CPR>(k, col >> 2)) * 16 + (col & 3) * 4);
+            }
+            return v;
+        }
+    }
+};
+
+// Workgroup shape: BI x BJ results on WI x WJ waves; a wave owns MI x MJ tiles of 16 x 16.
+template <int BI_, int BJ_, int WI_, int WJ_> struct Shape {
+    static constexpr int BI = BI_, BJ = BJ_, WI = WI_, WJ = WJ_, NT = 64 * WI * WJ;
+    static constexpr int MI = BI / WI / 16, MJ = BJ / WJ / 16;
+};
+
+// acc[mi][mj][r] = C[i][j] with i = 16 mi + (lane & 15), j = 16 mj + 4 (lane >> 4) + r inside the wave's part: the j side is
+// the MFMA's row operand, so a lane holds four neighbouring j of one i.
+template <typename T, bool AK, bool BK, typename S>
+__device__ __forceinline__ void tile_product(const Operand<T, AK, S::BI, S::NT>& A, const Operand<T, BK, S::BJ, S::NT>& B,
+                                             int klen, char* lds, f32x4 (&acc)[S::MI][S::MJ]) {
+    typedef Operand<T, AK, S::BI, S::NT> OA;
+    typedef Operand<T, BK, S::BJ, S::NT> OB;
+    constexpr int BUF = OA::BYTES + OB::BYTES;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+        for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
+    const int steps = (klen + Elem<T>::KSTEP - 1) / Elem<T>::KSTEP;
+    if (steps == 0) return;
+
+    typename Elem<T>::Frag va[OA::NLD], vb[OB::NLD];
+    A.load(va, 0, tid);
+    B.load(vb, 0, tid);
+    OA::store(lds, va, tid);
+    OB::store(lds + OA::BYTES, vb, tid);
+    __syncthreads();
+    for (int t = 0; t < steps; ++t) {
+        const char* ta = lds + (t & 1) * BUF;
+        const char* tb = ta + OA::BYTES;
+        if (t + 1 < steps) {
+            A.load(va, t + 1, tid);
+            B.load(vb, t + 1, tid);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            typename Elem<T>::Frag fa[S::MI], fb[S::MJ];
+#pragma unroll
+            for (int mi = 0; mi < S::MI; ++mi) fa[mi] = OA::frag(ta, i0 + 16 * mi, ks, lane);
+#pragma unroll
+            for (int mj = 0; mj < S::MJ; ++mj) fb[mj] = OB::frag(tb, j0 + 16 * mj, ks, lane);
+#pragma unroll
+            for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+                for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = pj_mma<T>(fb[mj], fa[mi], acc[mi][mj]);
+        }
+        if (t + 1 < steps) {
+            char* na = lds + ((t + 1) & 1) * BUF;
+            OA::store(na, va, tid);
+            OB::store(na + OA::BYTES, vb, tid);
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace fra

@@ -1,0 +1,249 @@
+"""Matrices behind the embeddings: heads and maps applied to rows, one for all of them or one per group, with gradients.
+
+    linear(x, weight, bias, activation, slope, residual)            y = act(x W^T + b) + r
+    group_rows(ids, n_groups) -> RowGroups                          rows sorted by the group they name
+    grouped_linear(x, weight[G], groups, ...)                       every row through its group's matrix
+
+Uses: a head on top of the 512-wide embeddings, a map that takes one network's embeddings into another's space so that an
+existing gallery stays searchable, one such map per camera / tenant / model version, and the training of all of these.  No
+counterpart in the reference.  All products run in the HIP library (``fra_linear``, ``fra_group_rows``); there is no CPU path.
+
+Types: float32, float16, bfloat16; ``x``, ``weight`` and ``residual`` share one, ``bias`` and ``slope`` are of it or float32.
+Sums are fp32.  The calls queue on the current stream and neither synchronise nor read anything back, so they can be
+captured into a graph.  Capture a backward pass as ``torch.autograd.grad`` on leaves of which no eager graph is alive.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.FRA_F32, torch.bfloat16: _lib.FRA_BF16, torch.float16: _lib.FRA_F16}
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "prelu": 2, "silu": 3, "gelu_tanh": 4}
+MAX_GROUPS = 4096
+
+
+class _on_device:
+    """``torch.cuda.device`` that costs nothing when the device is the current one already."""
+    __slots__ = ("index", "prev")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+class RowGroups:
+    """The rows of a batch sorted by group (``group_rows``).
+
+    ``order`` int32 [rows]: row numbers by group, ascending inside a group, rows of no group last; ``offsets`` int32
+    [n_groups + 1]: group g's rows are ``order[offsets[g]:offsets[g + 1]]``.  Serves any number of products of these rows.
+    """
+
+    def __init__(self, rows: int, n_groups: int, device: torch.device):
+        lib = _lib.load()
+        self.rows, self.n_groups, self.device = rows, n_groups, device
+        tile_rows, n_tiles = lib.fra_group_tile_rows(rows, n_groups), lib.fra_group_tiles(rows, n_groups)
+        # one allocation: tiles (16-byte aligned) | order | offsets | tile_offsets
+        buf = torch.empty(4 * n_tiles + rows + 2 * n_groups + 3, dtype=torch.int32, device=device)
+        at = 4 * n_tiles
+        self._buf = buf
+        self.order = buf[at:at + rows]
+        self.offsets = buf[at + rows:at + rows + n_groups + 1]
+        base = buf.data_ptr()
+        self._desc = _lib.RowGroupsDesc(rows, n_groups, tile_rows, n_tiles, base + 4 * at, base + 4 * (at + rows), base,
+                                        base + 4 * (at + rows + n_groups + 1))
+
+
+def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
+    """Sort rows by group id: ``ids`` int32 / int64 [rows] on the device.  Ids outside [0, n_groups) name no group."""
+    if not isinstance(ids, torch.Tensor) or ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("group_rows: ids must be an int32 or int64 vector")
+    if not ids.is_cuda:
+        raise RuntimeError("group_rows: ids live on the HIP device ('cuda'); there is no CPU path")
+    n_groups = int(n_groups)
+    if not 1 <= n_groups <= MAX_GROUPS:
+        raise RuntimeError(f"group_rows: {n_groups} groups (1 to {MAX_GROUPS})")
+    lib = _lib.load()
+    ids = ids.contiguous()
+    with _on_device(ids.device):
+        g = RowGroups(ids.shape[0], n_groups, ids.device)
+        need = C.c_size_t()
+        _lib.check(lib.fra_group_rows_workspace_bytes(g.rows, n_groups, C.byref(need)), "fra_group_rows_workspace_bytes")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=ids.device) if need.value else None
+        _lib.check(lib.fra_group_rows(ids.data_ptr(), int(ids.dtype == torch.int64), C.byref(g._desc),
+                                      ws.data_ptr() if ws is not None else None, need.value,
+                                      _lib.current_stream_ptr(ids.device)), "fra_group_rows")
+    return g
+
+
+def _rows(t: torch.Tensor):
+    """(tensor, pitch): 2-D with contiguous rows, copied only if it is not."""
+    r, c = t.shape
+    s0, s1 = t.stride()
+    if (s1 != 1 and c > 1) or (r > 1 and s0 < c):
+        t = t.contiguous()
+        s0 = c
+    return t, (s0 if r > 1 else c)
+
+
+def _desc(x, ldx, weight, ldw, wg, bias, slope, residual, ldr, act, groups):
+    return _lib.LinearDesc(_DTYPES[x.dtype], act, _DTYPES[bias.dtype] if bias is not None else 0,
+                           _DTYPES[slope.dtype] if slope is not None else 0, x.shape[0], x.shape[1], weight.shape[-2],
+                           x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
+                           slope.data_ptr() if slope is not None else None,
+                           residual.data_ptr() if residual is not None else None, ldx, ldw, ldr, wg,
+                           C.pointer(groups._desc) if groups is not None else None)
+
+
+def _weight(weight):
+    """(tensor, row pitch, group pitch) of [N,K] or [G,N,K] with contiguous rows."""
+    n, k = weight.shape[-2:]
+    s0, s1 = weight.stride()[-2:]
+    if (s1 != 1 and k > 1) or (n > 1 and s0 < k) or (weight.dim() == 3 and weight.stride(0) < 0):
+        weight = weight.contiguous()
+        s0 = k
+    return weight, (s0 if n > 1 else k), (weight.stride(0) if weight.dim() == 3 else 0)
+
+
+def _forward(x, weight, bias, slope, residual, act, groups, want_preact):
+    x, ldx = _rows(x)
+    weight, ldw, wg = _weight(weight)
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _rows(residual)
+    if bias is not None:
+        bias = bias.contiguous()
+    if slope is not None:
+        slope = slope.contiguous()
+    out = torch.empty((x.shape[0], weight.shape[-2]), dtype=x.dtype, device=x.device)
+    z = torch.empty_like(out) if want_preact else None
+    if out.shape[0]:
+        d = _desc(x, ldx, weight, ldw, wg, bias, slope, residual, ldr, act, groups)
+        with _on_device(x.device):
+            _lib.check(_lib.load().fra_linear(C.byref(d), z.data_ptr() if z is not None else None, out.data_ptr(),
+                                              _lib.current_stream_ptr(x.device)), "fra_linear")
+    return out, z
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, slope, residual, act, groups):
+        need = ctx.needs_input_grad
+        want = act != 0 and any(need[:4])
+        out, z = _forward(x, weight, bias, slope, residual, act, groups, want)
+        ctx.save_for_backward(x, weight, slope, z)
+        ctx.act, ctx.groups = act, groups
+        ctx.bias_dtype = bias.dtype if bias is not None else None
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, slope, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dev = x.device
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+        dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need[1] else None
+        par = weight.shape[:-1]
+        db = torch.empty(par, dtype=ctx.bias_dtype, device=dev) if need[2] else None
+        ds = torch.empty(par, dtype=slope.dtype, device=dev) if need[3] else None
+        if any(need[:4]):
+            lib = _lib.load()
+            g, lddy = _rows(dy)
+            xr, ldx = _rows(x)
+            w, ldw, wg = _weight(weight)
+            if slope is not None:
+                slope = slope.contiguous()
+            d = _desc(xr, ldx, w, ldw, wg, None, slope, None, 0, ctx.act, ctx.groups)
+            if ctx.bias_dtype is not None:
+                d.bias_dtype = _DTYPES[ctx.bias_dtype]
+            nbytes = C.c_size_t()
+            _lib.check(lib.fra_linear_backward_workspace_bytes(C.byref(d), need[0], need[1], need[2], need[3],
+                                                               C.byref(nbytes)), "fra_linear_backward_workspace_bytes")
+            with _on_device(dev):
+                ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+                ptr = [t.data_ptr() if t is not None else None for t in (dx, dw, db, ds)]
+                _lib.check(lib.fra_linear_backward(C.byref(d), z.data_ptr() if z is not None else None, g.data_ptr(), lddy,
+                                                   *ptr, ws.data_ptr(), nbytes.value, _lib.current_stream_ptr(dev)),
+                           "fra_linear_backward")
+        return dx, dw, db, ds, (dy if need[4] else None), None, None
+
+
+def _check(what, x, weight, bias, activation, slope, residual, lead):
+    if activation not in ACTIVATIONS:
+        raise RuntimeError(f"{what}: activation {activation!r} is none of {sorted(k for k in ACTIVATIONS if k)}")
+    act = ACTIVATIONS[activation]
+    if x.dtype not in _DTYPES:
+        raise RuntimeError(f"{what}: {x.dtype} is not supported (float32, float16, bfloat16)")
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: tensors live on the HIP device ('cuda'); there is no CPU path")
+    if weight.dim() != 2 + len(lead) or tuple(weight.shape[:len(lead)]) != lead:
+        raise RuntimeError(f"{what}: weight must be [{', '.join([str(v) for v in lead] + ['N', 'K'])}], got {tuple(weight.shape)}")
+    n, k = weight.shape[-2:]
+    if n == 0 or k == 0 or x.dim() < 1 or x.shape[-1] != k:
+        raise RuntimeError(f"{what}: x {tuple(x.shape)} does not go with weight {tuple(weight.shape)}")
+    if (act == 2) != (slope is not None):
+        raise RuntimeError(f"{what}: slope goes with activation 'prelu', and only with it")
+    for name, t in (("bias", bias), ("slope", slope)):
+        if t is not None and (tuple(t.shape) != lead + (n,) or t.dtype not in (x.dtype, torch.float32)):
+            raise RuntimeError(f"{what}: {name} must be {list(lead + (n,))} in {x.dtype} or float32, got {list(t.shape)} {t.dtype}")
+    if residual is not None and tuple(residual.shape) != tuple(x.shape[:-1]) + (n,):
+        raise RuntimeError(f"{what}: residual must be {list(x.shape[:-1]) + [n]}, got {list(residual.shape)}")
+    for name, t in (("weight", weight), ("residual", residual)):
+        if t is not None and t.dtype != x.dtype:
+            raise RuntimeError(f"{what}: {name} is {t.dtype}, x is {x.dtype}")
+    for name, t in (("weight", weight), ("bias", bias), ("slope", slope), ("residual", residual)):
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, x on {x.device}")
+    return act
+
+
+def _apply(x, weight, bias, slope, residual, act, groups):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, slope, residual)):
+        return _Linear.apply(x, weight, bias, slope, residual, act, groups)
+    return _forward(x, weight, bias, slope, residual, act, groups, False)[0]
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+           slope: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` in one kernel: x [..., K], weight [N,K], bias / slope [N], residual [..., N].
+
+    ``activation``: None, 'relu', 'prelu' (with ``slope``, one value per output channel), 'silu' or 'gelu_tanh'.
+    Differentiable (once) in every tensor argument.
+    """
+    act = _check("linear", x, weight, bias, activation, slope, residual, ())
+    if x.dim() == 2:
+        return _apply(x, weight, bias, slope, residual, act, None)
+    k, n = x.shape[-1], weight.shape[0]
+    m = x.numel() // k
+    y = _apply(x.reshape(m, k), weight, bias, slope, residual.reshape(m, n) if residual is not None else None, act, None)
+    return y.reshape(tuple(x.shape[:-1]) + (n,))
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bias: Optional[torch.Tensor] = None,
+                   activation: Optional[str] = None, slope: Optional[torch.Tensor] = None,
+                   residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``linear`` with one matrix per group: x [rows,K], weight [G,N,K], bias / slope [G,N], residual [rows,N].
+
+    Row i goes through the matrix of the group its id named (``group_rows``); the result keeps the order of x.  A row of no
+    group comes out as its residual, or as zeros, and has a zero gradient.
+    """
+    if not isinstance(groups, RowGroups):
+        raise RuntimeError("grouped_linear: groups must come from group_rows")
+    act = _check("grouped_linear", x, weight, bias, activation, slope, residual, (groups.n_groups,))
+    if x.dim() != 2 or x.shape[0] != groups.rows:
+        raise RuntimeError(f"grouped_linear: x must be [{groups.rows},K], got {tuple(x.shape)}")
+    if groups.device != x.device:
+        raise RuntimeError(f"grouped_linear: groups are on {groups.device}, x on {x.device}")
+    return _apply(x, weight, bias, slope, residual, act, groups)

@@ -289,6 +289,59 @@ int ev_fold_scores(float* fl, float* fr, const uint8_t* val_mask, int n_val, int
 int fa_align_warp(const uint8_t* frame, int H, int W, const double* matrices, int n_faces, uint8_t* crops,
                   int out_h, int out_w, fra_stream stream);
 
+/* ---- products behind the embeddings --------------------------------------------------------------
+ * No counterpart in the reference (its one linear layer closes the network, face_model.py:91-92): heads and maps applied to
+ * embeddings, one for all rows or one per group of rows (camera, tenant, model version), with their gradients.
+ *
+ *     z = x w^T + bias;   out = act(z) + resid          x [M,K], w [N,K], bias / slope [N], resid / out [M,N]
+ *
+ * Any M >= 0, K, N >= 1 up to 2^24.  dtype is the type of x, w, resid, preact, out and their gradients; bias and slope are of
+ * that type or fp32.  Sums are fp32 (fp32 products on the fp32 matrix instructions).  Rows are contiguous, at a pitch of ldx /
+ * ldw / ldr elements; any element alignment works, 16-byte aligned rows are the fast ones.  Results do not depend on timing.
+ * Nothing here allocates; scratch is the caller's. */
+enum fra_activation {
+    FRA_ACT_NONE = 0, FRA_ACT_RELU = 1,
+    FRA_ACT_PRELU = 2,          /* z > 0 ? z : slope z */
+    FRA_ACT_SILU = 3,           /* z / (1 + e^-z) */
+    FRA_ACT_GELU_TANH = 4       /* z / (1 + e^(-2 sqrt(2/pi) (z + 0.044715 z^3))) */
+};
+/* The rows of a product sorted by group, filled by fra_group_rows.  order dev int32 [rows]: row numbers by group, ascending
+ * inside a group; rows whose id is outside [0, n_groups) come last.  offsets dev int32 [n_groups + 1]: group g's rows are
+ * order[offsets[g] .. offsets[g + 1]).  tiles dev int32 [n_tiles][4], 16-byte aligned, and tile_offsets dev int32
+ * [n_groups + 2]: the products' work list.  tile_rows / n_tiles: what fra_group_tile_rows / fra_group_tiles return. */
+typedef struct {
+    int64_t rows;
+    int32_t n_groups, tile_rows, n_tiles;
+    int32_t *order, *offsets, *tiles, *tile_offsets;
+} fra_row_groups;
+typedef struct {
+    int32_t dtype, act, bias_dtype, slope_dtype;
+    int64_t M;
+    int32_t K, N;
+    const void *x, *w, *bias, *slope, *resid;       /* bias, resid: NULL = none; slope: with FRA_ACT_PRELU only */
+    int64_t ldx, ldw, ldr;
+    int64_t w_group_stride;                         /* elements between the groups' matrices; bias, slope: [n_groups][N] */
+    const fra_row_groups* groups;                   /* NULL: one matrix for all rows */
+} fra_linear_desc;
+/* ids: dev int32 or int64 [g->rows]; fills order, offsets, tiles and tile_offsets of *g (whose sizes the caller has set).  A
+ * stable counting sort: one launch up to 4096 rows, else three.  At most 4096 groups.  Scratch: dev,
+ * fra_group_rows_workspace_bytes(). */
+int fra_group_tile_rows(int64_t rows, int n_groups);
+int fra_group_tiles(int64_t rows, int n_groups);
+int fra_group_rows_workspace_bytes(int64_t rows, int n_groups, size_t* bytes);
+int fra_group_rows(const void* ids, int ids_are_64bit, const fra_row_groups* g, void* workspace, size_t workspace_bytes,
+                   fra_stream stream);
+/* out dev [M,N] contiguous.  preact dev [M,N] or NULL: receives z in dtype, for the backward pass (needed there with any
+ * activation).  With groups, a row of no group gets out = resid (or zeros), and its row of preact is not written. */
+int fra_linear(const fra_linear_desc* d, void* preact, void* out, fra_stream stream);
+/* Gradients of the wanted (non-NULL) of: dx [M,K], dw [N,K] or [n_groups,N,K] (a group without rows: zeros), dbias / dslope
+ * [N] or [n_groups,N] in bias_dtype / slope_dtype, all contiguous; the residual's gradient is dy itself.  dy dev [M,N] at a
+ * pitch of lddy.  The descriptor is the forward call's; its bias and resid are not read. */
+int fra_linear_backward_workspace_bytes(const fra_linear_desc* d, int want_dx, int want_dw, int want_dbias, int want_dslope,
+                                        size_t* bytes);
+int fra_linear_backward(const fra_linear_desc* d, const void* preact, const void* dy, int64_t lddy, void* dx, void* dw,
+                        void* dbias, void* dslope, void* workspace, size_t workspace_bytes, fra_stream stream);
+
 #ifdef __cplusplus
 }
 #endif
