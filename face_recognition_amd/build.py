@@ -14,13 +14,14 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libface_recognition_amd.so")
-SOURCES = ["api.cpp", "kernels_conv.hip", "kernels_gemm.hip", "kernels_block.hip", "kernels_rblock.hip", "kernels_wblock.hip", "kernels_pblock.hip", "kernels_stem.hip", "mfn_model.hip", "fb_search.hip", "ev_fold.hip", "fa_align.hip", "kernels_tail.hip", "kernels_linear.hip"]
+SOURCES = ["api.cpp", "kernels_conv.hip", "kernels_gemm.hip", "kernels_block.hip", "kernels_rblock.hip", "kernels_wblock.hip", "kernels_pblock.hip", "kernels_stem.hip", "mfn_model.hip", "fb_search.hip", "ev_fold.hip", "fa_align.hip", "kernels_tail.hip", "kernels_linear.hip", "kernels_orth.hip"]
 ARCH = "gfx950"
 # per-source flags.  kernels_wblock.hip runs one wave per SIMD with the whole register file: its compiler-issued MFMAs
 # keep their results in ordinary registers (the project sums sit in accumulation registers through inline assembly)
 EXTRA_FLAGS = {"kernels_wblock.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                # no packed fp32 arithmetic
-               "kernels_linear.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
+               "kernels_linear.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
+               "kernels_orth.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
 
 
 def _hipcc() -> str:

@@ -181,7 +181,8 @@ template <int BI_, int BJ_, int WI_, int WJ_> struct Shape {
 
 // acc[mi][mj][r] = C[i][j] with i = 16 mi + (lane & 15), j = 16 mj + 4 (lane >> 4) + r inside the wave's part: the j side is
 // the MFMA's row operand, so a lane holds four neighbouring j of one i.
-template <typename T, bool AK, bool BK, typename S>
+// ADD: on top of what acc holds.
+template <typename T, bool AK, bool BK, typename S, bool ADD = false>
 __device__ __forceinline__ void tile_product(const Operand<T, AK, S::BI, S::NT>& A, const Operand<T, BK, S::BJ, S::NT>& B,
                                              int klen, char* lds, f32x4 (&acc)[S::MI][S::MJ]) {
     typedef Operand<T, AK, S::BI, S::NT> OA;
@@ -190,10 +191,12 @@ __device__ __forceinline__ void tile_product(const Operand<T, AK, S::BI, S::NT>&
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (!ADD) {
 #pragma unroll
-    for (int mi = 0; mi < S::MI; ++mi)
+        for (int mi = 0; mi < S::MI; ++mi)
 #pragma unroll
-        for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
+            for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
+    }
     const int steps = (klen + Elem<T>::KSTEP - 1) / Elem<T>::KSTEP;
     if (steps == 0) return;
 

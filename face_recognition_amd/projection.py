@@ -3,10 +3,12 @@
     linear(x, weight, bias, activation, slope, residual)            y = act(x W^T + b) + r
     group_rows(ids, n_groups) -> RowGroups                          rows sorted by the group they name
     grouped_linear(x, weight[G], groups, ...)                       every row through its group's matrix
+    orthogonalize(matrix, steps, coefficients)                      an update (or a fitted map) made orthogonal
 
 Uses: a head on top of the 512-wide embeddings, a map that takes one network's embeddings into another's space so that an
-existing gallery stays searchable, one such map per camera / tenant / model version, and the training of all of these.  No
-counterpart in the reference.  All products run in the HIP library (``fra_linear``, ``fra_group_rows``); there is no CPU path.
+existing gallery stays searchable, one such map per camera / tenant / model version, and the training of all of these (an
+orthogonal map leaves distances, and the thresholds set for them, as they are).  No counterpart in the reference.  All
+products run in the HIP library (``fra_linear``, ``fra_group_rows``, ``fra_orthogonalize``); there is no CPU path.
 
 Types: float32, float16, bfloat16; ``x``, ``weight`` and ``residual`` share one, ``bias`` and ``slope`` are of it or float32.
 Sums are fp32.  The calls queue on the current stream and neither synchronise nor read anything back, so they can be
@@ -247,3 +249,41 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
     if groups.device != x.device:
         raise RuntimeError(f"grouped_linear: groups are on {groups.device}, x on {x.device}")
     return _apply(x, weight, bias, slope, residual, act, groups)
+
+
+def orthogonalize(matrix: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of [..., rows, cols] (every leading index a matrix of its own), in its type.
+
+    X = matrix / |matrix|_F, then ``steps`` times X <- a X + (b P + c P P) X with P = X X^T (of the transposed matrix where it
+    is taller than wide).  The default coefficients take every singular value of an update into about [0.7, 1.2] in five
+    steps; (1.5, -0.5, 0) or (1.875, -1.25, 0.375) converge to the nearest orthogonal matrix in more.  A matrix of zeros gives
+    zeros.  Between the products values keep 22 bits.  Not differentiable: it sees the values only.
+    """
+    if not isinstance(matrix, torch.Tensor) or matrix.dim() < 2 or matrix.dtype not in _DTYPES:
+        raise RuntimeError("orthogonalize: [..., rows, cols] in float32, float16 or bfloat16")
+    if not matrix.is_cuda:
+        raise RuntimeError("orthogonalize: tensors live on the HIP device ('cuda'); there is no CPU path")
+    if len(coefficients) != 3:
+        raise RuntimeError("orthogonalize: three coefficients")
+    rows, cols = matrix.shape[-2:]
+    if rows == 0 or cols == 0:
+        raise RuntimeError(f"orthogonalize: empty matrices {tuple(matrix.shape)}")
+    g = matrix.detach()
+    if g.dim() > 3:
+        g = g.reshape(-1, rows, cols)
+    s0, s1 = g.stride()[-2:]
+    if (s1 != 1 and cols > 1) or (rows > 1 and s0 < cols):
+        g = g.contiguous()
+        s0 = cols
+    batch = g.shape[0] if g.dim() == 3 else 1
+    lib = _lib.load()
+    out = torch.empty(matrix.shape, dtype=matrix.dtype, device=matrix.device)
+    need = C.c_size_t()
+    _lib.check(lib.fra_orthogonalize_workspace_bytes(batch, rows, cols, C.byref(need)), "fra_orthogonalize_workspace_bytes")
+    with _on_device(matrix.device):
+        ws = torch.empty(need.value, dtype=torch.uint8, device=matrix.device)
+        _lib.check(lib.fra_orthogonalize(_DTYPES[g.dtype], g.data_ptr(), s0 if rows > 1 else cols,
+                                         g.stride(0) if g.dim() == 3 else 0, batch, rows, cols, int(steps),
+                                         *[float(v) for v in coefficients], out.data_ptr(), ws.data_ptr(), need.value,
+                                         _lib.current_stream_ptr(matrix.device)), "fra_orthogonalize")
+    return out

@@ -341,6 +341,14 @@ int fra_linear_backward_workspace_bytes(const fra_linear_desc* d, int want_dx, i
                                         size_t* bytes);
 int fra_linear_backward(const fra_linear_desc* d, const void* preact, const void* dy, int64_t lddy, void* dx, void* dw,
                         void* dbias, void* dslope, void* workspace, size_t workspace_bytes, fra_stream stream);
+/* Newton-Schulz orthogonalisation of `batch` matrices g [rows][cols] (pitch ldg, batch_stride elements apart), as applied to
+ * the update of a weight matrix: X = g / |g|_F, then `steps` times X <- a X + (b P + c P P) X with P = X X^T (of the transposed
+ * matrix where rows > cols).  out dev [batch][rows][cols] contiguous, dtype as g.  A matrix of zeros gives zeros.  Between
+ * products values are held to 22 bits in a range of +-255: coefficients under which the singular values stay near one.
+ * Scratch: dev, fra_orthogonalize_workspace_bytes(). */
+int fra_orthogonalize_workspace_bytes(int64_t batch, int rows, int cols, size_t* bytes);
+int fra_orthogonalize(int dtype, const void* g, int64_t ldg, int64_t batch_stride, int64_t batch, int rows, int cols, int steps,
+                      float a, float b, float c, void* out, void* workspace, size_t workspace_bytes, fra_stream stream);
 
 #ifdef __cplusplus
 }

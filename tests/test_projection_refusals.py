@@ -92,3 +92,26 @@ def test_group_refusals():
         for k in (1, 3, 4096):
             t = lib.fra_group_tile_rows(rows, k)
             assert lib.fra_group_tiles(rows, k) >= rows // t + k + (1 if rows else 0)
+
+
+def test_orthogonalize_refusals():
+    with pytest.raises(RuntimeError, match="HIP device"):
+        projection.orthogonalize(torch.zeros(3, 3))
+    with pytest.raises(RuntimeError, match="rows, cols"):
+        projection.orthogonalize(torch.zeros(3))
+    with pytest.raises(RuntimeError, match="rows, cols"):
+        projection.orthogonalize(torch.zeros(3, 3, dtype=torch.float64))
+    lib = _lib.load()
+    n = C.c_size_t()
+    usual = (3.4445, -4.775, 2.0315)
+
+    def call(dtype=_lib.FRA_F32, g=64, ldg=8, bs=0, batch=1, rows=4, cols=8, steps=5, abc=usual, out=64, ws=64, nbytes=1 << 40):
+        return lib.fra_orthogonalize(dtype, g, ldg, bs, batch, rows, cols, steps, *abc, out, ws, nbytes, None)
+
+    for over in (dict(dtype=5), dict(g=None), dict(ldg=7), dict(bs=-1), dict(batch=-1), dict(batch=65536), dict(rows=0), dict(cols=0),
+                 dict(rows=40000), dict(steps=0), dict(steps=101), dict(abc=(17.0, 0.0, 0.0)), dict(abc=(1.0, float("nan"), 0.0)), dict(out=None)):
+        assert call(**over) == 1, over
+    assert lib.fra_orthogonalize_workspace_bytes(1, 4, 8, C.byref(n)) == 0 and n.value > 0
+    assert call(nbytes=n.value - 1) == 5 and call(ws=None) == 5
+    assert call(batch=0, g=None, out=None, ws=None, nbytes=0) == 0
+    assert lib.fra_orthogonalize_workspace_bytes(1, 0, 8, C.byref(n)) == 1 and lib.fra_orthogonalize_workspace_bytes(1, 4, 8, None) == 1
