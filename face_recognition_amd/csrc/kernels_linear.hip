@@ -73,7 +73,7 @@ struct FwdArgs {
     int K, N, act, bias_f32, slope_f32, n_col_tiles;
 };
 
-template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_forward_kernel(FwdArgs a) {
+template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_forward_kernel(FwdArgs a) {
     typedef Operand<T, false, S::BI, S::NT> OA;
     typedef Operand<T, false, S::BJ, S::NT> OB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -87,7 +87,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_fo
     A.base = (const T*)a.x; A.order = a.rows.order; A.ld = a.ldx; A.row0 = begin; A.rows = end - begin; A.klen = a.K; A.cols = 0;
     OB B;
     B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0); B.order = nullptr; B.ld = a.ldw; B.row0 = n0; B.rows = a.N - n0; B.klen = a.K; B.cols = 0;
-    tile_product<T, false, false, S>(A, B, live ? a.K : 0, lds, acc);
+    tile_product<T, false, false, S, DMA>(A, B, live ? a.K : 0, lds, acc);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i0 = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), j0 = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);
@@ -117,15 +117,15 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_fo
     }
 }
 
-// dx = dz W: rows of dz (contiguous [M][N]), W contraction-major
+// dx = dz W: rows of dz, W contraction-major
 struct DxArgs {
     RowArgs rows;
     const void *dz, *w;
     void* dx;
     int64_t lddz, ldw, wg;
-    int K, N, n_col_tiles;
+    int K, N, Np, n_col_tiles;  // Np: columns of dz, zeros from N on (its pitch if it lies in the workspace, else N)
 };
-template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dx_kernel(DxArgs a) {
+template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_dx_kernel(DxArgs a) {
     typedef Operand<T, false, S::BI, S::NT> OA;
     typedef Operand<T, true, S::BJ, S::NT> OB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -136,10 +136,10 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dx
     const int k0 = ct * S::BJ;
     f32x4 acc[S::MI][S::MJ];
     OA A;
-    A.base = (const T*)a.dz; A.order = a.rows.order; A.ld = a.lddz; A.row0 = begin; A.rows = end - begin; A.klen = a.N; A.cols = 0;
+    A.base = (const T*)a.dz; A.order = a.rows.order; A.ld = a.lddz; A.row0 = begin; A.rows = end - begin; A.klen = a.Np; A.cols = 0;
     OB B;
     B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0) + k0; B.order = nullptr; B.ld = a.ldw; B.row0 = 0; B.rows = 0; B.klen = a.N; B.cols = a.K - k0;
-    tile_product<T, false, true, S>(A, B, live ? a.N : 0, lds, acc);
+    tile_product<T, false, true, S, DMA>(A, B, live ? a.Np : 0, lds, acc);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i0 = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), j0 = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);
@@ -165,9 +165,9 @@ struct DwArgs {
     const void *dz, *x;
     void* dw;                   // T [G][N][K], or float partial sums if splits > 1
     int64_t lddz, ldx;
-    int K, N, n_ti, n_tj, splits;
+    int K, N, Np, n_ti, n_tj, splits;
 };
-template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dw_kernel(DwArgs a) {
+template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_dw_kernel(DwArgs a) {
     typedef Operand<T, true, S::BI, S::NT> OA;
     typedef Operand<T, true, S::BJ, S::NT> OB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -186,10 +186,10 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dw
     const int n0 = ti * S::BI, k0 = tj * S::BJ;
     f32x4 acc[S::MI][S::MJ];
     OA A;
-    A.base = (const T*)a.dz + n0; A.order = a.rows.order; A.ld = a.lddz; A.row0 = begin; A.rows = 0; A.klen = end - begin; A.cols = a.N - n0;
+    A.base = (const T*)a.dz + n0; A.order = a.rows.order; A.ld = a.lddz; A.row0 = begin; A.rows = 0; A.klen = end - begin; A.cols = a.Np - n0;
     OB B;
     B.base = (const T*)a.x + k0; B.order = a.rows.order; B.ld = a.ldx; B.row0 = begin; B.rows = 0; B.klen = end - begin; B.cols = a.K - k0;
-    tile_product<T, true, true, S>(A, B, end - begin, lds, acc);
+    tile_product<T, true, true, S, DMA>(A, B, end - begin, lds, acc);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i0 = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), j0 = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);
@@ -227,10 +227,10 @@ template <typename T> __global__ __launch_bounds__(256) void pj_join_kernel(cons
 struct DzArgs {
     RowArgs rows;
     const void *dy, *z, *slope;
-    void* dz;                   // nullptr: dz = dy (no activation), only the sums are wanted
+    void* dz;                   // [M][Np], zeros from column N on; nullptr: dz = dy, only the sums are wanted
     float *part_b, *part_s;     // [tiles][N], nullptr where not wanted
     int64_t lddy;
-    int N, act, slope_f32, tile_rows, n_col_tiles;
+    int N, Np, act, slope_f32, tile_rows, n_col_tiles;
 };
 template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs a) {
     __shared__ f32x4 sums[2][4][64];
@@ -240,7 +240,7 @@ template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = ct * 256 + lane * 4, left = a.N - n;
     float sb[4] = {0, 0, 0, 0}, ss[4] = {0, 0, 0, 0}, sl[4] = {0, 0, 0, 0};
-    if (left > 0) {
+    if (n < a.Np) {
         if (a.slope) load_param4<T>(a.slope, a.slope_f32, (int64_t)g * a.N + n, left, sl);
         for (int at = begin + wave; at < end; at += 4) {
             const int64_t row = a.rows.order ? a.rows.order[at] : at;
@@ -253,7 +253,7 @@ template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs
                 sb[e] += d[e];
                 ss[e] += z[e] > 0.0f ? 0.0f : dy[e] * z[e];
             }
-            if (a.dz) store_four<T>((T*)a.dz + row * a.N + n, left, d);
+            if (a.dz) store_four<T>((T*)a.dz + row * a.Np + n, 4, d);
         }
     }
 #pragma unroll
@@ -444,7 +444,12 @@ __global__ __launch_bounds__(256) void pj_group_scan_kernel(GroupArgs a) {
 // ---- launchers ------------------------------------------------------------------------------------------------------
 
 // dynamic LDS of a product kernel: two buffers of both operands' tiles
-template <typename T, typename S> constexpr int product_lds() { return 2 * (S::BI + S::BJ) * 128; }
+template <typename S> constexpr int product_lds() { return 2 * (S::BI + S::BJ) * 128; }
+
+// rows at `p`, `pitches` (one, or several or-ed together) elements apart and `len` long, consist of whole aligned chunks
+template <typename T> static bool dma_ok(const void* p, int64_t pitches, int64_t len) {
+    return ((uintptr_t)p & 15) == 0 && ((pitches | len) & (16 / (int64_t)sizeof(T) - 1)) == 0;
+}
 
 template <typename K> static int raise_lds(K kernel, int bytes, std::atomic<uint64_t>& done) {
     return ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), bytes, done);
@@ -514,15 +519,18 @@ template <typename T> static int forward_t(const fra_linear_desc* d, void* z, vo
     a.n_col_tiles = cdiv(d->N, bi);
     const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
     if (int rc = check_grid(blocks, "fra_linear")) return rc;
-    if (big) PJ_LAUNCH((pj_forward_kernel<T, Big>), blocks, Big::NT, (product_lds<T, Big>()), s, a);
-    else PJ_LAUNCH((pj_forward_kernel<T, Small>), blocks, Small::NT, (product_lds<T, Small>()), s, a);
+    const bool dma = dma_ok<T>(d->x, d->ldx, d->K) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
+    if (big && dma) PJ_LAUNCH((pj_forward_kernel<T, Big, true>), blocks, Big::NT, product_lds<Big>(), s, a);
+    else if (big) PJ_LAUNCH((pj_forward_kernel<T, Big, false>), blocks, Big::NT, product_lds<Big>(), s, a);
+    else if (dma) PJ_LAUNCH((pj_forward_kernel<T, Small, true>), blocks, Small::NT, product_lds<Small>(), s, a);
+    else PJ_LAUNCH((pj_forward_kernel<T, Small, false>), blocks, Small::NT, product_lds<Small>(), s, a);
     return FRA_OK;
 }
 
 // ---- backward: what goes where in the workspace
 struct BackwardPlan {
     bool need_dz, need_sums;
-    int dz_rows, n_tiles, splits;
+    int dz_rows, n_tiles, splits, Np;
     size_t off_dz, off_b, off_s, off_part, bytes;
 };
 static BackwardPlan backward_plan(const fra_linear_desc* d, bool dx, bool dw, bool db, bool ds) {
@@ -531,7 +539,11 @@ static BackwardPlan backward_plan(const fra_linear_desc* d, bool dx, bool dw, bo
     const fra_row_groups* g = d->groups;
     const int G = g ? g->n_groups : 1;
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-    p.need_dz = d->act != PJ_NONE && (dx || dw);
+    // dz gets rows of whole 16-byte chunks, so that the products can fetch it by DMA: without activation, a copy of dy where
+    // N does not give it such rows
+    const int epc = (int)(16 / es);
+    p.Np = (d->N + epc - 1) / epc * epc;
+    p.need_dz = (d->act != PJ_NONE || p.Np != d->N) && (dx || dw);
     p.need_sums = db || ds;
     p.dz_rows = g ? g->tile_rows : 64;
     p.n_tiles = g ? g->n_tiles : cdiv(d->M, p.dz_rows);
@@ -542,7 +554,7 @@ static BackwardPlan backward_plan(const fra_linear_desc* d, bool dx, bool dw, bo
     if (sp > steps / 4) sp = steps / 4;
     p.splits = dw && sp > 1 ? (int)sp : 1;
     size_t at = 0;
-    p.off_dz = at; if (p.need_dz) at += up((size_t)d->M * d->N * es);
+    p.off_dz = at; if (p.need_dz) at += up((size_t)d->M * p.Np * es);
     p.off_b = at; if (db) at += up((size_t)p.n_tiles * d->N * 4);
     p.off_s = at; if (ds) at += up((size_t)p.n_tiles * d->N * 4);
     p.off_part = at; if (p.splits > 1) at += up((size_t)p.splits * G * d->N * d->K * 4);
@@ -562,8 +574,8 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& p, const voi
         a.dz = p.need_dz ? ws + p.off_dz : nullptr;
         a.part_b = db ? (float*)(ws + p.off_b) : nullptr;
         a.part_s = ds ? (float*)(ws + p.off_s) : nullptr;
-        a.lddy = lddy; a.N = d->N; a.act = d->act; a.slope_f32 = d->slope_dtype == FRA_F32;
-        a.tile_rows = p.dz_rows; a.n_col_tiles = cdiv(d->N, 256);
+        a.lddy = lddy; a.N = d->N; a.Np = p.Np; a.act = d->act; a.slope_f32 = d->slope_dtype == FRA_F32;
+        a.tile_rows = p.dz_rows; a.n_col_tiles = cdiv(p.Np, 256);
         const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
         if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
         hipLaunchKernelGGL((pj_dz_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
@@ -580,27 +592,32 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& p, const voi
         FRA_HIP(hipGetLastError());
     }
     const void* dz = p.need_dz ? ws + p.off_dz : dy;
-    const int64_t lddz = p.need_dz ? d->N : lddy;
+    const int64_t lddz = p.need_dz ? p.Np : lddy;
+    const int Np = p.need_dz ? p.Np : d->N;
     if (dx && d->M > 0) {
         DxArgs a;
         const bool big = g ? g->tile_rows == 128 : big_tiles(d->M, d->K);
         const int bi = big ? 128 : 64;
         a.rows = row_args(d, bi);
-        a.dz = dz; a.w = d->w; a.dx = dx; a.lddz = lddz; a.ldw = d->ldw; a.wg = d->w_group_stride; a.K = d->K; a.N = d->N;
+        a.dz = dz; a.w = d->w; a.dx = dx; a.lddz = lddz; a.ldw = d->ldw; a.wg = d->w_group_stride; a.K = d->K; a.N = d->N; a.Np = Np;
         a.n_col_tiles = cdiv(d->K, bi);
         const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
         if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
-        if (big) PJ_LAUNCH((pj_dx_kernel<T, Big>), blocks, Big::NT, (product_lds<T, Big>()), s, a);
-        else PJ_LAUNCH((pj_dx_kernel<T, Small>), blocks, Small::NT, (product_lds<T, Small>()), s, a);
+        const bool dma = dma_ok<T>(dz, lddz, Np) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
+        if (big && dma) PJ_LAUNCH((pj_dx_kernel<T, Big, true>), blocks, Big::NT, product_lds<Big>(), s, a);
+        else if (big) PJ_LAUNCH((pj_dx_kernel<T, Big, false>), blocks, Big::NT, product_lds<Big>(), s, a);
+        else if (dma) PJ_LAUNCH((pj_dx_kernel<T, Small, true>), blocks, Small::NT, product_lds<Small>(), s, a);
+        else PJ_LAUNCH((pj_dx_kernel<T, Small, false>), blocks, Small::NT, product_lds<Small>(), s, a);
     }
     if (dw) {
         DwArgs a;
         a.rows = row_args(d, 128);
-        a.dz = dz; a.x = d->x; a.dw = p.splits > 1 ? (void*)(ws + p.off_part) : dw; a.lddz = lddz; a.ldx = d->ldx; a.K = d->K; a.N = d->N;
+        a.dz = dz; a.x = d->x; a.dw = p.splits > 1 ? (void*)(ws + p.off_part) : dw; a.lddz = lddz; a.ldx = d->ldx; a.K = d->K; a.N = d->N; a.Np = Np;
         a.n_ti = cdiv(d->N, 128); a.n_tj = cdiv(d->K, 128); a.splits = p.splits;
         const int64_t blocks = (int64_t)a.n_ti * a.n_tj * a.splits * G;
         if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
-        PJ_LAUNCH((pj_dw_kernel<T, Big>), blocks, Big::NT, (product_lds<T, Big>()), s, a);
+        if (dma_ok<T>(dz, lddz, Np) && dma_ok<T>(d->x, d->ldx, d->K)) PJ_LAUNCH((pj_dw_kernel<T, Big, true>), blocks, Big::NT, product_lds<Big>(), s, a);
+        else PJ_LAUNCH((pj_dw_kernel<T, Big, false>), blocks, Big::NT, product_lds<Big>(), s, a);
         if (p.splits > 1) {
             const int64_t n = (int64_t)G * d->N * d->K, jb = (n + 1023) / 1024;
             if (int rc = check_grid(jb, "fra_linear_backward")) return rc;

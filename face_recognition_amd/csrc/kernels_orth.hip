@@ -109,11 +109,11 @@ template <typename T, bool BK, typename S> __global__ __launch_bounds__(S::NT) v
     const int64_t boff = b * a.sb + (BK ? j0 : 0);
     // the small parts first, so that they are added before the large ones
     A.base = a.al + b * a.sa; B.base = a.bh + boff;
-    tile_product<f16, false, BK, S>(A, B, a.K, lds, acc);
+    tile_product<f16, false, BK, S, true>(A, B, a.K, lds, acc);
     A.base = a.ah + b * a.sa; B.base = a.bl + boff;
-    tile_product<f16, false, BK, S, true>(A, B, a.K, lds, acc);
+    tile_product<f16, false, BK, S, true, true>(A, B, a.K, lds, acc);
     A.base = a.ah + b * a.sa; B.base = a.bh + boff;
-    tile_product<f16, false, BK, S, true>(A, B, a.K, lds, acc);
+    tile_product<f16, false, BK, S, true, true>(A, B, a.K, lds, acc);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int li = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), lj = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);

@@ -94,6 +94,22 @@ template <typename T, int CPR> __device__ __forceinline__ int swz_k_major(int k,
     else return c ^ ((((k >> 1) & 1) | ((k >> 2) & 2)) << 1);       // two rows of k share a row of banks
 }
 
+// 16 bytes per lane from global memory into LDS at `lds` + 16 lane, without passing through registers.  Written out (the
+// instruction has no register result) so that the compiler does not put a wait for it in front of every LDS read; the loops
+// that use it wait by count (dma_wait_barrier) before the barrier that publishes a tile.  m0 holds the LDS address; one wait
+// state lies between its write and the load.
+// The asm takes the LDS pointer itself: memory whose address never leaves the kernel's own loads counts as unwritten.
+typedef __attribute__((address_space(3))) char* LdsPtr;
+__device__ __forceinline__ void dma16(const void* g, LdsPtr lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+}
+// at most N loads of this wave still on their way, all its LDS reads done; then the workgroup's barrier
+template <int N> __device__ __forceinline__ void dma_wait_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+// what a lane reads in place of a chunk outside its operand
+static __device__ __attribute__((aligned(16))) const float pj_zeros[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+
 // One operand of a workgroup's tile: where its chunks come from and how a wave reads its fragments.
 //   row-major: `rows` tile rows start at row0 of a row list (`order`, or the rows themselves), each `klen` long from k = 0;
 //   contraction-major: columns col0 .. col0 + DIM of an array whose rows (through `order`) k0 .. k0 + klen are summed over.
@@ -141,6 +157,62 @@ template <typename T, bool KMAJOR, int DIM, int NT> struct Operand {
 #pragma unroll
         for (int j = 0; j < NLD; ++j) *reinterpret_cast<Frag*>(tile + (j * NT + tid) * 16) = v[j];
     }
+    // ---- staging by DMA: every chunk is wholly inside or outside (klen or cols, pitch and base multiples of 16 bytes)
+    struct Dma {
+        const char* p[NLD];     // this lane's chunk of every pass at step 0 (k-major through a list: its column)
+        int next[KMAJOR ? NLD : 1];     // k-major through a list: row numbers of the next step to issue
+        bool in;                // k-major: the lane's column is inside (the same for all passes)
+    };
+    __device__ __forceinline__ void dma_init(Dma& d, int tid) const {
+        if constexpr (!KMAJOR) {
+            // the lane's chunk is at the same k in every pass: rows of one lane differ by a multiple of 8
+            static_assert(NT / 8 % 8 == 0, "");
+            const int c = swz_row_major<T>(tid / 8, tid % 8) * EPC;
+#pragma unroll
+            for (int j = 0; j < NLD; ++j) d.p[j] = reinterpret_cast<const char*>(row_ptr(j * (NT / 8) + tid / 8) + c);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NLD; ++j) {
+                const int r = j * (NT / CPR) + tid / CPR, col = swz_k_major<T, CPR>(r, tid % CPR) * EPC;
+                d.p[j] = reinterpret_cast<const char*>(base + (order ? 0 : (int64_t)(row0 + r) * ld) + (col < cols ? col : 0));
+                d.next[j] = 0;
+            }
+            dma_rows(d, 0, tid);
+        }
+    }
+    // k-major through a list: fetch the row numbers of `step`
+    __device__ __forceinline__ void dma_rows(Dma& d, int step, int tid) const {
+        if constexpr (KMAJOR) {
+            if (!order) return;
+#pragma unroll
+            for (int j = 0; j < NLD; ++j) {
+                const int k = step * KSTEP + j * (NT / CPR) + tid / CPR;
+                d.next[j] = order[row0 + (k < klen ? k : klen - 1)];
+            }
+        }
+    }
+    __device__ __forceinline__ void dma_issue(const Dma& d, int step, LdsPtr lds, int tid) const {
+        const bool tail = (step + 1) * KSTEP > klen;
+        if constexpr (KMAJOR) {     // the row numbers have arrived before the first load leaves: a wait for one of them in
+                                    // between would wait for the loads before it as well
+#pragma unroll
+            for (int j = 0; j < NLD; ++j) asm volatile("" ::"v"(d.next[j]));
+        }
+#pragma unroll
+        for (int j = 0; j < NLD; ++j) {
+            const char* p;
+            if constexpr (!KMAJOR) {
+                p = d.p[j] + (int64_t)step * 128;
+                if (tail && step * KSTEP + swz_row_major<T>(tid / 8, tid % 8) * EPC >= klen) p = reinterpret_cast<const char*>(pj_zeros);
+            } else {
+                const int r = j * (NT / CPR) + tid / CPR;
+                const bool inside = swz_k_major<T, CPR>(r, tid % CPR) * EPC < cols && (!tail || step * KSTEP + r < klen);
+                p = d.p[j] + (order ? (int64_t)d.next[j] * ld : (int64_t)step * KSTEP * ld) * (int)sizeof(T);
+                if (!inside) p = reinterpret_cast<const char*>(pj_zeros);
+            }
+            dma16(p, lds + j * (NT * 16));
+        }
+    }
     // fragment of the 16 rows / columns from `d0`, k half `ks` (0, 1) of the step
     static __device__ __forceinline__ Frag frag(const char* tile, int d0, int ks, int lane) {
         const int m = lane & 15, g = lane >> 4;
@@ -179,10 +251,30 @@ template <int BI_, int BJ_, int WI_, int WJ_> struct Shape {
     static constexpr int MI = BI / WI / 16, MJ = BJ / WJ / 16;
 };
 
+// The MFMAs of one step on the tiles in LDS.
+template <typename T, bool AK, bool BK, typename S>
+__device__ __forceinline__ void tile_step(const char* ta, const char* tb, int i0, int j0, int lane, f32x4 (&acc)[S::MI][S::MJ]) {
+    typedef Operand<T, AK, S::BI, S::NT> OA;
+    typedef Operand<T, BK, S::BJ, S::NT> OB;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+        typename Elem<T>::Frag fa[S::MI], fb[S::MJ];
+#pragma unroll
+        for (int mi = 0; mi < S::MI; ++mi) fa[mi] = OA::frag(ta, i0 + 16 * mi, ks, lane);
+#pragma unroll
+        for (int mj = 0; mj < S::MJ; ++mj) fb[mj] = OB::frag(tb, j0 + 16 * mj, ks, lane);
+#pragma unroll
+        for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+            for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = pj_mma<T>(fb[mj], fa[mi], acc[mi][mj]);
+    }
+}
+
 // acc[mi][mj][r] = C[i][j] with i = 16 mi + (lane & 15), j = 16 mj + 4 (lane >> 4) + r inside the wave's part: the j side is
-// the MFMA's row operand, so a lane holds four neighbouring j of one i.
-// ADD: on top of what acc holds.
-template <typename T, bool AK, bool BK, typename S, bool ADD = false>
+// the MFMA's row operand, so a lane holds four neighbouring j of one i.  klen: the longer of the operands' (an operand's
+// chunks past its own are zeros).  ADD: on top of what acc holds.  Two LDS buffers: step t + 1 is on its way while t runs.
+// DMA: both operands are staged without registers (see Operand::Dma for what that asks of them).
+template <typename T, bool AK, bool BK, typename S, bool DMA, bool ADD = false>
 __device__ __forceinline__ void tile_product(const Operand<T, AK, S::BI, S::NT>& A, const Operand<T, BK, S::BJ, S::NT>& B,
                                              int klen, char* lds, f32x4 (&acc)[S::MI][S::MJ]) {
     typedef Operand<T, AK, S::BI, S::NT> OA;
@@ -200,37 +292,57 @@ __device__ __forceinline__ void tile_product(const Operand<T, AK, S::BI, S::NT>&
     const int steps = (klen + Elem<T>::KSTEP - 1) / Elem<T>::KSTEP;
     if (steps == 0) return;
 
-    typename Elem<T>::Frag va[OA::NLD], vb[OB::NLD];
-    A.load(va, 0, tid);
-    B.load(vb, 0, tid);
-    OA::store(lds, va, tid);
-    OB::store(lds + OA::BYTES, vb, tid);
-    __syncthreads();
-    for (int t = 0; t < steps; ++t) {
-        const char* ta = lds + (t & 1) * BUF;
-        const char* tb = ta + OA::BYTES;
-        if (t + 1 < steps) {
-            A.load(va, t + 1, tid);
-            B.load(vb, t + 1, tid);
+    if constexpr (DMA) {
+        constexpr int NLD = OA::NLD + OB::NLD;
+        typename OA::Dma da;
+        typename OB::Dma db;
+        const LdsPtr dst = (LdsPtr)lds + __builtin_amdgcn_readfirstlane(wave) * 1024;
+        A.dma_init(da, tid);
+        B.dma_init(db, tid);
+        A.dma_issue(da, 0, dst, tid);
+        B.dma_issue(db, 0, dst + OA::BYTES, tid);
+        if (steps > 1) {
+            A.dma_rows(da, 1, tid);
+            B.dma_rows(db, 1, tid);
         }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            typename Elem<T>::Frag fa[S::MI], fb[S::MJ];
-#pragma unroll
-            for (int mi = 0; mi < S::MI; ++mi) fa[mi] = OA::frag(ta, i0 + 16 * mi, ks, lane);
-#pragma unroll
-            for (int mj = 0; mj < S::MJ; ++mj) fb[mj] = OB::frag(tb, j0 + 16 * mj, ks, lane);
-#pragma unroll
-            for (int mi = 0; mi < S::MI; ++mi)
-#pragma unroll
-                for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = pj_mma<T>(fb[mj], fa[mi], acc[mi][mj]);
+        for (int t = 0; t < steps; ++t) {
+            if (t + 1 < steps) {
+                const LdsPtr to = dst + ((t + 1) & 1) * BUF;
+                A.dma_issue(da, t + 1, to, tid);
+                B.dma_issue(db, t + 1, to + OA::BYTES, tid);
+                dma_wait_barrier<NLD>();            // step t is in LDS, t + 1 on its way
+            } else {
+                dma_wait_barrier<0>();
+            }
+            if (t + 2 < steps) {
+                A.dma_rows(da, t + 2, tid);
+                B.dma_rows(db, t + 2, tid);
+            }
+            const char* ta = lds + (t & 1) * BUF;
+            tile_step<T, AK, BK, S>(ta, ta + OA::BYTES, i0, j0, lane, acc);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // everyone is done with step t's buffer
         }
-        if (t + 1 < steps) {
-            char* na = lds + ((t + 1) & 1) * BUF;
-            OA::store(na, va, tid);
-            OB::store(na + OA::BYTES, vb, tid);
-        }
+    } else {
+        typename Elem<T>::Frag va[OA::NLD], vb[OB::NLD];
+        A.load(va, 0, tid);
+        B.load(vb, 0, tid);
+        OA::store(lds, va, tid);
+        OB::store(lds + OA::BYTES, vb, tid);
         __syncthreads();
+        for (int t = 0; t < steps; ++t) {
+            const char* ta = lds + (t & 1) * BUF;
+            if (t + 1 < steps) {
+                A.load(va, t + 1, tid);
+                B.load(vb, t + 1, tid);
+            }
+            tile_step<T, AK, BK, S>(ta, ta + OA::BYTES, i0, j0, lane, acc);
+            if (t + 1 < steps) {
+                char* na = lds + ((t + 1) & 1) * BUF;
+                OA::store(na, va, tid);
+                OB::store(na + OA::BYTES, vb, tid);
+            }
+            __syncthreads();
+        }
     }
 }
 
