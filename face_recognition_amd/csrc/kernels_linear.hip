@@ -30,6 +30,18 @@ template <typename T> __device__ __forceinline__ float pj_act(int act, float z, 
         default: return z;
     }
 }
+// one branch for a whole piece
+template <typename T, int V> __device__ __forceinline__ void pj_act_all(int act, float (&v)[V], const float (&s)[V]) {
+    switch (act) {
+#define PJ_CASE(A)                                                \
+    case A:                                                       \
+        _Pragma("unroll") for (int e = 0; e < V; ++e) v[e] = pj_act<T>(A, v[e], s[e]); \
+        break;
+        PJ_CASE(PJ_RELU) PJ_CASE(PJ_PRELU) PJ_CASE(PJ_SILU) PJ_CASE(PJ_GELU_TANH)
+#undef PJ_CASE
+        default: break;
+    }
+}
 template <typename T> __device__ __forceinline__ float pj_act_grad(int act, float z, float s) {
     switch (act) {
         case PJ_RELU: return z > 0.0f ? 1.0f : 0.0f;
@@ -73,6 +85,62 @@ struct FwdArgs {
     int K, N, act, bias_f32, slope_f32, n_col_tiles;
 };
 
+// A lane's columns are the same in all its pieces, so bias and slope sit in registers.
+template <typename T> struct ForwardEmit {
+    static constexpr int V = 16 / sizeof(T);
+    struct Pre {
+        int row;                    // -1: past the tile's rows or columns
+        typename Elem<T>::Frag r;
+    };
+    const FwdArgs* a;
+    int begin, count, n0, left;     // left: valid columns from the lane's first
+    bool live;
+    float bi[V], sl[V];
+    __device__ __forceinline__ void init(int g, int col) {
+        const int n = n0 + col;
+        left = a->N - n;
+#pragma unroll
+        for (int q = 0; q < V; q += 4) {
+            float b4[4] = {0, 0, 0, 0}, s4[4] = {0, 0, 0, 0};
+            if (a->bias && live) load_param4<T>(a->bias, a->bias_f32, (int64_t)g * a->N + n + q, left - q, b4);
+            if (a->slope && live) load_param4<T>(a->slope, a->slope_f32, (int64_t)g * a->N + n + q, left - q, s4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { bi[q + e] = b4[e]; sl[q + e] = s4[e]; }
+        }
+    }
+    __device__ __forceinline__ Pre pre(int i, int j) const {
+        Pre p;
+        p.row = -1;
+#pragma unroll
+        for (int e = 0; e < V; ++e) p.r[e] = (T)0.0f;
+        if (i < count && left > 0) {
+            p.row = a->rows.order ? a->rows.order[begin + i] : begin + i;
+            if (a->resid) p.r = load_chunk<T>((const T*)a->resid + (int64_t)p.row * a->ldr + n0 + j, left);
+        }
+        return p;
+    }
+    __device__ __forceinline__ void emit(const Pre& p, int, int j, float (&v)[V]) const {
+        if (p.row < 0) return;
+        const int64_t at = (int64_t)p.row * a->N + n0 + j;
+        typename Elem<T>::Frag o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += bi[e];
+        if (a->z && live) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = (T)v[e];
+            store_chunk<T>((T*)a->z + at, left, o);
+        }
+        if (!live) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = 0.0f;
+        } else {
+            pj_act_all<T, V>(a->act, v, sl);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = (T)(v[e] + (float)p.r[e]);
+        store_chunk<T>((T*)a->y + at, left, o);
+    }
+};
 template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_forward_kernel(FwdArgs a) {
     typedef Operand<T, false, S::BI, S::NT> OA;
     typedef Operand<T, false, S::BJ, S::NT> OB;
@@ -89,32 +157,10 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
     B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0); B.order = nullptr; B.ld = a.ldw; B.row0 = n0; B.rows = a.N - n0; B.klen = a.K; B.cols = 0;
     tile_product<T, false, false, S, DMA>(A, B, live ? a.K : 0, lds, acc);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), j0 = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);
-#pragma unroll
-    for (int mj = 0; mj < S::MJ; ++mj) {
-        const int n = n0 + j0 + 16 * mj, left = a.N - n;
-        if (left <= 0) continue;
-        float bi[4] = {0, 0, 0, 0}, sl[4] = {0, 0, 0, 0};
-        if (a.bias && live) load_param4<T>(a.bias, a.bias_f32, (int64_t)g * a.N + n, left, bi);
-        if (a.slope && live) load_param4<T>(a.slope, a.slope_f32, (int64_t)g * a.N + n, left, sl);
-#pragma unroll
-        for (int mi = 0; mi < S::MI; ++mi) {
-            const int at = begin + i0 + 16 * mi;
-            if (at >= end) continue;
-            const int64_t row = a.rows.order ? a.rows.order[at] : at;
-            float v[4], r[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[mi][mj][e] + bi[e];
-            if (a.z && live) store_four<T>((T*)a.z + row * a.N + n, left, v);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = live ? pj_act<T>(a.act, v[e], sl[e]) : 0.0f;
-            if (a.resid) load_four<T>((const T*)a.resid + row * a.ldr + n, left, r);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += r[e];
-            store_four<T>((T*)a.y + row * a.N + n, left, v);
-        }
-    }
+    ForwardEmit<T> f;
+    f.a = &a; f.begin = begin; f.count = end - begin; f.n0 = n0; f.live = live;
+    f.init(g, (threadIdx.x >> 6) / S::WI * (S::BJ / S::WJ) + (int)(threadIdx.x & 63) % (S::MJ * 16 / f.V) * f.V);
+    tile_emit<T, S>(acc, lds, f);
 }
 
 // dx = dz W: rows of dz, W contraction-major
@@ -141,21 +187,21 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
     B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0) + k0; B.order = nullptr; B.ld = a.ldw; B.row0 = 0; B.rows = 0; B.klen = a.N; B.cols = a.K - k0;
     tile_product<T, false, true, S, DMA>(A, B, live ? a.Np : 0, lds, acc);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), j0 = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);
+    struct Emit {
+        typedef int Pre;
+        const DxArgs* a;
+        int begin, count, k0;
+        __device__ __forceinline__ int pre(int i, int) const { return i < count ? (a->rows.order ? a->rows.order[begin + i] : begin + i) : -1; }
+        __device__ __forceinline__ void emit(int row, int, int j, float (&v)[16 / sizeof(T)]) const {
+            const int left = a->K - k0 - j;
+            if (row < 0 || left <= 0) return;
+            typename Elem<T>::Frag o;
 #pragma unroll
-    for (int mi = 0; mi < S::MI; ++mi) {
-        const int at = begin + i0 + 16 * mi;
-        if (at >= end) continue;
-        const int64_t row = a.rows.order ? a.rows.order[at] : at;
-#pragma unroll
-        for (int mj = 0; mj < S::MJ; ++mj) {
-            const int k = k0 + j0 + 16 * mj, left = a.K - k;
-            if (left <= 0) continue;
-            const float v[4] = {acc[mi][mj][0], acc[mi][mj][1], acc[mi][mj][2], acc[mi][mj][3]};
-            store_four<T>((T*)a.dx + row * a.K + k, left, v);
+            for (int e = 0; e < 16 / (int)sizeof(T); ++e) o[e] = (T)v[e];
+            store_chunk<T>((T*)a->dx + (int64_t)row * a->K + k0 + j, left, o);
         }
-    }
+    } f = {&a, begin, end - begin, k0};
+    tile_emit<T, S>(acc, lds, f);
 }
 
 // dW[g] = sum over the group's rows of dz^T x: both operands contraction-major.  `splits` workgroups share a group's rows
@@ -166,6 +212,20 @@ struct DwArgs {
     void* dw;                   // T [G][N][K], or float partial sums if splits > 1
     int64_t lddz, ldx;
     int K, N, Np, n_ti, n_tj, splits;
+};
+template <typename O> struct DwEmit {
+    typedef int Pre;
+    O* out;
+    int N, K, n0, k0;
+    __device__ __forceinline__ int pre(int, int) const { return 0; }
+    __device__ __forceinline__ void emit(int, int i, int j, float (&v)[16 / sizeof(O)]) const {
+        const int n = n0 + i, left = K - k0 - j;
+        if (n >= N || left <= 0) return;
+        typename Elem<O>::Frag o;
+#pragma unroll
+        for (int e = 0; e < 16 / (int)sizeof(O); ++e) o[e] = (O)v[e];
+        store_chunk<O>(out + (int64_t)n * K + k0 + j, left, o);
+    }
 };
 template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_dw_kernel(DwArgs a) {
     typedef Operand<T, true, S::BI, S::NT> OA;
@@ -191,21 +251,13 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
     B.base = (const T*)a.x + k0; B.order = a.rows.order; B.ld = a.ldx; B.row0 = begin; B.rows = 0; B.klen = end - begin; B.cols = a.K - k0;
     tile_product<T, true, true, S, DMA>(A, B, end - begin, lds, acc);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), j0 = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);
     const int64_t plane = (int64_t)a.N * a.K;
-#pragma unroll
-    for (int mi = 0; mi < S::MI; ++mi) {
-        const int n = n0 + i0 + 16 * mi;
-        if (n >= a.N) continue;
-#pragma unroll
-        for (int mj = 0; mj < S::MJ; ++mj) {
-            const int k = k0 + j0 + 16 * mj, left = a.K - k;
-            if (left <= 0) continue;
-            const float v[4] = {acc[mi][mj][0], acc[mi][mj][1], acc[mi][mj][2], acc[mi][mj][3]};
-            if (a.splits > 1) store_four<float>((float*)a.dw + ((int64_t)s * a.rows.G + g) * plane + (int64_t)n * a.K + k, left, v);
-            else store_four<T>((T*)a.dw + (int64_t)g * plane + (int64_t)n * a.K + k, left, v);
-        }
+    if (a.splits > 1) {
+        DwEmit<float> f = {(float*)a.dw + ((int64_t)s * a.rows.G + g) * plane, a.N, a.K, n0, k0};
+        tile_emit<float, S>(acc, lds, f);
+    } else {
+        DwEmit<T> f = {(T*)a.dw + (int64_t)g * plane, a.N, a.K, n0, k0};
+        tile_emit<T, S>(acc, lds, f);
     }
 }
 // out[e] = sum over splits of part[s][e], s ascending

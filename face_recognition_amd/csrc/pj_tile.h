@@ -59,6 +59,15 @@ template <typename T> __device__ __forceinline__ typename Elem<T>::Frag load_chu
     }
     return v;
 }
+template <typename T> __device__ __forceinline__ void store_chunk(T* p, int n, typename Elem<T>::Frag v) {
+    if (n >= Elem<T>::EPC) {
+        reinterpret_cast<Chunk<T>*>(p)->v = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < Elem<T>::EPC; ++e)
+            if (e < n) p[e] = v[e];
+    }
+}
 template <typename T> __device__ __forceinline__ void load_four(const T* p, int n, float (&o)[4]) {
     if (n >= 4) {
         const typename Elem<T>::Quad v = reinterpret_cast<const Four<T>*>(p)->v;
@@ -250,6 +259,46 @@ template <int BI_, int BJ_, int WI_, int WJ_> struct Shape {
     static constexpr int BI = BI_, BJ = BJ_, WI = WI_, WJ = WJ_, NT = 64 * WI * WJ;
     static constexpr int MI = BI / WI / 16, MJ = BJ / WJ / 16;
 };
+
+// Hands a workgroup's results on as 16-byte pieces of rows: a wave turns its accumulators through its own part of LDS, 16 rows
+// at a time (written as a lane's four neighbouring columns, pitch + 16 bytes: no bank conflicts; read as V neighbouring
+// columns, so that eight or sixteen lanes cover a row's whole line), and calls
+//     pre(i, j)           for every piece first (loads that the results wait for go out together), then
+//     emit(state, i, j, v)  with the V = 16 / sizeof(T) values of row i, columns j .. j + V of the tile.
+// `lds` is free when every wave is past the last step's barrier.
+template <typename T, typename S, typename F> __device__ __forceinline__ void tile_emit(const f32x4 (&acc)[S::MI][S::MJ], char* lds, const F& f) {
+    constexpr int COLS = S::MJ * 16, V = 16 / sizeof(T), LPR = COLS / V, RPP = 64 / LPR, NP = 16 / RPP, PITCH = COLS + 4;
+    static_assert(S::WI * S::WJ * 16 * PITCH * 4 <= 2 * (S::BI + S::BJ) * 128, "the strips fit the tiles' buffers");
+    static_assert(16 % RPP == 0, "whole passes per strip");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
+    float* strip = reinterpret_cast<float*>(lds) + wave * (16 * PITCH);
+    const int r = lane / LPR, c = (lane % LPR) * V;
+    typename F::Pre pre[S::MI * NP];
+#pragma unroll
+    for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) pre[mi * NP + p] = f.pre(i0 + 16 * mi + p * RPP + r, j0 + c);
+#pragma unroll
+    for (int mi = 0; mi < S::MI; ++mi) {
+#pragma unroll
+        for (int mj = 0; mj < S::MJ; ++mj)
+            *reinterpret_cast<f32x4*>(strip + (lane & 15) * PITCH + 16 * mj + 4 * (lane >> 4)) = acc[mi][mj];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            float v[V];
+#pragma unroll
+            for (int q = 0; q < V / 4; ++q) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(strip + (p * RPP + r) * PITCH + c + 4 * q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e];
+            }
+            f.emit(pre[mi * NP + p], i0 + 16 * mi + p * RPP + r, j0 + c, v);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
 
 // The MFMAs of one step on the tiles in LDS.
 template <typename T, bool AK, bool BK, typename S>
