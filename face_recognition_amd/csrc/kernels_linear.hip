@@ -4,9 +4,11 @@
 //   forward      z = x W^T + b,  y = act(z) + r         rows of one group against that group's matrix
 //   backward     dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = sum dz;  dslope = sum dy min(z, 0);  dr = dy
 //
-// A row list (`order`, stable by group) stands between the rows in memory and the tiles: a tile gathers its rows through it
-// and scatters its results back, so nothing is permuted in memory.  Sums are fp32; z and dz are rounded once to the product's
-// type (they are operands of the matrix instructions / of act' only, the same half step as the outputs').
+// A row list (`order`, stable by group) stands between the rows in memory and the tiles: a tile of the forward product gathers
+// its rows through it and scatters its results back.  The backward pass sorts once, while it reads anyway: dz lies in list
+// order, x is copied into it for dW, and both gradients' products then run over contiguous rows.  Sums are fp32; z and dz are
+// rounded once to the product's type (they are operands of the matrix instructions / of act' only, the same half step as the
+// outputs').
 #include "pj_tile.h"
 
 namespace fra {
@@ -55,6 +57,18 @@ template <typename T> __device__ __forceinline__ float pj_act_grad(int act, floa
             return q + z * q * (1.0f - q) * GELU_C * (1.0f + 3.0f * GELU_A * z * z);
         }
         default: return 1.0f;
+    }
+}
+
+template <typename T, int V> __device__ __forceinline__ void pj_act_grad_all(int act, typename Elem<T>::Frag z, const float (&s)[V], float (&d)[V]) {
+    switch (act) {
+#define PJ_CASE(A)                                                \
+    case A:                                                       \
+        _Pragma("unroll") for (int e = 0; e < V; ++e) d[e] = pj_act_grad<T>(A, (float)z[e], s[e]); \
+        break;
+        PJ_CASE(PJ_RELU) PJ_CASE(PJ_PRELU) PJ_CASE(PJ_SILU) PJ_CASE(PJ_GELU_TANH)
+#undef PJ_CASE
+        default: break;
     }
 }
 
@@ -142,8 +156,6 @@ template <typename T> struct ForwardEmit {
     }
 };
 template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_forward_kernel(FwdArgs a) {
-    typedef Operand<T, false, S::BI, S::NT> OA;
-    typedef Operand<T, false, S::BJ, S::NT> OB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
     int g, begin, end;
@@ -151,9 +163,9 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
     const bool live = g < a.rows.G;                                 // group G: rows of no group
     const int n0 = ct * S::BJ;
     f32x4 acc[S::MI][S::MJ];
-    OA A;
+    OperandA<T, false, S> A;
     A.base = (const T*)a.x; A.order = a.rows.order; A.ld = a.ldx; A.row0 = begin; A.rows = end - begin; A.klen = a.K; A.cols = 0;
-    OB B;
+    OperandB<T, false, S> B;
     B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0); B.order = nullptr; B.ld = a.ldw; B.row0 = n0; B.rows = a.N - n0; B.klen = a.K; B.cols = 0;
     tile_product<T, false, false, S, DMA>(A, B, live ? a.K : 0, lds, acc);
 
@@ -163,17 +175,81 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
     tile_emit<T, S>(acc, lds, f);
 }
 
-// dx = dz W: rows of dz, W contraction-major
+// The same for few rows (tiles of 16 MT): a workgroup takes 16 columns, its four waves every fourth group of k, and their sums
+// meet in LDS, wave 0's first.  Bound by the latency of one trip to memory, or by W's bytes: a column's weights are read once,
+// straight into MFMA operands, in pieces of 64 bytes of sixteen rows whose neighbours the other waves take.
+template <typename T, int MT> __global__ __launch_bounds__(256) void pj_few_rows_kernel(FwdArgs a) {
+    typedef typename Elem<T>::Frag Frag;
+    constexpr int KG = Elem<T>::KG, EPC = Elem<T>::EPC, U = MT == 4 ? 2 : 4;
+    __shared__ float red[4][MT][16][17];
+    const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
+    int g, begin, end;
+    if (!row_tile(a.rows, rt, 16 * MT, g, begin, end)) return;
+    const bool live = g < a.rows.G;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, q = lane >> 4, n0 = ct * 16;
+    if (live) {
+        f32x4 acc[MT];
+        const T* xr[MT];
+        const T* wr = (const T*)a.w + (int64_t)g * a.wg + (int64_t)(n0 + m < a.N ? n0 + m : a.N - 1) * a.ldw + q * EPC;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            acc[i] = zero;
+            const int at = begin + 16 * i + m < end ? begin + 16 * i + m : end - 1;
+            xr[i] = (const T*)a.x + (int64_t)(a.rows.order ? a.rows.order[at] : at) * a.ldx + q * EPC;
+        }
+        for (int k0 = wave * KG; k0 < a.K; k0 += 4 * KG * U) {
+            Frag w[U], x[U][MT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = k0 + u * 4 * KG, left = a.K - k - q * EPC;
+                w[u] = load_chunk<T>(wr + k, left);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) x[u][i] = load_chunk<T>(xr[i] + k, left);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[i] = pj_mma<T>(w[u], x[u][i], acc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[wave][i][m][4 * q + e] = acc[i][e];
+    }
+    __syncthreads();
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, n = n0 + c;
+    if (n >= a.N) return;
+    float bi = 0.0f, sl = 0.0f;
+    if (live && a.bias) bi = a.bias_f32 ? ((const float*)a.bias)[(int64_t)g * a.N + n] : (float)((const T*)a.bias)[(int64_t)g * a.N + n];
+    if (live && a.slope) sl = a.slope_f32 ? ((const float*)a.slope)[(int64_t)g * a.N + n] : (float)((const T*)a.slope)[(int64_t)g * a.N + n];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int at = begin + 16 * i + r;
+        if (at >= end) continue;
+        const int64_t row = a.rows.order ? a.rows.order[at] : at;
+        float v = 0.0f;
+        if (live) {
+            v = ((red[0][i][r][c] + red[1][i][r][c]) + (red[2][i][r][c] + red[3][i][r][c])) + bi;
+            if (a.z) ((T*)a.z)[row * a.N + n] = (T)v;
+            v = pj_act<T>(a.act, v, sl);
+        }
+        if (a.resid) v += (float)((const T*)a.resid)[row * a.ldr + n];
+        ((T*)a.y)[row * a.N + n] = (T)v;
+    }
+}
+
+// ---- backward: everything the products read lies in rows of whole aligned chunks, in list order
+
+// dx = dz W, scattered back to the rows
 struct DxArgs {
     RowArgs rows;
     const void *dz, *w;
     void* dx;
     int64_t lddz, ldw, wg;
-    int K, N, Np, n_col_tiles;  // Np: columns of dz, zeros from N on (its pitch if it lies in the workspace, else N)
+    int K, Kp, N, Np, n_col_tiles;      // Np, Kp: columns of dz and W, zeros past N and K
 };
-template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_dx_kernel(DxArgs a) {
-    typedef Operand<T, false, S::BI, S::NT> OA;
-    typedef Operand<T, true, S::BJ, S::NT> OB;
+template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dx_kernel(DxArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
     int g, begin, end;
@@ -181,12 +257,11 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
     const bool live = g < a.rows.G;
     const int k0 = ct * S::BJ;
     f32x4 acc[S::MI][S::MJ];
-    OA A;
-    A.base = (const T*)a.dz; A.order = a.rows.order; A.ld = a.lddz; A.row0 = begin; A.rows = end - begin; A.klen = a.Np; A.cols = 0;
-    OB B;
-    B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0) + k0; B.order = nullptr; B.ld = a.ldw; B.row0 = 0; B.rows = 0; B.klen = a.N; B.cols = a.K - k0;
-    tile_product<T, false, true, S, DMA>(A, B, live ? a.Np : 0, lds, acc);
-
+    OperandA<T, false, S> A;
+    A.base = (const T*)a.dz; A.order = nullptr; A.ld = a.lddz; A.row0 = begin; A.rows = end - begin; A.klen = a.Np; A.cols = 0;
+    OperandB<T, true, S> B;
+    B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0) + k0; B.order = nullptr; B.ld = a.ldw; B.row0 = 0; B.rows = 0; B.klen = a.N; B.cols = a.Kp - k0;
+    tile_product<T, false, true, S, true>(A, B, live ? a.Np : 0, lds, acc);
     struct Emit {
         typedef int Pre;
         const DxArgs* a;
@@ -204,14 +279,14 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
     tile_emit<T, S>(acc, lds, f);
 }
 
-// dW[g] = sum over the group's rows of dz^T x: both operands contraction-major.  `splits` workgroups share a group's rows
-// and leave fp32 partial sums [split][G][N][K], which pj_join_kernel adds in order; one split writes dW itself.
+// dW[g] = sum over the group's rows of dz^T x: both operands k-major.  `splits` workgroups share a group's rows and leave fp32
+// partial sums [split][G][N][K], which pj_join_kernel adds in order; one split writes dW itself.
 struct DwArgs {
     RowArgs rows;
     const void *dz, *x;
     void* dw;                   // T [G][N][K], or float partial sums if splits > 1
     int64_t lddz, ldx;
-    int K, N, Np, n_ti, n_tj, splits;
+    int K, Kp, N, Np, n_ti, n_tj, splits;
 };
 template <typename O> struct DwEmit {
     typedef int Pre;
@@ -227,9 +302,7 @@ template <typename O> struct DwEmit {
         store_chunk<O>(out + (int64_t)n * K + k0 + j, left, o);
     }
 };
-template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_dw_kernel(DwArgs a) {
-    typedef Operand<T, true, S::BI, S::NT> OA;
-    typedef Operand<T, true, S::BJ, S::NT> OB;
+template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dw_kernel(DwArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     unsigned b = blockIdx.x;
     const int tj = b % a.n_tj; b /= a.n_tj;
@@ -237,20 +310,20 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
     const int s = b % a.splits, g = b / a.splits;
     int begin = a.rows.offsets ? a.rows.offsets[g] : 0, end = a.rows.offsets ? a.rows.offsets[g + 1] : a.rows.M;
     if (a.splits > 1) {                                             // whole steps per split
-        const int steps = (end - begin + Elem<T>::KSTEP - 1) / Elem<T>::KSTEP;
-        const int per = (steps + a.splits - 1) / a.splits * Elem<T>::KSTEP;
+        const int step = S::KS * Elem<T>::KG;
+        const int steps = (end - begin + step - 1) / step;
+        const int per = (steps + a.splits - 1) / a.splits * step;
         const int64_t b0 = (int64_t)begin + (int64_t)s * per, e0 = b0 + per;
         begin = b0 < end ? (int)b0 : end;
         end = e0 < end ? (int)e0 : end;
     }
     const int n0 = ti * S::BI, k0 = tj * S::BJ;
     f32x4 acc[S::MI][S::MJ];
-    OA A;
-    A.base = (const T*)a.dz + n0; A.order = a.rows.order; A.ld = a.lddz; A.row0 = begin; A.rows = 0; A.klen = end - begin; A.cols = a.Np - n0;
-    OB B;
-    B.base = (const T*)a.x + k0; B.order = a.rows.order; B.ld = a.ldx; B.row0 = begin; B.rows = 0; B.klen = end - begin; B.cols = a.K - k0;
-    tile_product<T, true, true, S, DMA>(A, B, end - begin, lds, acc);
-
+    OperandA<T, true, S> A;
+    A.base = (const T*)a.dz + n0; A.order = nullptr; A.ld = a.lddz; A.row0 = begin; A.rows = 0; A.klen = end - begin; A.cols = a.Np - n0;
+    OperandB<T, true, S> B;
+    B.base = (const T*)a.x + k0; B.order = nullptr; B.ld = a.ldx; B.row0 = begin; B.rows = 0; B.klen = end - begin; B.cols = a.Kp - k0;
+    tile_product<T, true, true, S, true>(A, B, end - begin, lds, acc);
     const int64_t plane = (int64_t)a.N * a.K;
     if (a.splits > 1) {
         DwEmit<float> f = {(float*)a.dw + ((int64_t)s * a.rows.G + g) * plane, a.N, a.K, n0, k0};
@@ -264,9 +337,11 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) 
 template <typename T> __global__ __launch_bounds__(256) void pj_join_kernel(const float* part, T* out, int64_t n, int splits) {
     const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (e >= n) return;
-    float v[4] = {0, 0, 0, 0}, o[4];
+    float v[4] = {0, 0, 0, 0};
     const int left = n - e < 4 ? (int)(n - e) : 4;
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
+        float o[4];
         load_four<float>(part + (int64_t)s * n + e, left, o);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += o[i];
@@ -274,113 +349,191 @@ template <typename T> __global__ __launch_bounds__(256) void pj_join_kernel(cons
     store_four<T>(out + e, left, v);
 }
 
-// dz = dy act'(z) and, per row tile, the column sums of dz and of dy min(z, 0).  A workgroup takes one row tile x 256 columns,
-// wave w its rows w, w + 4, ...; the waves' sums meet in LDS.
+// dz = dy act'(z) in list order and, per row tile, the column sums of dz and of dy min(z, 0).  A workgroup takes one row tile x
+// `lpr` 16-byte pieces of columns (lpr lanes side by side, a power of two up to 64; 256 / lpr rows at a time); four rows per
+// lane are requested together.  Bound by HBM: dy and z in, dz out.
 struct DzArgs {
     RowArgs rows;
     const void *dy, *z, *slope;
     void* dz;                   // [M][Np], zeros from column N on; nullptr: dz = dy, only the sums are wanted
     float *part_b, *part_s;     // [tiles][N], nullptr where not wanted
     int64_t lddy;
-    int N, Np, act, slope_f32, tile_rows, n_col_tiles;
+    int N, Np, act, slope_f32, tile_rows, n_col_tiles, lpr_log2;
 };
 template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs a) {
-    __shared__ f32x4 sums[2][4][64];
+    typedef typename Elem<T>::Frag Frag;
+    constexpr int V = Elem<T>::EPC, U = 4;
+    __shared__ float sums[256][V + 1];
     const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
     int g, begin, end;
     if (!row_tile(a.rows, rt, a.tile_rows, g, begin, end) || g >= a.rows.G) return;     // the same for the whole workgroup
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = ct * 256 + lane * 4, left = a.N - n;
-    float sb[4] = {0, 0, 0, 0}, ss[4] = {0, 0, 0, 0}, sl[4] = {0, 0, 0, 0};
-    if (n < a.Np) {
-        if (a.slope) load_param4<T>(a.slope, a.slope_f32, (int64_t)g * a.N + n, left, sl);
-        for (int at = begin + wave; at < end; at += 4) {
-            const int64_t row = a.rows.order ? a.rows.order[at] : at;
-            float dy[4], z[4] = {0, 0, 0, 0}, d[4];
-            load_four<T>((const T*)a.dy + row * a.lddy + n, left, dy);
-            if (a.act != PJ_NONE) load_four<T>((const T*)a.z + row * a.N + n, left, z);
+    const int lpr = 1 << a.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> a.lpr_log2, nsub = 256 >> a.lpr_log2;
+    const int n = (ct * lpr + lane) * V, left = a.N - n;
+    float sb[V], ss[V], sl[V];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                d[e] = a.act != PJ_NONE ? dy[e] * pj_act_grad<T>(a.act, z[e], sl[e]) : dy[e];
-                sb[e] += d[e];
-                ss[e] += z[e] > 0.0f ? 0.0f : dy[e] * z[e];
+    for (int e = 0; e < V; ++e) sb[e] = ss[e] = sl[e] = 0.0f;
+    if (n < a.Np) {
+        if (a.slope) {
+#pragma unroll
+            for (int q = 0; q < V; q += 4) {
+                float s4[4];
+                load_param4<T>(a.slope, a.slope_f32, (int64_t)g * a.N + n + q, left - q, s4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sl[q + e] = s4[e];
             }
-            if (a.dz) store_four<T>((T*)a.dz + row * a.Np + n, 4, d);
+        }
+        for (int at0 = begin + sub; at0 < end; at0 += nsub * U) {
+            Frag dy[U], z[U];
+            int64_t row[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int at = at0 + u * nsub;
+                row[u] = at >= end ? -1 : a.rows.order ? a.rows.order[at] : at;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int have = row[u] >= 0 ? left : 0;
+                dy[u] = load_chunk<T>((const T*)a.dy + (have > 0 ? row[u] * a.lddy + n : 0), have);
+                if (a.act != PJ_NONE) z[u] = load_chunk<T>((const T*)a.z + (have > 0 ? row[u] * a.N + n : 0), have);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (row[u] < 0) continue;
+                Frag d = dy[u];
+                if (a.act != PJ_NONE) {
+                    float dv[V];
+                    pj_act_grad_all<T, V>(a.act, z[u], sl, dv);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float y = (float)dy[u][e], zv = (float)z[u][e], dz = y * dv[e];
+                        sb[e] += dz;
+                        ss[e] += zv > 0.0f ? 0.0f : y * zv;
+                        d[e] = (T)dz;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) sb[e] += (float)dy[u][e];
+                }
+                if (a.dz) *reinterpret_cast<Frag*>((T*)a.dz + (int64_t)(at0 + u * nsub) * a.Np + n) = d;
+            }
         }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { sums[0][wave][lane][e] = sb[e]; sums[1][wave][lane][e] = ss[e]; }
-    __syncthreads();
-    if (wave < 2 && left > 0) {
-        float* part = wave == 0 ? a.part_b : a.part_s;
-        if (part) {
-            float v[4];
+    for (int which = 0; which < 2; ++which) {
+        float* part = which == 0 ? a.part_b : a.part_s;
+        if (!part) continue;                                        // the same for the whole workgroup
+        __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                v[e] = (sums[wave][0][lane][e] + sums[wave][1][lane][e]) + (sums[wave][2][lane][e] + sums[wave][3][lane][e]);
-            store_four<float>(part + (int64_t)rt * a.N + n, left, v);
+        for (int e = 0; e < V; ++e) sums[threadIdx.x][e] = which == 0 ? sb[e] : ss[e];
+        __syncthreads();
+        for (int c = threadIdx.x; c < lpr * V; c += 256) {
+            const int col = ct * lpr * V + c;
+            if (col >= a.N) continue;
+            float v = 0.0f;
+            for (int s = 0; s < nsub; ++s) v += sums[(s << a.lpr_log2) + c / V][c % V];
+            part[(int64_t)rt * a.N + col] = v;
         }
     }
 }
-// out[g][n] = sum of part[t][n] over the group's tiles, in order: 4 waves take every fourth tile of 64 columns
-template <typename T> __global__ __launch_bounds__(256) void pj_colsum_kernel(const float* part, const int* tile_offsets, int n_tiles,
-                                                                             int N, int n_col_tiles, void* out, int out_f32) {
-    __shared__ float sums[4][64];
-    const int ct = blockIdx.x % n_col_tiles, g = blockIdx.x / n_col_tiles;
+// out[g][n] = sum of part[t][n] over the group's tiles: 16 waves take every sixteenth tile of 64 columns, their sums are added in
+// order.  blockIdx.y: bias / slope
+struct ColsumArgs {
+    const float* part[2];
+    void* out[2];
+    int out_f32[2];
+    const int* tile_offsets;
+    int n_tiles, N, n_col_tiles;
+};
+template <typename T> __global__ __launch_bounds__(1024) void pj_colsum_kernel(ColsumArgs a) {
+    __shared__ float sums[16][64];
+    const int which = blockIdx.y;
+    if (!a.out[which]) return;
+    const int ct = blockIdx.x % a.n_col_tiles, g = blockIdx.x / a.n_col_tiles;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = ct * 64 + lane;
-    const int t0 = tile_offsets ? tile_offsets[g] : 0, t1 = tile_offsets ? tile_offsets[g + 1] : n_tiles;
+    const int t0 = a.tile_offsets ? a.tile_offsets[g] : 0, t1 = a.tile_offsets ? a.tile_offsets[g + 1] : a.n_tiles;
     float v = 0.0f;
-    if (n < N)
-        for (int t = t0 + wave; t < t1; t += 4) v += part[(int64_t)t * N + n];
+    if (n < a.N) {
+#pragma unroll 4
+        for (int t = t0 + wave; t < t1; t += 16) v += a.part[which][(int64_t)t * a.N + n];
+    }
     sums[wave][lane] = v;
     __syncthreads();
-    if (wave == 0 && n < N) {
-        v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
-        if (out_f32) ((float*)out)[(int64_t)g * N + n] = v;
-        else ((T*)out)[(int64_t)g * N + n] = (T)v;
+    if (wave == 0 && n < a.N) {
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) v += sums[w][lane];
+        if (a.out_f32[which]) ((float*)a.out[which])[(int64_t)g * a.N + n] = v;
+        else ((T*)a.out[which])[(int64_t)g * a.N + n] = (T)v;
+    }
+}
+// rows of `src` (through `order`, or row r of group r / per_group) to rows of whole aligned chunks, zeros past `cols`
+struct PackArgs {
+    const void* src;
+    void* dst;
+    const int* order;
+    const int* count;           // rows to copy (device), nullptr: `rows`
+    int64_t ld, gs;
+    int rows, per_group, cols, cpr;     // cpr: chunks per row of dst
+};
+template <typename T> __global__ __launch_bounds__(256) void pj_pack_kernel(PackArgs a) {
+    typedef typename Elem<T>::Frag Frag;
+    const int64_t n = (int64_t)(a.count ? *a.count : a.rows) * a.cpr, stride = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+        const int r = (int)(i / a.cpr), c = (int)(i - (int64_t)r * a.cpr) * Elem<T>::EPC;
+        const T* p = (const T*)a.src;
+        if (a.order) p += (int64_t)a.order[r] * a.ld;
+        else if (a.per_group) p += (int64_t)(r / a.per_group) * a.gs + (int64_t)(r % a.per_group) * a.ld;
+        else p += (int64_t)r * a.ld;
+        reinterpret_cast<Frag*>(a.dst)[i] = load_chunk<T>(p + c, a.cols - c);
     }
 }
 
 // ---- rows by group: a stable counting sort --------------------------------------------------------------------------
-// key = id, or G where id is outside [0, G).  Workgroup b of `nb` owns rows [b R, (b + 1) R), its four waves consecutive
-// quarters of them.  A wave walks over 64 rows at a time: lanes with the same key find each other by ballots over the key's
-// bits, so a row's rank among its wave's rows of the key is the wave's running count plus the equal lanes below, without
-// atomics, and the order does not depend on timing.
-constexpr int GR_MAX_GROUPS = 4096;
+// key = id, or G where id is outside [0, G).  A workgroup of NW waves owns NW * 256 consecutive rows, a wave 256 of them, kept
+// as four keys per lane.  Lanes with the same key find each other by ballots over the key's bits, so a row's rank among its
+// wave's rows of the key is the wave's running count plus the equal lanes below: no atomics, and the order does not depend on
+// timing.  One launch for one workgroup; else the counts of all workgroups first.
+constexpr int GR_MAX_GROUPS = 4096, GR_KEYS = 4, GR_WAVE_ROWS = 64 * GR_KEYS;
+constexpr int GR_WIDE_KEYS = 1025;          // up to this many keys sixteen waves' counters fit in LDS, beyond it four waves'
+constexpr int GR_INLINE_SCAN = 8192;        // counters up to which every workgroup adds the others' counts itself
 struct GroupArgs {
     const void* ids;
-    int ids64, M, G, nb, rows_per_block, tile_rows, n_tiles;
-    int* counts;                // [nb][G + 1]: a block's rows of a key; after the scan: list entries of the key before the block
+    int ids64, M, G, nb, bits, tile_rows, n_tiles, scanned;
+    int* counts;                // [nb][G + 1]: a workgroup's rows of a key (scanned: list entries of the key before it), then totals
     int *order, *offsets, *tile_offsets;    // [M], [G + 1], [G + 2]
     int4* tiles;
 };
-__device__ __forceinline__ int group_key(const GroupArgs& a, int row) {
-    const int64_t id = a.ids64 ? ((const int64_t*)a.ids)[row] : ((const int*)a.ids)[row];
-    return id >= 0 && id < a.G ? (int)id : a.G;
-}
-// running counts of this wave in cnt[key]; place == true: writes order[] at cnt[key] + rank, cnt then holding list positions
-template <bool PLACE> __device__ __forceinline__ void group_walk(const GroupArgs& a, int begin, int end, int bits, int* cnt, int lane) {
-    for (int r0 = begin; r0 < end; r0 += 64) {
-        const int row = r0 + lane;
-        const bool in = row < end;
-        const int key = in ? group_key(a, row) : 0;
-        unsigned long long same = __ballot(in);
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long m = __ballot((key >> b) & 1);
-            same &= ((key >> b) & 1) ? m : ~m;
+// ranks the wave's rows among its rows of the same key; cnt[key] ends as the count
+__device__ __forceinline__ void group_rank(const GroupArgs& a, int64_t first, int* cnt, int lane, int (&key)[GR_KEYS], int (&rank)[GR_KEYS]) {
+#pragma unroll
+    for (int i = 0; i < GR_KEYS; ++i) {
+        const int64_t row = first + 64 * i + lane;
+        key[i] = -1;
+        if (row < a.M) {
+            const int64_t id = a.ids64 ? ((const int64_t*)a.ids)[row] : ((const int*)a.ids)[row];
+            key[i] = id >= 0 && id < a.G ? (int)id : a.G;
         }
-        const int below = __popcll(same & ((1ull << lane) - 1)), all = __popcll(same);
-        int at = 0;
-        if (in) at = cnt[key];
-        if (PLACE && in) a.order[at + below] = row;
+    }
+#pragma unroll
+    for (int i = 0; i < GR_KEYS; ++i) {
+        const bool in = key[i] >= 0;
+        unsigned long long same = __ballot(in);
+        if (!same) break;
+        for (int b = 0; b < a.bits; ++b) {
+            const unsigned long long m = __ballot((key[i] >> b) & 1);
+            same &= ((key[i] >> b) & 1) ? m : ~m;
+        }
+        const int below = __popcll(same & ((1ull << lane) - 1));
+        const int at = in ? cnt[key[i]] : 0;
+        rank[i] = at + below;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (in && below == 0) cnt[key] = at + all;
+        if (in && below == 0) cnt[key[i]] = at + __popcll(same);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the next rows' lanes read what this row's leader wrote
     }
 }
-// exclusive sums over 256 threads' values; returns this thread's, total to every thread
+// exclusive sums over the workgroup's values; returns this thread's, `total` to every thread
 __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
     int x = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -391,32 +544,38 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
     if (lane == 63) tmp[wave] = x;
     __syncthreads();
     int base = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) base += w < wave ? tmp[w] : 0;
-    total = tmp[0] + tmp[1] + tmp[2] + tmp[3];
+    total = 0;
+    for (int w = 0; w < nw; ++w) {
+        base += w < wave ? tmp[w] : 0;
+        total += tmp[w];
+    }
     return base + x - v;
 }
-// totals[key] -> offsets, tile_offsets, the tile table and (in totals) every key's first list entry
-__device__ __forceinline__ void group_tables(const GroupArgs& a, int* totals, int* tofs, int* tmp) {
-    const int keys = a.G + 1;
+// totals[key] -> every key's first list entry (in place), tofs[key] its first tile; WRITE: offsets, tile_offsets and the tiles
+template <bool WRITE> __device__ __forceinline__ void group_tables(const GroupArgs& a, int* totals, int* tofs, int* tmp) {
+    const int keys = a.G + 1, nt = blockDim.x;
     int base = 0, tbase = 0;
-    for (int k0 = 0; k0 < keys; k0 += 256) {
+    for (int k0 = 0; k0 < keys; k0 += nt) {
         const int k = k0 + threadIdx.x;
         const int c = k < keys ? totals[k] : 0, tc = (c + a.tile_rows - 1) / a.tile_rows;
-        int tot, ttot;
-        const int o = base + block_scan(c, tmp, tot), to = tbase + block_scan(tc, tmp, ttot);
+        int tot, ttot = 0, to = 0;
+        const int o = base + block_scan(c, tmp, tot);
+        if (WRITE) to = tbase + block_scan(tc, tmp, ttot);
         if (k < keys) {
             totals[k] = o;
-            tofs[k] = to;
-            a.offsets[k] = o;
-            a.tile_offsets[k] = to;
+            if (WRITE) {
+                tofs[k] = to;
+                a.offsets[k] = o;
+                a.tile_offsets[k] = to;
+            }
         }
         base += tot;
         tbase += ttot;
     }
-    if (threadIdx.x == 0) a.tile_offsets[keys] = tbase;
     __syncthreads();
-    for (int t = threadIdx.x; t < a.n_tiles; t += 256) {
+    if (!WRITE) return;
+    if (threadIdx.x == 0) a.tile_offsets[keys] = tbase;
+    for (int t = threadIdx.x; t < a.n_tiles; t += nt) {
         int4 e = {-1, 0, 0, 0};
         if (t < tbase) {
             int lo = 0, hi = keys - 1;                              // the last key whose first tile is <= t
@@ -429,60 +588,91 @@ __device__ __forceinline__ void group_tables(const GroupArgs& a, int* totals, in
             const int end = lo + 1 < keys ? totals[lo + 1] : a.M;
             e.x = lo;
             e.y = first;
-            e.z = first + a.tile_rows < end ? first + a.tile_rows : end;
+            e.z = end - first > a.tile_rows ? first + a.tile_rows : end;
         }
         a.tiles[t] = e;
     }
 }
-__device__ __forceinline__ void wave_range(const GroupArgs& a, int b, int wave, int& begin, int& end) {
-    const int64_t lo = (int64_t)b * a.rows_per_block, q = a.rows_per_block / 4;
-    const int64_t e = lo + (wave + 1) * q, s = lo + wave * q;
-    begin = s < a.M ? (int)s : a.M;
-    end = e < a.M ? (int)e : a.M;
-}
-// MODE 0: everything in one workgroup; 1: a block's counts; 2: place, after pj_group_scan_kernel
-template <int MODE> __global__ __launch_bounds__(256) void pj_group_kernel(GroupArgs a, int bits) {
-    extern __shared__ int cnt[];                                    // [4][keys], mode 0: + totals[keys], tofs[keys]
-    __shared__ int tmp[4];
-    const int keys = a.G + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int begin, end;
-    wave_range(a, blockIdx.x, wave, begin, end);
-    for (int i = threadIdx.x; i < 4 * keys; i += 256) cnt[i] = 0;
+// COUNT: a workgroup's counts; else place (the only workgroup, or after the counts, or after pj_group_scan_kernel)
+template <int NW, bool COUNT> __global__ __launch_bounds__(64 * NW) void pj_group_kernel(GroupArgs a) {
+    extern __shared__ int cnt[];                                    // [NW][keys]; place: + totals[keys], before[keys] (= tofs)
+    __shared__ int tmp[NW];
+    const int keys = a.G + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = 64 * NW;
+    int key[GR_KEYS], rank[GR_KEYS];
+    const int64_t first = ((int64_t)blockIdx.x * NW + wave) * GR_WAVE_ROWS;
+    for (int i = threadIdx.x; i < NW * keys; i += nt) cnt[i] = 0;
     __syncthreads();
-    group_walk<false>(a, begin, end, bits, cnt + wave * keys, lane);
+    group_rank(a, first, cnt + wave * keys, lane, key, rank);
     __syncthreads();
-    if (MODE == 1) {
-        for (int k = threadIdx.x; k < keys; k += 256)
-            a.counts[(int64_t)blockIdx.x * keys + k] = cnt[k] + cnt[keys + k] + cnt[2 * keys + k] + cnt[3 * keys + k];
-        return;
-    }
-    if (MODE == 0) {
-        int* totals = cnt + 4 * keys;
-        for (int k = threadIdx.x; k < keys; k += 256) totals[k] = cnt[k] + cnt[keys + k] + cnt[2 * keys + k] + cnt[3 * keys + k];
-        __syncthreads();
-        group_tables(a, totals, totals + keys, tmp);
-        __syncthreads();
-    }
-    for (int k = threadIdx.x; k < keys; k += 256) {                 // counts -> the wave's first list entry of the key
-        int at = MODE == 0 ? cnt[4 * keys + k] : a.offsets[k] + a.counts[(int64_t)blockIdx.x * keys + k];
+    int* totals = cnt + NW * keys;
+    int* before = totals + keys;
+    if (COUNT || a.nb == 1) {
+        for (int k = threadIdx.x; k < keys; k += nt) {
+            int c = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < NW; ++w) c += cnt[w * keys + k];
+            if (COUNT) a.counts[(int64_t)blockIdx.x * keys + k] = c;
+            else totals[k] = c;
+        }
+        if (COUNT) return;
+        __syncthreads();
+        group_tables<true>(a, totals, before, tmp);
+        __syncthreads();
+        for (int k = threadIdx.x; k < keys; k += nt) before[k] = 0;
+    } else if (a.scanned) {
+        for (int k = threadIdx.x; k < keys; k += nt) {
+            totals[k] = a.offsets[k];
+            before[k] = a.counts[(int64_t)blockIdx.x * keys + k];
+        }
+    } else {
+        for (int k = threadIdx.x; k < keys; k += nt) {
+            int all = 0;
+            for (int b = 0; b < a.nb; ++b) all += a.counts[(int64_t)b * keys + k];
+            totals[k] = all;
+        }
+        __syncthreads();
+        if (blockIdx.x == 0) group_tables<true>(a, totals, before, tmp);
+        else group_tables<false>(a, totals, before, tmp);
+        __syncthreads();
+        for (int k = threadIdx.x; k < keys; k += nt) {
+            int mine = 0;
+            for (int b = 0; b < (int)blockIdx.x; ++b) mine += a.counts[(int64_t)b * keys + k];
+            before[k] = mine;
+        }
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < keys; k += nt) {                  // counts -> the wave's first list entry of the key
+        int at = totals[k] + before[k];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
             const int c = cnt[w * keys + k];
             cnt[w * keys + k] = at;
             at += c;
         }
     }
     __syncthreads();
-    group_walk<true>(a, begin, end, bits, cnt + wave * keys, lane);
+#pragma unroll
+    for (int i = 0; i < GR_KEYS; ++i)
+        if (key[i] >= 0) a.order[cnt[wave * keys + key[i]] + rank[i]] = (int)(first + 64 * i + lane);
 }
 // counts[b][key] -> exclusive sums over b; totals -> tables
-__global__ __launch_bounds__(256) void pj_group_scan_kernel(GroupArgs a) {
-    extern __shared__ int cnt[];
-    __shared__ int tmp[4];
+__global__ __launch_bounds__(1024) void pj_group_scan_kernel(GroupArgs a) {
+    extern __shared__ int cnt[];                                    // totals[keys], tofs[keys]
+    __shared__ int tmp[16];
     const int keys = a.G + 1;
-    for (int k = threadIdx.x; k < keys; k += 256) {
-        int sum = 0;
-        for (int b = 0; b < a.nb; ++b) {
+    for (int k = threadIdx.x; k < keys; k += 1024) {
+        int sum = 0, b = 0;
+        for (; b + 8 <= a.nb; b += 8) {
+            int c[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = a.counts[(int64_t)(b + i) * keys + k];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a.counts[(int64_t)(b + i) * keys + k] = sum;
+                sum += c[i];
+            }
+        }
+        for (; b < a.nb; ++b) {
             const int c = a.counts[(int64_t)b * keys + k];
             a.counts[(int64_t)b * keys + k] = sum;
             sum += c;
@@ -490,13 +680,10 @@ __global__ __launch_bounds__(256) void pj_group_scan_kernel(GroupArgs a) {
         cnt[k] = sum;
     }
     __syncthreads();
-    group_tables(a, cnt, cnt + keys, tmp);
+    group_tables<true>(a, cnt, cnt + keys, tmp);
 }
 
 // ---- launchers ------------------------------------------------------------------------------------------------------
-
-// dynamic LDS of a product kernel: two buffers of both operands' tiles
-template <typename S> constexpr int product_lds() { return 2 * (S::BI + S::BJ) * 128; }
 
 // rows at `p`, `pitches` (one, or several or-ed together) elements apart and `len` long, consist of whole aligned chunks
 template <typename T> static bool dma_ok(const void* p, int64_t pitches, int64_t len) {
@@ -515,8 +702,8 @@ template <typename K> static int raise_lds(K kernel, int bytes, std::atomic<uint
         FRA_HIP(hipGetLastError());                                                      \
     } while (0)
 
-typedef Shape<128, 128, 2, 2> Big;
-typedef Shape<64, 64, 2, 2> Small;
+typedef Shape<128, 128, 2, 2, 1, 4> Big;
+typedef Shape<64, 64, 2, 2, 2, 3> Small;
 
 static int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -560,65 +747,102 @@ static int check_grid(int64_t blocks, const char* what) {
 // 128 x 128 tiles once they fill the 256 compute units, else 64 x 64
 static bool big_tiles(int64_t rows, int64_t cols) { return (int64_t)cdiv(rows, 128) * cdiv(cols, 128) >= 256; }
 
+template <typename T, typename S> static int launch_forward(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
+    a.n_col_tiles = cdiv(d->N, S::BJ);
+    const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
+    if (int rc = check_grid(blocks, "fra_linear")) return rc;
+    if (dma_ok<T>(d->x, d->ldx, d->K) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K))
+        PJ_LAUNCH((pj_forward_kernel<T, S, true>), blocks, S::NT, S::LDS, s, a);
+    else
+        PJ_LAUNCH((pj_forward_kernel<T, S, false>), blocks, S::NT, S::LDS, s, a);
+    return FRA_OK;
+}
+template <typename T, int MT> static int launch_few_rows(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
+    a.n_col_tiles = cdiv(d->N, 16);
+    const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
+    if (int rc = check_grid(blocks, "fra_linear")) return rc;
+    hipLaunchKernelGGL((pj_few_rows_kernel<T, MT>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    FRA_HIP(hipGetLastError());
+    return FRA_OK;
+}
 template <typename T> static int forward_t(const fra_linear_desc* d, void* z, void* y, hipStream_t s) {
     FwdArgs a;
-    const bool big = d->groups ? d->groups->tile_rows == 128 : big_tiles(d->M, d->N);
-    const int bi = big ? 128 : 64;
+    // up to 64 rows: the kernel for few rows; then by the number of tiles
+    const int bi = d->groups ? d->groups->tile_rows : d->M <= 16 ? 16 : d->M <= 32 ? 32 : d->M <= 64 ? 64 : big_tiles(d->M, d->N) ? 128 : 64;
     a.rows = row_args(d, bi);
     a.x = d->x; a.w = d->w; a.bias = d->bias; a.slope = d->slope; a.resid = d->resid; a.z = z; a.y = y;
     a.ldx = d->ldx; a.ldw = d->ldw; a.wg = d->w_group_stride; a.ldr = d->ldr;
     a.K = d->K; a.N = d->N; a.act = d->act; a.bias_f32 = d->bias_dtype == FRA_F32; a.slope_f32 = d->slope_dtype == FRA_F32;
-    a.n_col_tiles = cdiv(d->N, bi);
-    const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
-    if (int rc = check_grid(blocks, "fra_linear")) return rc;
-    const bool dma = dma_ok<T>(d->x, d->ldx, d->K) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
-    if (big && dma) PJ_LAUNCH((pj_forward_kernel<T, Big, true>), blocks, Big::NT, product_lds<Big>(), s, a);
-    else if (big) PJ_LAUNCH((pj_forward_kernel<T, Big, false>), blocks, Big::NT, product_lds<Big>(), s, a);
-    else if (dma) PJ_LAUNCH((pj_forward_kernel<T, Small, true>), blocks, Small::NT, product_lds<Small>(), s, a);
-    else PJ_LAUNCH((pj_forward_kernel<T, Small, false>), blocks, Small::NT, product_lds<Small>(), s, a);
-    return FRA_OK;
+    if (bi == 16) return launch_few_rows<T, 1>(d, a, s);
+    if (bi == 32) return launch_few_rows<T, 2>(d, a, s);
+    if (bi == 64 && !d->groups && d->M <= 64) return launch_few_rows<T, 4>(d, a, s);
+    if (bi == 64) return launch_forward<T, Small>(d, a, s);
+    return launch_forward<T, Big>(d, a, s);
 }
 
 // ---- backward: what goes where in the workspace
 struct BackwardPlan {
-    bool need_dz, need_sums;
-    int dz_rows, n_tiles, splits, Np;
-    size_t off_dz, off_b, off_s, off_part, bytes;
+    bool need_dz, need_sums, pack_x, pack_w;
+    int dz_rows, n_tiles, splits, Np, Kp;
+    size_t off_dz, off_x, off_w, off_b, off_s, off_part, bytes;
 };
-static BackwardPlan backward_plan(const fra_linear_desc* d, bool dx, bool dw, bool db, bool ds) {
+template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc* d, bool dx, bool dw, bool db, bool ds) {
     BackwardPlan p;
-    const int64_t es = d->dtype == FRA_F32 ? 4 : 2;
+    const int64_t es = sizeof(T), epc = Elem<T>::EPC;
     const fra_row_groups* g = d->groups;
     const int G = g ? g->n_groups : 1;
     auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-    // dz gets rows of whole 16-byte chunks, so that the products can fetch it by DMA: without activation, a copy of dy where
-    // N does not give it such rows
-    const int epc = (int)(16 / es);
-    p.Np = (d->N + epc - 1) / epc * epc;
-    p.need_dz = (d->act != PJ_NONE || p.Np != d->N) && (dx || dw);
+    // the products' operands have rows of whole aligned chunks: dz always, a copy of dy included where N does not give it such
+    // rows; copies of x (in list order with groups) and W only where theirs are not
+    p.Np = (int)((d->N + epc - 1) / epc * epc);
+    p.Kp = (int)((d->K + epc - 1) / epc * epc);
+    p.need_dz = dx || dw;
     p.need_sums = db || ds;
+    p.pack_x = dw && (g || !dma_ok<T>(d->x, d->ldx, d->K));
+    p.pack_w = dx && !dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
     p.dz_rows = g ? g->tile_rows : 64;
     p.n_tiles = g ? g->n_tiles : cdiv(d->M, p.dz_rows);
-    // workgroups of dW: enough to fill the chip twice, each with at least four steps of its group's average share
-    const int64_t tiles = (int64_t)cdiv(d->N, 128) * cdiv(d->K, 128) * G;
-    const int64_t steps = cdiv(cdiv(d->M, G), d->dtype == FRA_F32 ? 32 : 64);
+    // workgroups of dW: enough to fill the chip twice, each with at least 256 rows of its group's average share
+    const int64_t tiles = (int64_t)cdiv(d->N, Big::BI) * cdiv(d->K, Big::BJ) * G;
     int64_t sp = (512 + tiles - 1) / tiles;
-    if (sp > steps / 4) sp = steps / 4;
+    if (sp > d->M / G / 256) sp = d->M / G / 256;
     p.splits = dw && sp > 1 ? (int)sp : 1;
     size_t at = 0;
     p.off_dz = at; if (p.need_dz) at += up((size_t)d->M * p.Np * es);
+    p.off_x = at; if (p.pack_x) at += up((size_t)d->M * p.Kp * es);
+    p.off_w = at; if (p.pack_w) at += up((size_t)G * d->N * p.Kp * es);
     p.off_b = at; if (db) at += up((size_t)p.n_tiles * d->N * 4);
     p.off_s = at; if (ds) at += up((size_t)p.n_tiles * d->N * 4);
     p.off_part = at; if (p.splits > 1) at += up((size_t)p.splits * G * d->N * d->K * 4);
     p.bytes = at;
     return p;
 }
+static BackwardPlan backward_plan(const fra_linear_desc* d, bool dx, bool dw, bool db, bool ds) {
+    return d->dtype == FRA_F32 ? backward_plan_t<float>(d, dx, dw, db, ds) : backward_plan_t<f16>(d, dx, dw, db, ds);
+}
 
+template <typename T> static int launch_pack(const PackArgs& a, hipStream_t s) {
+    const int64_t chunks = (int64_t)a.rows * a.cpr, blocks = (chunks + 255) / 256;
+    if (blocks == 0) return FRA_OK;
+    hipLaunchKernelGGL((pj_pack_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a);
+    FRA_HIP(hipGetLastError());
+    return FRA_OK;
+}
+template <typename T, typename S> static int launch_dx(DxArgs& a, hipStream_t s) {
+    a.n_col_tiles = cdiv(a.K, S::BJ);
+    const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
+    if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
+    PJ_LAUNCH((pj_dx_kernel<T, S>), blocks, S::NT, S::LDS, s, a);
+    return FRA_OK;
+}
 template <typename T>
-static int backward_t(const fra_linear_desc* d, const BackwardPlan& p, const void* z, const void* dy, int64_t lddy, void* dx, void* dw,
+static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const void* z, const void* dy, int64_t lddy, void* dx, void* dw,
                       void* db, void* ds, char* ws, hipStream_t s) {
+    BackwardPlan p = plan;
     const fra_row_groups* g = d->groups;
     const int G = g ? g->n_groups : 1;
+    // without groups or activation an aligned dy is dz
+    if (!g && d->act == PJ_NONE && dma_ok<T>(dy, lddy, d->N)) p.need_dz = false;
     if ((p.need_dz || p.need_sums) && d->M > 0) {
         DzArgs a;
         a.rows = row_args(d, p.dz_rows);
@@ -627,49 +851,62 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& p, const voi
         a.part_b = db ? (float*)(ws + p.off_b) : nullptr;
         a.part_s = ds ? (float*)(ws + p.off_s) : nullptr;
         a.lddy = lddy; a.N = d->N; a.Np = p.Np; a.act = d->act; a.slope_f32 = d->slope_dtype == FRA_F32;
-        a.tile_rows = p.dz_rows; a.n_col_tiles = cdiv(p.Np, 256);
+        a.tile_rows = p.dz_rows;
+        const int pieces = p.Np / Elem<T>::EPC;
+        a.lpr_log2 = 0;
+        while (a.lpr_log2 < 6 && (1 << a.lpr_log2) < pieces) ++a.lpr_log2;
+        a.n_col_tiles = cdiv(pieces, 1 << a.lpr_log2);
         const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
         if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
         hipLaunchKernelGGL((pj_dz_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
         FRA_HIP(hipGetLastError());
     }
-    for (int which = 0; which < 2; ++which) {
-        void* out = which == 0 ? db : ds;
-        if (!out) continue;
-        const int ct = cdiv(d->N, 64);
-        if (int rc = check_grid((int64_t)ct * G, "fra_linear_backward")) return rc;
-        hipLaunchKernelGGL((pj_colsum_kernel<T>), dim3((unsigned)ct * G), dim3(256), 0, s, (const float*)(ws + (which == 0 ? p.off_b : p.off_s)),
-                           g ? (const int*)g->tile_offsets : nullptr, p.n_tiles, d->N, ct, out,
-                           (int)((which == 0 ? d->bias_dtype : d->slope_dtype) == FRA_F32));
+    if (p.need_sums) {
+        ColsumArgs a;
+        a.part[0] = (const float*)(ws + p.off_b); a.part[1] = (const float*)(ws + p.off_s);
+        a.out[0] = db; a.out[1] = ds;
+        a.out_f32[0] = d->bias_dtype == FRA_F32; a.out_f32[1] = d->slope_dtype == FRA_F32;
+        a.tile_offsets = g ? (const int*)g->tile_offsets : nullptr;
+        a.n_tiles = p.n_tiles; a.N = d->N; a.n_col_tiles = cdiv(d->N, 64);
+        const int64_t blocks = (int64_t)a.n_col_tiles * G;
+        if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
+        hipLaunchKernelGGL((pj_colsum_kernel<T>), dim3((unsigned)blocks, ds ? 2 : 1), dim3(1024), 0, s, a);
         FRA_HIP(hipGetLastError());
     }
     const void* dz = p.need_dz ? ws + p.off_dz : dy;
     const int64_t lddz = p.need_dz ? p.Np : lddy;
-    const int Np = p.need_dz ? p.Np : d->N;
     if (dx && d->M > 0) {
         DxArgs a;
+        a.w = d->w; a.ldw = d->ldw; a.wg = d->w_group_stride;
+        if (p.pack_w) {
+            PackArgs k;
+            k.src = d->w; k.dst = ws + p.off_w; k.order = nullptr; k.count = nullptr; k.ld = d->ldw; k.gs = d->w_group_stride;
+            FRA_REQUIRE((int64_t)G * d->N <= 2147483647LL, FRA_ERR_ARG, "fra_linear_backward: %d matrices of %d rows", G, d->N);
+            k.rows = G * d->N; k.per_group = d->N; k.cols = d->K; k.cpr = p.Kp / Elem<T>::EPC;
+            if (int rc = launch_pack<T>(k, s)) return rc;
+            a.w = k.dst; a.ldw = p.Kp; a.wg = (int64_t)d->N * p.Kp;
+        }
         const bool big = g ? g->tile_rows == 128 : big_tiles(d->M, d->K);
-        const int bi = big ? 128 : 64;
-        a.rows = row_args(d, bi);
-        a.dz = dz; a.w = d->w; a.dx = dx; a.lddz = lddz; a.ldw = d->ldw; a.wg = d->w_group_stride; a.K = d->K; a.N = d->N; a.Np = Np;
-        a.n_col_tiles = cdiv(d->K, bi);
-        const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
-        if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
-        const bool dma = dma_ok<T>(dz, lddz, Np) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
-        if (big && dma) PJ_LAUNCH((pj_dx_kernel<T, Big, true>), blocks, Big::NT, product_lds<Big>(), s, a);
-        else if (big) PJ_LAUNCH((pj_dx_kernel<T, Big, false>), blocks, Big::NT, product_lds<Big>(), s, a);
-        else if (dma) PJ_LAUNCH((pj_dx_kernel<T, Small, true>), blocks, Small::NT, product_lds<Small>(), s, a);
-        else PJ_LAUNCH((pj_dx_kernel<T, Small, false>), blocks, Small::NT, product_lds<Small>(), s, a);
+        a.rows = row_args(d, big ? 128 : 64);
+        a.dz = dz; a.dx = dx; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
+        if (int rc = big ? launch_dx<T, Big>(a, s) : launch_dx<T, Small>(a, s)) return rc;
     }
     if (dw) {
         DwArgs a;
+        a.x = d->x; a.ldx = d->ldx;
+        if (p.pack_x) {
+            PackArgs k;
+            k.src = d->x; k.dst = ws + p.off_x; k.order = g ? (const int*)g->order : nullptr; k.count = g ? g->offsets + G : nullptr;
+            k.ld = d->ldx; k.gs = 0; k.rows = (int)d->M; k.per_group = 0; k.cols = d->K; k.cpr = p.Kp / Elem<T>::EPC;
+            if (int rc = launch_pack<T>(k, s)) return rc;
+            a.x = k.dst; a.ldx = p.Kp;
+        }
         a.rows = row_args(d, 128);
-        a.dz = dz; a.x = d->x; a.dw = p.splits > 1 ? (void*)(ws + p.off_part) : dw; a.lddz = lddz; a.ldx = d->ldx; a.K = d->K; a.N = d->N; a.Np = Np;
-        a.n_ti = cdiv(d->N, 128); a.n_tj = cdiv(d->K, 128); a.splits = p.splits;
+        a.dz = dz; a.dw = p.splits > 1 ? (void*)(ws + p.off_part) : dw; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
+        a.n_ti = cdiv(d->N, Big::BI); a.n_tj = cdiv(d->K, Big::BJ); a.splits = p.splits;
         const int64_t blocks = (int64_t)a.n_ti * a.n_tj * a.splits * G;
         if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
-        if (dma_ok<T>(dz, lddz, Np) && dma_ok<T>(d->x, d->ldx, d->K)) PJ_LAUNCH((pj_dw_kernel<T, Big, true>), blocks, Big::NT, product_lds<Big>(), s, a);
-        else PJ_LAUNCH((pj_dw_kernel<T, Big, false>), blocks, Big::NT, product_lds<Big>(), s, a);
+        PJ_LAUNCH((pj_dw_kernel<T, Big>), blocks, Big::NT, Big::LDS, s, a);
         if (p.splits > 1) {
             const int64_t n = (int64_t)G * d->N * d->K, jb = (n + 1023) / 1024;
             if (int rc = check_grid(jb, "fra_linear_backward")) return rc;
@@ -680,13 +917,28 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& p, const voi
     return FRA_OK;
 }
 
-static int group_blocks(int64_t M, int& rows_per_block) {
-    // one workgroup up to 4096 rows; beyond, at most 512 of at least 2048 rows
-    int64_t per = M <= 4096 ? 4096 : (M + 511) / 512;
-    if (M > 4096 && per < 2048) per = 2048;
-    per = (per + 255) / 256 * 256;
-    rows_per_block = (int)per;
-    return M > 0 ? cdiv(M, per) : 1;
+static bool group_wide(int n_groups) { return n_groups + 1 <= GR_WIDE_KEYS; }
+static int group_blocks(int64_t M, int n_groups) {
+    const int per = (group_wide(n_groups) ? 16 : 4) * GR_WAVE_ROWS;
+    return M > per ? cdiv(M, per) : 1;
+}
+template <int NW> static int launch_groups(GroupArgs& a, hipStream_t s) {
+    const int keys = a.G + 1, most = (NW == 16 ? GR_WIDE_KEYS : GR_MAX_GROUPS + 1) * 4, lds = (NW + 2) * keys * 4;
+    static std::atomic<uint64_t> done_count{0}, done_place{0};
+    if (int rc = raise_lds(pj_group_kernel<NW, false>, (NW + 2) * most, done_place)) return rc;
+    if (a.nb > 1) {
+        if (int rc = raise_lds(pj_group_kernel<NW, true>, NW * most, done_count)) return rc;
+        hipLaunchKernelGGL((pj_group_kernel<NW, true>), dim3(a.nb), dim3(64 * NW), NW * keys * 4, s, a);
+        FRA_HIP(hipGetLastError());
+        a.scanned = (int64_t)a.nb * keys > GR_INLINE_SCAN;
+        if (a.scanned) {
+            hipLaunchKernelGGL(pj_group_scan_kernel, dim3(1), dim3(1024), 2 * keys * 4, s, a);
+            FRA_HIP(hipGetLastError());
+        }
+    }
+    hipLaunchKernelGGL((pj_group_kernel<NW, false>), dim3(a.nb), dim3(64 * NW), lds, s, a);
+    FRA_HIP(hipGetLastError());
+    return FRA_OK;
 }
 
 }  // namespace fra
@@ -730,9 +982,10 @@ int fra_linear_backward(const fra_linear_desc* d, const void* preact, const void
     return backward_t<f16>(d, p, preact, dy, lddy, dx, dw, dbias, dslope, ws, s);
 }
 
-// rows of a tile: 128 where a group has that many rows on average, else 64
+// rows of a tile, by the rows a group has on average: the kernel for few rows below 24, 64 x 64 tiles below 128
 int fra_group_tile_rows(int64_t rows, int n_groups) {
-    return n_groups >= 1 && rows / n_groups >= 128 ? 128 : 64;
+    const int64_t average = n_groups >= 1 ? rows / n_groups : rows;
+    return average >= 128 ? 128 : average >= 24 ? 64 : 16;
 }
 int fra_group_tiles(int64_t rows, int n_groups) {
     if (rows < 0 || n_groups < 1 || n_groups > GR_MAX_GROUPS) return 0;
@@ -742,8 +995,7 @@ int fra_group_rows_workspace_bytes(int64_t rows, int n_groups, size_t* bytes) {
     FRA_REQUIRE(bytes, FRA_ERR_ARG, "fra_group_rows_workspace_bytes: null pointer");
     FRA_REQUIRE(rows >= 0 && rows <= 2147483647LL - 1024 && n_groups >= 1 && n_groups <= GR_MAX_GROUPS, FRA_ERR_ARG,
                 "fra_group_rows_workspace_bytes: %lld rows, %d groups (1 to %d)", (long long)rows, n_groups, GR_MAX_GROUPS);
-    int per;
-    const int nb = group_blocks(rows, per);
+    const int nb = group_blocks(rows, n_groups);
     *bytes = nb > 1 ? (size_t)nb * (n_groups + 1) * 4 : 0;
     return FRA_OK;
 }
@@ -759,31 +1011,13 @@ int fra_group_rows(const void* ids, int ids_are_64bit, const fra_row_groups* g, 
                 workspace_bytes, need);
     GroupArgs a;
     a.ids = ids; a.ids64 = ids_are_64bit != 0; a.M = (int)g->rows; a.G = g->n_groups; a.tile_rows = g->tile_rows; a.n_tiles = g->n_tiles;
-    a.nb = group_blocks(g->rows, a.rows_per_block);
+    a.nb = group_blocks(a.M, a.G);
     a.counts = (int*)workspace;
     a.order = g->order; a.offsets = g->offsets; a.tile_offsets = g->tile_offsets; a.tiles = (int4*)g->tiles;
-    const int keys = a.G + 1;
-    int bits = 0;
-    while ((1 << bits) < keys) ++bits;
-    hipStream_t s = (hipStream_t)stream;
-    static std::atomic<uint64_t> done0{0}, done1{0}, done2{0};
-    if (a.nb == 1) {
-        const int lds = 6 * keys * 4;
-        if (int rc = raise_lds(pj_group_kernel<0>, 6 * (GR_MAX_GROUPS + 1) * 4, done0)) return rc;
-        hipLaunchKernelGGL((pj_group_kernel<0>), dim3(1), dim3(256), lds, s, a, bits);
-        FRA_HIP(hipGetLastError());
-        return FRA_OK;
-    }
-    const int lds = 4 * keys * 4;
-    if (int rc = raise_lds(pj_group_kernel<1>, 4 * (GR_MAX_GROUPS + 1) * 4, done1)) return rc;
-    if (int rc = raise_lds(pj_group_kernel<2>, 4 * (GR_MAX_GROUPS + 1) * 4, done2)) return rc;
-    hipLaunchKernelGGL((pj_group_kernel<1>), dim3(a.nb), dim3(256), lds, s, a, bits);
-    FRA_HIP(hipGetLastError());
-    hipLaunchKernelGGL(pj_group_scan_kernel, dim3(1), dim3(256), 2 * keys * 4, s, a);
-    FRA_HIP(hipGetLastError());
-    hipLaunchKernelGGL((pj_group_kernel<2>), dim3(a.nb), dim3(256), lds, s, a, bits);
-    FRA_HIP(hipGetLastError());
-    return FRA_OK;
+    a.scanned = 0;
+    a.bits = 0;
+    while ((1 << a.bits) < a.G + 1) ++a.bits;
+    return group_wide(a.G) ? launch_groups<16>(a, (hipStream_t)stream) : launch_groups<4>(a, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -94,16 +94,14 @@ struct OrthArgs {
     int n_col_tiles, transposed;
 };
 template <typename T, bool BK, typename S> __global__ __launch_bounds__(S::NT) void orth_product_kernel(OrthArgs a) {
-    typedef Operand<f16, false, S::BI, S::NT> OA;
-    typedef Operand<f16, BK, S::BJ, S::NT> OB;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
     const int i0 = rt * S::BI, j0 = ct * S::BJ;
     const int64_t b = blockIdx.y;
     f32x4 acc[S::MI][S::MJ];
-    OA A;
+    OperandA<f16, false, S> A;
     A.order = nullptr; A.ld = a.lda; A.row0 = i0; A.rows = a.I - i0; A.klen = a.K; A.cols = 0;
-    OB B;
+    OperandB<f16, BK, S> B;
     B.order = nullptr; B.ld = a.ldb; B.klen = a.K;
     B.row0 = BK ? 0 : j0; B.rows = BK ? 0 : a.J - j0; B.cols = BK ? a.J - j0 : 0;
     const int64_t boff = b * a.sb + (BK ? j0 : 0);
@@ -157,7 +155,7 @@ template <typename T, bool BK, typename S> __global__ __launch_bounds__(S::NT) v
     }
 }
 
-typedef Shape<64, 64, 2, 2> OrthTile;
+typedef Shape<64, 64, 2, 2, 2, 3> OrthTile;
 
 struct OrthPlan {
     OrthDims d;
@@ -201,7 +199,7 @@ static int orth_t(const OrthPlan& p, const T* g, int64_t ldg, int64_t bs, int st
     hipLaunchKernelGGL((orth_split_kernel<T>), dim3((d.np + 63) / 64, (d.m + 63) / 64, d.batch), dim3(256), 0, s, g, ldg, bs, d, part, p.n_part,
                        xh[0], xh[0] + xlo);
     FRA_HIP(hipGetLastError());
-    constexpr int LDS = 2 * (OrthTile::BI + OrthTile::BJ) * 128;
+    constexpr int LDS = OrthTile::LDS;
     static_assert(LDS <= 65536, "no raised limit needed");
     const int ti = (d.m + 63) / 64, tp = (d.mp + 63) / 64, tx = (d.np + 63) / 64;
     for (int t = 0; t < steps; ++t) {

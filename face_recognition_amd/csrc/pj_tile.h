@@ -1,17 +1,15 @@
 // The tiled matrix product behind the projections: C[i][j] = sum_k A(i,k) B(j,k) on one workgroup, fp32 accumulation.
 //
-// Either operand may lie row by row ("row-major": k is the contiguous index) or contraction by contraction
-// ("contraction-major": i or j is contiguous); the four combinations are the forward product, the two gradients and the
-// Gram products, with no transposed copy in memory.  A step covers 128 bytes of k per row: 64 sixteen-bit values (two
-// 16x16x32 MFMAs deep) or 32 floats (eight 16x16x4 MFMAs deep).
+// Either operand may lie row by row ("row-major": k is the contiguous index) or contraction by contraction ("k-major": i or j
+// is contiguous); the combinations are the forward product, the two gradients and the Gram products, with no transposed copy
+// in memory.  A step covers KS groups of k: 32 sixteen-bit values (one 16x16x32 MFMA deep) or 16 floats (four 16x16x4) each.
 //
 // LDS images, in 16-byte chunks:
-//   row-major          [DIM rows][8 chunks of k], chunk c of row r at slot c ^ (r & 7): the sixteen rows a fragment read
-//                      touches fall on all banks;
-//   contraction-major  [KSTEP rows of k][DIM], 16 bit: chunk pair p of row k at p ^ ((k & 3) | (k >> 1 & 4)) (128 columns;
-//                      with 64, two rows of k fill a row of banks: p ^ ((k >> 1 & 1) | (k >> 2 & 2))), so the eight 32-byte
-//                      pieces that half a wave's transposing read (ds_read_b64_tr_b16) takes are on different banks;
-//                      float: chunk c at c ^ 4 (k >> 2 & 3).
+//   row-major  [DIM rows][4 KS chunks of k]; chunk c of row r at slot c ^ (r & 7) (KS = 2) or c ^ (r >> 1 & 3) (KS = 1): the eight
+//              rows of a read's phase are on different banks;
+//   k-major    [step's rows of k][DIM], 16 bit: chunk pair p of row k at p ^ ((k & 3) | (k >> 1 & 4)) (128 columns and more; with
+//              64, two rows of k fill a row of banks: p ^ ((k >> 1 & 1) | (k >> 2 & 2))), so the eight 32-byte pieces that half a
+//              wave's transposing read (ds_read_b64_tr_b16) takes are on different banks; float: chunk c at c ^ 4 (k >> 2 & 3).
 #pragma once
 
 #include "common.h"
@@ -20,13 +18,13 @@ namespace fra {
 
 template <typename T> struct Elem {                 // 16-bit element types
     static constexpr int EPC = 8;                   // elements per 16-byte chunk
-    static constexpr int KSTEP = 64;                // contraction per step
+    static constexpr int KG = 32;                   // contraction per group
     typedef typename vec8<T>::type Frag;            // one lane's operand of an MFMA group: 16 bytes
     typedef typename vec4<T>::type Quad;
 };
 template <> struct Elem<float> {
     static constexpr int EPC = 4;
-    static constexpr int KSTEP = 32;
+    static constexpr int KG = 16;
     typedef f32x4 Frag;
     typedef f32x4 Quad;
 };
@@ -96,7 +94,7 @@ template <typename T> __device__ __forceinline__ void load_param4(const void* p,
     else load_four<T>(reinterpret_cast<const T*>(p) + at, n, o);
 }
 
-template <typename T> __device__ __forceinline__ int swz_row_major(int row, int c) { return c ^ (row & 7); }
+template <int KS> __device__ __forceinline__ int swz_row_major(int row, int c) { return KS == 2 ? c ^ (row & 7) : c ^ ((row >> 1) & 3); }
 template <typename T, int CPR> __device__ __forceinline__ int swz_k_major(int k, int c) {
     if constexpr (sizeof(T) == 4) return c ^ (((k >> 2) & 3) << 2);
     else if constexpr (CPR >= 16) return c ^ (((k & 3) | ((k >> 1) & 4)) << 1);
@@ -121,113 +119,76 @@ static __device__ __attribute__((aligned(16))) const float pj_zeros[4] = {0.0f, 
 
 // One operand of a workgroup's tile: where its chunks come from and how a wave reads its fragments.
 //   row-major: `rows` tile rows start at row0 of a row list (`order`, or the rows themselves), each `klen` long from k = 0;
-//   contraction-major: columns col0 .. col0 + DIM of an array whose rows (through `order`) k0 .. k0 + klen are summed over.
-template <typename T, bool KMAJOR, int DIM, int NT> struct Operand {
-    static constexpr int EPC = Elem<T>::EPC, KSTEP = Elem<T>::KSTEP;
-    static constexpr int CPR = KMAJOR ? DIM / EPC : 8;              // chunks per LDS row
-    static constexpr int CHUNKS = DIM * 8;                          // 16-byte chunks per tile
+//   k-major: columns 0 .. cols of `base`, whose rows row0 .. row0 + klen are summed over.
+// Chunks outside are zeros.
+template <typename T, bool KMAJOR, int DIM, int NT, int KS> struct Operand {
+    static constexpr int EPC = Elem<T>::EPC, KSTEP = KS * Elem<T>::KG;
+    static constexpr int CPR = KMAJOR ? DIM / EPC : 4 * KS;         // chunks per LDS row
+    static constexpr int CHUNKS = DIM * 4 * KS;                     // 16-byte chunks per tile
     static constexpr int BYTES = CHUNKS * 16;
     static constexpr int NLD = CHUNKS / NT;                         // per thread
+    static constexpr int RPP = NT / CPR;                            // LDS rows per pass
     static_assert(CHUNKS % NT == 0 && NT % CPR == 0, "whole chunks per thread, whole rows per pass");
     typedef typename Elem<T>::Frag Frag;
 
     const T* base;
-    const int* order;
+    const int* order;               // row-major only
     int64_t ld;
-    int row0, rows, klen, cols;     // k-major: row0 = first contraction row, cols = valid columns from `base`
+    int row0, rows, klen, cols;
 
-    // row-major: rows >= 1; tile row r stands for list entry row0 + min(r, rows - 1) (rows past the end repeat the last:
-    // their results are not stored)
-    __device__ __forceinline__ const T* row_ptr(int r) const {
-        const int at = row0 + (r < rows ? r : rows - 1);
-        return base + (int64_t)(order ? order[at] : at) * ld;
-    }
-    __device__ __forceinline__ void load(Frag (&v)[NLD], int step, int tid) const {
+    // this lane's chunk of every pass at step 0
+    struct Src {
+        const T* p[NLD];
+    };
+    // row-major: rows >= 1; tile row r stands for list entry row0 + min(r, rows - 1) (rows past the end repeat the last: their
+    // results are not stored)
+    __device__ __forceinline__ void init(Src& d, int tid) const {
 #pragma unroll
         for (int j = 0; j < NLD; ++j) {
-            const int slot = j * NT + tid, r = slot / CPR, s = slot % CPR;
+            const int r = j * RPP + tid / CPR;
             if constexpr (!KMAJOR) {
-                const int k = step * KSTEP + swz_row_major<T>(r, s) * EPC;
-                const int n = klen - k;
-                v[j] = load_chunk<T>(row_ptr(r) + (n > 0 ? k : 0), n);
+                const int at = row0 + (r < rows ? r : rows - 1);
+                d.p[j] = base + (int64_t)(order ? order[at] : at) * ld + swz_row_major<KS>(r, tid % CPR) * EPC;
             } else {
-                const int k = step * KSTEP + r, col = swz_k_major<T, CPR>(r, s) * EPC;
-                const int n = k < klen ? cols - col : 0;
-                const T* p = base;
-                if (n > 0) {
-                    const int at = row0 + k;
-                    p = base + (int64_t)(order ? order[at] : at) * ld + col;
-                }
-                v[j] = load_chunk<T>(p, n);
+                d.p[j] = base + (int64_t)(row0 + r) * ld + swz_k_major<T, CPR>(r, tid % CPR) * EPC;
             }
         }
+    }
+    // elements of the lane's chunk of pass j that are inside at `step` (<= 0: none)
+    __device__ __forceinline__ int valid(int j, int step, int tid) const {
+        const int r = j * RPP + tid / CPR;
+        if constexpr (!KMAJOR) return klen - step * KSTEP - swz_row_major<KS>(r, tid % CPR) * EPC;
+        else return step * KSTEP + r < klen ? cols - swz_k_major<T, CPR>(r, tid % CPR) * EPC : 0;
+    }
+    __device__ __forceinline__ int64_t advance(int step) const {
+        if constexpr (!KMAJOR) return (int64_t)step * KSTEP;
+        else return (int64_t)step * KSTEP * ld;
+    }
+
+    // ---- staging through registers: any alignment, any number of valid elements
+    __device__ __forceinline__ void load(const Src& d, Frag (&v)[NLD], int step, int tid) const {
+#pragma unroll
+        for (int j = 0; j < NLD; ++j) v[j] = load_chunk<T>(d.p[j] + advance(step), valid(j, step, tid));
     }
     static __device__ __forceinline__ void store(char* tile, const Frag (&v)[NLD], int tid) {
 #pragma unroll
         for (int j = 0; j < NLD; ++j) *reinterpret_cast<Frag*>(tile + (j * NT + tid) * 16) = v[j];
     }
     // ---- staging by DMA: every chunk is wholly inside or outside (klen or cols, pitch and base multiples of 16 bytes)
-    struct Dma {
-        const char* p[NLD];     // this lane's chunk of every pass at step 0 (k-major through a list: its column)
-        int next[KMAJOR ? NLD : 1];     // k-major through a list: row numbers of the next step to issue
-        bool in;                // k-major: the lane's column is inside (the same for all passes)
-    };
-    __device__ __forceinline__ void dma_init(Dma& d, int tid) const {
-        if constexpr (!KMAJOR) {
-            // the lane's chunk is at the same k in every pass: rows of one lane differ by a multiple of 8
-            static_assert(NT / 8 % 8 == 0, "");
-            const int c = swz_row_major<T>(tid / 8, tid % 8) * EPC;
-#pragma unroll
-            for (int j = 0; j < NLD; ++j) d.p[j] = reinterpret_cast<const char*>(row_ptr(j * (NT / 8) + tid / 8) + c);
-        } else {
-#pragma unroll
-            for (int j = 0; j < NLD; ++j) {
-                const int r = j * (NT / CPR) + tid / CPR, col = swz_k_major<T, CPR>(r, tid % CPR) * EPC;
-                d.p[j] = reinterpret_cast<const char*>(base + (order ? 0 : (int64_t)(row0 + r) * ld) + (col < cols ? col : 0));
-                d.next[j] = 0;
-            }
-            dma_rows(d, 0, tid);
-        }
-    }
-    // k-major through a list: fetch the row numbers of `step`
-    __device__ __forceinline__ void dma_rows(Dma& d, int step, int tid) const {
-        if constexpr (KMAJOR) {
-            if (!order) return;
-#pragma unroll
-            for (int j = 0; j < NLD; ++j) {
-                const int k = step * KSTEP + j * (NT / CPR) + tid / CPR;
-                d.next[j] = order[row0 + (k < klen ? k : klen - 1)];
-            }
-        }
-    }
-    __device__ __forceinline__ void dma_issue(const Dma& d, int step, LdsPtr lds, int tid) const {
-        const bool tail = (step + 1) * KSTEP > klen;
-        if constexpr (KMAJOR) {     // the row numbers have arrived before the first load leaves: a wait for one of them in
-                                    // between would wait for the loads before it as well
-#pragma unroll
-            for (int j = 0; j < NLD; ++j) asm volatile("" ::"v"(d.next[j]));
-        }
+    __device__ __forceinline__ void issue(const Src& d, int step, LdsPtr lds, int tid) const {
 #pragma unroll
         for (int j = 0; j < NLD; ++j) {
-            const char* p;
-            if constexpr (!KMAJOR) {
-                p = d.p[j] + (int64_t)step * 128;
-                if (tail && step * KSTEP + swz_row_major<T>(tid / 8, tid % 8) * EPC >= klen) p = reinterpret_cast<const char*>(pj_zeros);
-            } else {
-                const int r = j * (NT / CPR) + tid / CPR;
-                const bool inside = swz_k_major<T, CPR>(r, tid % CPR) * EPC < cols && (!tail || step * KSTEP + r < klen);
-                p = d.p[j] + (order ? (int64_t)d.next[j] * ld : (int64_t)step * KSTEP * ld) * (int)sizeof(T);
-                if (!inside) p = reinterpret_cast<const char*>(pj_zeros);
-            }
+            const T* p = d.p[j] + advance(step);
+            if (valid(j, step, tid) <= 0) p = reinterpret_cast<const T*>(pj_zeros);
             dma16(p, lds + j * (NT * 16));
         }
     }
-    // fragment of the 16 rows / columns from `d0`, k half `ks` (0, 1) of the step
+    // fragment of the 16 rows / columns from `d0`, k group `ks` of the step
     static __device__ __forceinline__ Frag frag(const char* tile, int d0, int ks, int lane) {
         const int m = lane & 15, g = lane >> 4;
         if constexpr (!KMAJOR) {
             const int r = d0 + m;
-            return *reinterpret_cast<const Frag*>(tile + (r * 8 + swz_row_major<T>(r, ks * 4 + g)) * 16);
+            return *reinterpret_cast<const Frag*>(tile + (r * CPR + swz_row_major<KS>(r, ks * 4 + g)) * 16);
         } else if constexpr (sizeof(T) == 2) {
             // sixteen lanes take four rows of k x sixteen columns and receive one column of four k each
             typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -254,11 +215,15 @@ template <typename T, bool KMAJOR, int DIM, int NT> struct Operand {
     }
 };
 
-// Workgroup shape: BI x BJ results on WI x WJ waves; a wave owns MI x MJ tiles of 16 x 16.
-template <int BI_, int BJ_, int WI_, int WJ_> struct Shape {
-    static constexpr int BI = BI_, BJ = BJ_, WI = WI_, WJ = WJ_, NT = 64 * WI * WJ;
+// Workgroup shape: BI x BJ results on WI x WJ waves (a wave owns MI x MJ tiles of 16 x 16), KS groups of k per step, NB steps in
+// LDS.
+template <int BI_, int BJ_, int WI_, int WJ_, int KS_, int NB_> struct Shape {
+    static constexpr int BI = BI_, BJ = BJ_, WI = WI_, WJ = WJ_, KS = KS_, NB = NB_, NT = 64 * WI * WJ;
     static constexpr int MI = BI / WI / 16, MJ = BJ / WJ / 16;
+    static constexpr int LDS = NB * (BI + BJ) * KS * 64;
 };
+template <typename T, bool KMAJOR, typename S> using OperandA = Operand<T, KMAJOR, S::BI, S::NT, S::KS>;
+template <typename T, bool KMAJOR, typename S> using OperandB = Operand<T, KMAJOR, S::BJ, S::NT, S::KS>;
 
 // Hands a workgroup's results on as 16-byte pieces of rows: a wave turns its accumulators through its own part of LDS, 16 rows
 // at a time (written as a lane's four neighbouring columns, pitch + 16 bytes: no bank conflicts; read as V neighbouring
@@ -268,7 +233,7 @@ template <int BI_, int BJ_, int WI_, int WJ_> struct Shape {
 // `lds` is free when every wave is past the last step's barrier.
 template <typename T, typename S, typename F> __device__ __forceinline__ void tile_emit(const f32x4 (&acc)[S::MI][S::MJ], char* lds, const F& f) {
     constexpr int COLS = S::MJ * 16, V = 16 / sizeof(T), LPR = COLS / V, RPP = 64 / LPR, NP = 16 / RPP, PITCH = COLS + 4;
-    static_assert(S::WI * S::WJ * 16 * PITCH * 4 <= 2 * (S::BI + S::BJ) * 128, "the strips fit the tiles' buffers");
+    static_assert(S::WI * S::WJ * 16 * PITCH * 4 <= S::LDS, "the strips fit the tiles' buffers");
     static_assert(16 % RPP == 0, "whole passes per strip");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
@@ -303,10 +268,10 @@ template <typename T, typename S, typename F> __device__ __forceinline__ void ti
 // The MFMAs of one step on the tiles in LDS.
 template <typename T, bool AK, bool BK, typename S>
 __device__ __forceinline__ void tile_step(const char* ta, const char* tb, int i0, int j0, int lane, f32x4 (&acc)[S::MI][S::MJ]) {
-    typedef Operand<T, AK, S::BI, S::NT> OA;
-    typedef Operand<T, BK, S::BJ, S::NT> OB;
+    typedef OperandA<T, AK, S> OA;
+    typedef OperandB<T, BK, S> OB;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
+    for (int ks = 0; ks < S::KS; ++ks) {
         typename Elem<T>::Frag fa[S::MI], fb[S::MJ];
 #pragma unroll
         for (int mi = 0; mi < S::MI; ++mi) fa[mi] = OA::frag(ta, i0 + 16 * mi, ks, lane);
@@ -321,14 +286,17 @@ __device__ __forceinline__ void tile_step(const char* ta, const char* tb, int i0
 
 // acc[mi][mj][r] = C[i][j] with i = 16 mi + (lane & 15), j = 16 mj + 4 (lane >> 4) + r inside the wave's part: the j side is
 // the MFMA's row operand, so a lane holds four neighbouring j of one i.  klen: the longer of the operands' (an operand's
-// chunks past its own are zeros).  ADD: on top of what acc holds.  Two LDS buffers: step t + 1 is on its way while t runs.
-// DMA: both operands are staged without registers (see Operand::Dma for what that asks of them).
+// chunks past its own are zeros).  ADD: on top of what acc holds.
+// DMA: the next NB - 1 steps are on their way while one runs; one barrier per step says both that the step has arrived for
+// every wave and that every wave has left the buffer the next load goes to.  Otherwise the next step waits in registers.
+// On return every wave is past its last LDS read.
 template <typename T, bool AK, bool BK, typename S, bool DMA, bool ADD = false>
-__device__ __forceinline__ void tile_product(const Operand<T, AK, S::BI, S::NT>& A, const Operand<T, BK, S::BJ, S::NT>& B,
-                                             int klen, char* lds, f32x4 (&acc)[S::MI][S::MJ]) {
-    typedef Operand<T, AK, S::BI, S::NT> OA;
-    typedef Operand<T, BK, S::BJ, S::NT> OB;
-    constexpr int BUF = OA::BYTES + OB::BYTES;
+__device__ __forceinline__ void tile_product(const OperandA<T, AK, S>& A, const OperandB<T, BK, S>& B, int klen, char* lds,
+                                             f32x4 (&acc)[S::MI][S::MJ]) {
+    typedef OperandA<T, AK, S> OA;
+    typedef OperandB<T, BK, S> OB;
+    constexpr int BUF = OA::BYTES + OB::BYTES, NB = S::NB;
+    static_assert(BUF * NB == S::LDS && NB >= 2 && NB <= 5, "");
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -338,51 +306,50 @@ __device__ __forceinline__ void tile_product(const Operand<T, AK, S::BI, S::NT>&
 #pragma unroll
             for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
     }
-    const int steps = (klen + Elem<T>::KSTEP - 1) / Elem<T>::KSTEP;
+    const int steps = (klen + OA::KSTEP - 1) / OA::KSTEP;
     if (steps == 0) return;
+    typename OA::Src sa;
+    typename OB::Src sb;
+    A.init(sa, tid);
+    B.init(sb, tid);
 
     if constexpr (DMA) {
         constexpr int NLD = OA::NLD + OB::NLD;
-        typename OA::Dma da;
-        typename OB::Dma db;
         const LdsPtr dst = (LdsPtr)lds + __builtin_amdgcn_readfirstlane(wave) * 1024;
-        A.dma_init(da, tid);
-        B.dma_init(db, tid);
-        A.dma_issue(da, 0, dst, tid);
-        B.dma_issue(db, 0, dst + OA::BYTES, tid);
-        if (steps > 1) {
-            A.dma_rows(da, 1, tid);
-            B.dma_rows(db, 1, tid);
-        }
+#pragma unroll
+        for (int t = 0; t < NB - 1; ++t)
+            if (t < steps) {
+                A.issue(sa, t, dst + t * BUF, tid);
+                B.issue(sb, t, dst + t * BUF + OA::BYTES, tid);
+            }
+        int cur = 0, nxt = (NB - 1) * BUF;
         for (int t = 0; t < steps; ++t) {
-            if (t + 1 < steps) {
-                const LdsPtr to = dst + ((t + 1) & 1) * BUF;
-                A.dma_issue(da, t + 1, to, tid);
-                B.dma_issue(db, t + 1, to + OA::BYTES, tid);
-                dma_wait_barrier<NLD>();            // step t is in LDS, t + 1 on its way
-            } else {
-                dma_wait_barrier<0>();
+            const int behind = steps - 1 - t;       // steps after this one, at most NB - 2 of them on their way
+            if (behind >= NB - 2) dma_wait_barrier<(NB - 2) * NLD>();
+            else if (NB > 4 && behind == 2) dma_wait_barrier<2 * NLD>();
+            else if (NB > 3 && behind == 1) dma_wait_barrier<NLD>();
+            else dma_wait_barrier<0>();
+            if (t + NB - 1 < steps) {
+                A.issue(sa, t + NB - 1, dst + nxt, tid);
+                B.issue(sb, t + NB - 1, dst + nxt + OA::BYTES, tid);
             }
-            if (t + 2 < steps) {
-                A.dma_rows(da, t + 2, tid);
-                B.dma_rows(db, t + 2, tid);
-            }
-            const char* ta = lds + (t & 1) * BUF;
-            tile_step<T, AK, BK, S>(ta, ta + OA::BYTES, i0, j0, lane, acc);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // everyone is done with step t's buffer
+            tile_step<T, AK, BK, S>(lds + cur, lds + cur + OA::BYTES, i0, j0, lane, acc);
+            nxt = cur;
+            cur = cur + BUF == NB * BUF ? 0 : cur + BUF;
         }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     } else {
         typename Elem<T>::Frag va[OA::NLD], vb[OB::NLD];
-        A.load(va, 0, tid);
-        B.load(vb, 0, tid);
+        A.load(sa, va, 0, tid);
+        B.load(sb, vb, 0, tid);
         OA::store(lds, va, tid);
         OB::store(lds + OA::BYTES, vb, tid);
         __syncthreads();
         for (int t = 0; t < steps; ++t) {
             const char* ta = lds + (t & 1) * BUF;
             if (t + 1 < steps) {
-                A.load(va, t + 1, tid);
-                B.load(vb, t + 1, tid);
+                A.load(sa, va, t + 1, tid);
+                B.load(sb, vb, t + 1, tid);
             }
             tile_step<T, AK, BK, S>(ta, ta + OA::BYTES, i0, j0, lane, acc);
             if (t + 1 < steps) {
