@@ -15,33 +15,23 @@ namespace fra {
 
 enum { PJ_NONE = 0, PJ_RELU = 1, PJ_PRELU = 2, PJ_SILU = 3, PJ_GELU_TANH = 4 };
 
-// 1 / (1 + e^-v).  For 16-bit results the hardware's reciprocal (1 ulp) is far below the final rounding.
-template <typename T> __device__ __forceinline__ float pj_sigmoid(float v) {
-    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.0f + __expf(-v));
-    else return 1.0f / (1.0f + expf(-v));
+// 1 / (1 + 2^-t): the sigmoid of t ln 2, so that callers fold log2(e) into their constants.  For 16-bit results the hardware's
+// exponential and reciprocal (1 ulp each) are far below the final rounding; the epilogues run on the vector ALU beside the
+// matrix cores, where these two cost four slots each.
+constexpr float LOG2E = 1.4426950408889634f, GELU_C = 1.5957691216057308f, GELU_A = 0.044715f;      // GELU_C: 2 sqrt(2 / pi)
+template <typename T> __device__ __forceinline__ float pj_sigmoid2(float t) {
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-t));
+    else return 1.0f / (1.0f + exp2f(-t));
 }
-constexpr float GELU_C = 1.5957691216057308f, GELU_A = 0.044715f;       // 2 sqrt(2 / pi)
 
 // comparisons are written so that a NaN goes through
 template <typename T> __device__ __forceinline__ float pj_act(int act, float z, float s) {
     switch (act) {
         case PJ_RELU: return z < 0.0f ? 0.0f : z;
         case PJ_PRELU: return z < 0.0f ? z * s : z;
-        case PJ_SILU: return z * pj_sigmoid<T>(z);
-        case PJ_GELU_TANH: return z * pj_sigmoid<T>(GELU_C * (z + GELU_A * z * z * z));
+        case PJ_SILU: return z * pj_sigmoid2<T>(LOG2E * z);
+        case PJ_GELU_TANH: return z * pj_sigmoid2<T>(z * (LOG2E * GELU_C + LOG2E * GELU_C * GELU_A * (z * z)));
         default: return z;
-    }
-}
-// one branch for a whole piece
-template <typename T, int V> __device__ __forceinline__ void pj_act_all(int act, float (&v)[V], const float (&s)[V]) {
-    switch (act) {
-#define PJ_CASE(A)                                                \
-    case A:                                                       \
-        _Pragma("unroll") for (int e = 0; e < V; ++e) v[e] = pj_act<T>(A, v[e], s[e]); \
-        break;
-        PJ_CASE(PJ_RELU) PJ_CASE(PJ_PRELU) PJ_CASE(PJ_SILU) PJ_CASE(PJ_GELU_TANH)
-#undef PJ_CASE
-        default: break;
     }
 }
 template <typename T> __device__ __forceinline__ float pj_act_grad(int act, float z, float s) {
@@ -49,12 +39,12 @@ template <typename T> __device__ __forceinline__ float pj_act_grad(int act, floa
         case PJ_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case PJ_PRELU: return z > 0.0f ? 1.0f : s;
         case PJ_SILU: {
-            const float q = pj_sigmoid<T>(z);
+            const float q = pj_sigmoid2<T>(LOG2E * z);
             return q * (1.0f + z * (1.0f - q));
         }
         case PJ_GELU_TANH: {
-            const float q = pj_sigmoid<T>(GELU_C * (z + GELU_A * z * z * z));
-            return q + z * q * (1.0f - q) * GELU_C * (1.0f + 3.0f * GELU_A * z * z);
+            const float q = pj_sigmoid2<T>(z * (LOG2E * GELU_C + LOG2E * GELU_C * GELU_A * (z * z)));
+            return q * (1.0f + z * (1.0f - q) * (GELU_C + 3.0f * GELU_A * GELU_C * (z * z)));
         }
         default: return 1.0f;
     }
@@ -77,8 +67,10 @@ struct RowArgs {
     const int* order;           // nullptr: the rows themselves
     const int4* tiles;          // (group, first list entry, end, -) per row tile; nullptr: one group, tiles of BI rows
     const int* offsets;         // [G + 1] list entries of a group (grouped only)
+    const int* tile_offsets;    // [G + 2], the last one the number of tiles in use (grouped only)
     int n_tiles, M, G;
 };
+__device__ __forceinline__ int tiles_in_use(const RowArgs& a) { return a.tiles ? a.tile_offsets[a.G + 1] : a.n_tiles; }
 __device__ __forceinline__ bool row_tile(const RowArgs& a, int t, int bi, int& g, int& begin, int& end) {
     if (a.tiles) {
         const int4 e = a.tiles[t];
@@ -99,80 +91,119 @@ struct FwdArgs {
     int K, N, act, bias_f32, slope_f32, n_col_tiles;
 };
 
-// A lane's columns are the same in all its pieces, so bias and slope sit in registers.
-template <typename T> struct ForwardEmit {
+// A lane's columns are the same in all its pieces, so bias and slope sit in registers.  FULL: the tile's columns are all inside
+// and ACT is the activation, so that the pieces are straight-line code whose loads and arithmetic overlap (with a guard around
+// every access and the activation chosen per piece a 262144 x 512 x 512 product took 316 us, see pj_forward_kernel); otherwise
+// everything is checked, and ACT is not used.
+template <typename T> struct LaneParams {
     static constexpr int V = 16 / sizeof(T);
-    struct Pre {
-        int row;                    // -1: past the tile's rows or columns
-        typename Elem<T>::Frag r;
-    };
-    const FwdArgs* a;
-    int begin, count, n0, left;     // left: valid columns from the lane's first
-    bool live;
     float bi[V], sl[V];
-    __device__ __forceinline__ void init(int g, int col) {
-        const int n = n0 + col;
-        left = a->N - n;
+    __device__ __forceinline__ void load(const FwdArgs& a, int64_t at, int left, bool live) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) bi[e] = sl[e] = 0.0f;
+        if (a.bias && live) vec(a.bias, a.bias_f32, at, left, bi);
+        if (a.slope && live) vec(a.slope, a.slope_f32, at, left, sl);
+    }
+    __device__ __forceinline__ static void vec(const void* p, int is_f32, int64_t at, int left, float (&o)[V]) {
 #pragma unroll
         for (int q = 0; q < V; q += 4) {
-            float b4[4] = {0, 0, 0, 0}, s4[4] = {0, 0, 0, 0};
-            if (a->bias && live) load_param4<T>(a->bias, a->bias_f32, (int64_t)g * a->N + n + q, left - q, b4);
-            if (a->slope && live) load_param4<T>(a->slope, a->slope_f32, (int64_t)g * a->N + n + q, left - q, s4);
+            float t[4];
+            load_param4<T>(p, is_f32, at + q, left - q, t);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { bi[q + e] = b4[e]; sl[q + e] = s4[e]; }
+            for (int e = 0; e < 4; ++e) o[q + e] = t[e];
         }
     }
+};
+template <typename T, int ACT, bool FULL> struct ForwardEmit {
+    static constexpr int V = 16 / sizeof(T);
+    typedef typename Elem<T>::Frag Frag;
+    struct Pre {
+        int row;                    // -1: nothing to store
+        Frag r;
+    };
+    const FwdArgs& a;
+    const LaneParams<T>& par;
+    int begin, count, n0, left;     // left: valid columns from the lane's first
+    bool live;
     __device__ __forceinline__ Pre pre(int i, int j) const {
         Pre p;
-        p.row = -1;
-#pragma unroll
-        for (int e = 0; e < V; ++e) p.r[e] = (T)0.0f;
-        if (i < count && left > 0) {
-            p.row = a->rows.order ? a->rows.order[begin + i] : begin + i;
-            if (a->resid) p.r = load_chunk<T>((const T*)a->resid + (int64_t)p.row * a->ldr + n0 + j, left);
+        if constexpr (FULL) {
+            const int at = begin + (i < count ? i : count - 1);
+            p.row = a.rows.order ? a.rows.order[at] : at;
+            if (a.resid) p.r = load_chunk<T>((const T*)a.resid + (int64_t)p.row * a.ldr + n0 + j, V);
+            if (i >= count) p.row = -1;
+        } else {
+            p.row = -1;
+            if (i < count && left > 0) {
+                p.row = a.rows.order ? a.rows.order[begin + i] : begin + i;
+                if (a.resid) p.r = load_chunk<T>((const T*)a.resid + (int64_t)p.row * a.ldr + n0 + j, left);
+            }
         }
         return p;
     }
     __device__ __forceinline__ void emit(const Pre& p, int, int j, float (&v)[V]) const {
-        if (p.row < 0) return;
-        const int64_t at = (int64_t)p.row * a->N + n0 + j;
-        typename Elem<T>::Frag o;
+        const int64_t at = (int64_t)p.row * a.N + n0 + j;
+        const int n = FULL ? V : left;
+        Frag o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] += bi[e];
-        if (a->z && live) {
+        for (int e = 0; e < V; ++e) v[e] += par.bi[e];
+        if (a.z && live && p.row >= 0) {
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = (T)v[e];
-            store_chunk<T>((T*)a->z + at, left, o);
+            store_chunk<T>((T*)a.z + at, n, o);
         }
-        if (!live) {
+        if constexpr (FULL) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = 0.0f;
+            for (int e = 0; e < V; ++e) v[e] = pj_act<T>(ACT, v[e], par.sl[e]);
         } else {
-            pj_act_all<T, V>(a->act, v, sl);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = live ? pj_act<T>(a.act, v[e], par.sl[e]) : 0.0f;
+        }
+        if (a.resid) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += (float)p.r[e];
         }
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = (T)(v[e] + (float)p.r[e]);
-        store_chunk<T>((T*)a->y + at, left, o);
+        for (int e = 0; e < V; ++e) o[e] = (T)v[e];
+        if (p.row >= 0) store_chunk<T>((T*)a.y + at, n, o);
     }
 };
-template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT) void pj_forward_kernel(FwdArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
-    int g, begin, end;
-    if (!row_tile(a.rows, rt, S::BI, g, begin, end)) return;
-    const bool live = g < a.rows.G;                                 // group G: rows of no group
-    const int n0 = ct * S::BJ;
-    f32x4 acc[S::MI][S::MJ];
-    OperandA<T, false, S> A;
-    A.base = (const T*)a.x; A.order = a.rows.order; A.ld = a.ldx; A.row0 = begin; A.rows = end - begin; A.klen = a.K; A.cols = 0;
-    OperandB<T, false, S> B;
-    B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0); B.order = nullptr; B.ld = a.ldw; B.row0 = n0; B.rows = a.N - n0; B.klen = a.K; B.cols = 0;
-    tile_product<T, false, false, S, DMA>(A, B, live ? a.K : 0, lds, acc);
+// A tile of rows x columns as the product kernels see it
+struct Tile {
+    int g, begin, end, c0;
+    bool live;                      // false: rows of no group
+};
+__device__ __forceinline__ bool next_tile(const RowArgs& a, unsigned b, int n_col_tiles, int bi, int bj, Tile& t) {
+    int rt, ct;
+    if (!tile_of_block(b, tiles_in_use(a), n_col_tiles, rt, ct) || !row_tile(a, rt, bi, t.g, t.begin, t.end)) return false;
+    t.c0 = ct * bj;
+    t.live = t.g < a.G;
+    return true;
+}
 
-    ForwardEmit<T> f;
-    f.a = &a; f.begin = begin; f.count = end - begin; f.n0 = n0; f.live = live;
-    f.init(g, (threadIdx.x >> 6) / S::WI * (S::BJ / S::WJ) + (int)(threadIdx.x & 63) % (S::MJ * 16 / f.V) * f.V);
-    tile_emit<T, S>(acc, lds, f);
+template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_forward_kernel(FwdArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    typedef Product<T, false, false, S, DMA> P;
+    constexpr int V = 16 / sizeof(T);
+    f32x4 acc[S::MI][S::MJ];
+    P p;
+    Tile t;
+    if (!next_tile(a.rows, blockIdx.x, a.n_col_tiles, S::BI, S::BJ, t)) return;
+    p.A.base = (const T*)a.x; p.A.order = a.rows.order; p.A.ld = a.ldx; p.A.row0 = t.begin; p.A.rows = t.end - t.begin; p.A.klen = a.K; p.A.cols = 0;
+    p.B.base = (const T*)a.w + (t.live ? (int64_t)t.g * a.wg : 0); p.B.order = nullptr; p.B.ld = a.ldw; p.B.row0 = t.c0; p.B.rows = a.N - t.c0; p.B.klen = a.K; p.B.cols = 0;
+    p.start(t.live ? a.K : 0, lds);
+    const int col = (threadIdx.x >> 6) / S::WI * (S::BJ / S::WJ) + (int)(threadIdx.x & 63) % (S::MJ * 16 / V) * V;
+    const int left = a.N - t.c0 - col;
+    LaneParams<T> par;                                              // on their way while the product runs
+    par.load(a, (int64_t)t.g * a.N + t.c0 + col, left, t.live);
+    p.run(lds, acc);
+    switch (t.live && t.c0 + S::BJ <= a.N ? a.act : -1) {
+#define PJ_CASE(A) \
+    case A: tile_emit<T, S>(acc, lds, ForwardEmit<T, A, true>{a, par, t.begin, t.end - t.begin, t.c0, left, true}); break;
+        PJ_CASE(PJ_NONE) PJ_CASE(PJ_RELU) PJ_CASE(PJ_PRELU) PJ_CASE(PJ_SILU) PJ_CASE(PJ_GELU_TANH)
+#undef PJ_CASE
+        default: tile_emit<T, S>(acc, lds, ForwardEmit<T, 0, false>{a, par, t.begin, t.end - t.begin, t.c0, left, t.live});
+    }
 }
 
 // The same for few rows (tiles of 16 MT): a workgroup takes 16 columns, its four waves every fourth group of k, and their sums
@@ -249,34 +280,32 @@ struct DxArgs {
     int64_t lddz, ldw, wg;
     int K, Kp, N, Np, n_col_tiles;      // Np, Kp: columns of dz and W, zeros past N and K
 };
-template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dx_kernel(DxArgs a) {
+template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_dx_kernel(DxArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
-    int g, begin, end;
-    if (!row_tile(a.rows, rt, S::BI, g, begin, end)) return;
-    const bool live = g < a.rows.G;
-    const int k0 = ct * S::BJ;
-    f32x4 acc[S::MI][S::MJ];
-    OperandA<T, false, S> A;
-    A.base = (const T*)a.dz; A.order = nullptr; A.ld = a.lddz; A.row0 = begin; A.rows = end - begin; A.klen = a.Np; A.cols = 0;
-    OperandB<T, true, S> B;
-    B.base = (const T*)a.w + (live ? (int64_t)g * a.wg : 0) + k0; B.order = nullptr; B.ld = a.ldw; B.row0 = 0; B.rows = 0; B.klen = a.N; B.cols = a.Kp - k0;
-    tile_product<T, false, true, S, true>(A, B, live ? a.Np : 0, lds, acc);
+    typedef Product<T, false, true, S, true> P;
     struct Emit {
         typedef int Pre;
-        const DxArgs* a;
-        int begin, count, k0;
-        __device__ __forceinline__ int pre(int i, int) const { return i < count ? (a->rows.order ? a->rows.order[begin + i] : begin + i) : -1; }
+        const DxArgs& a;
+        Tile t;
+        __device__ __forceinline__ int pre(int i, int) const { return t.begin + i < t.end ? (a.rows.order ? a.rows.order[t.begin + i] : t.begin + i) : -1; }
         __device__ __forceinline__ void emit(int row, int, int j, float (&v)[16 / sizeof(T)]) const {
-            const int left = a->K - k0 - j;
+            const int left = a.K - t.c0 - j;
             if (row < 0 || left <= 0) return;
             typename Elem<T>::Frag o;
 #pragma unroll
             for (int e = 0; e < 16 / (int)sizeof(T); ++e) o[e] = (T)v[e];
-            store_chunk<T>((T*)a->dx + (int64_t)row * a->K + k0 + j, left, o);
+            store_chunk<T>((T*)a.dx + (int64_t)row * a.K + t.c0 + j, left, o);
         }
-    } f = {&a, begin, end - begin, k0};
-    tile_emit<T, S>(acc, lds, f);
+    };
+    f32x4 acc[S::MI][S::MJ];
+    P p;
+    Tile t;
+    if (!next_tile(a.rows, blockIdx.x, a.n_col_tiles, S::BI, S::BJ, t)) return;
+    p.A.base = (const T*)a.dz; p.A.order = nullptr; p.A.ld = a.lddz; p.A.row0 = t.begin; p.A.rows = t.end - t.begin; p.A.klen = a.Np; p.A.cols = 0;
+    p.B.base = (const T*)a.w + (t.live ? (int64_t)t.g * a.wg : 0) + t.c0; p.B.order = nullptr; p.B.ld = a.ldw; p.B.row0 = 0; p.B.rows = 0; p.B.klen = a.N; p.B.cols = a.Kp - t.c0;
+    p.start(t.live ? a.Np : 0, lds);
+    p.run(lds, acc);
+    tile_emit<T, S>(acc, lds, Emit{a, t});
 }
 
 // dW[g] = sum over the group's rows of dz^T x: both operands k-major.  `splits` workgroups share a group's rows and leave fp32
@@ -302,12 +331,12 @@ template <typename O> struct DwEmit {
         store_chunk<O>(out + (int64_t)n * K + k0 + j, left, o);
     }
 };
-template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dw_kernel(DwArgs a) {
+template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_dw_kernel(DwArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    unsigned b = blockIdx.x;
-    const int tj = b % a.n_tj; b /= a.n_tj;
-    const int ti = b % a.n_ti; b /= a.n_ti;
-    const int s = b % a.splits, g = b / a.splits;
+    // blockIdx.y: group and split
+    const int s = blockIdx.y % a.splits, g = blockIdx.y / a.splits;
+    int ti, tj;
+    if (!tile_of_block(blockIdx.x, a.n_ti, a.n_tj, ti, tj)) return;
     int begin = a.rows.offsets ? a.rows.offsets[g] : 0, end = a.rows.offsets ? a.rows.offsets[g + 1] : a.rows.M;
     if (a.splits > 1) {                                             // whole steps per split
         const int step = S::KS * Elem<T>::KG;
@@ -318,12 +347,13 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT) void pj_dw
         end = e0 < end ? (int)e0 : end;
     }
     const int n0 = ti * S::BI, k0 = tj * S::BJ;
+    typedef Product<T, true, true, S, true> P;
     f32x4 acc[S::MI][S::MJ];
-    OperandA<T, true, S> A;
-    A.base = (const T*)a.dz + n0; A.order = nullptr; A.ld = a.lddz; A.row0 = begin; A.rows = 0; A.klen = end - begin; A.cols = a.Np - n0;
-    OperandB<T, true, S> B;
-    B.base = (const T*)a.x + k0; B.order = nullptr; B.ld = a.ldx; B.row0 = begin; B.rows = 0; B.klen = end - begin; B.cols = a.Kp - k0;
-    tile_product<T, true, true, S, true>(A, B, end - begin, lds, acc);
+    P p;
+    p.A.base = (const T*)a.dz + n0; p.A.order = nullptr; p.A.ld = a.lddz; p.A.row0 = begin; p.A.rows = 0; p.A.klen = end - begin; p.A.cols = a.Np - n0;
+    p.B.base = (const T*)a.x + k0; p.B.order = nullptr; p.B.ld = a.ldx; p.B.row0 = begin; p.B.rows = 0; p.B.klen = end - begin; p.B.cols = a.Kp - k0;
+    p.start(end - begin, lds);
+    p.run(lds, acc);
     const int64_t plane = (int64_t)a.N * a.K;
     if (a.splits > 1) {
         DwEmit<float> f = {(float*)a.dw + ((int64_t)s * a.rows.G + g) * plane, a.N, a.K, n0, k0};
@@ -350,7 +380,7 @@ template <typename T> __global__ __launch_bounds__(256) void pj_join_kernel(cons
 }
 
 // dz = dy act'(z) in list order and, per row tile, the column sums of dz and of dy min(z, 0).  A workgroup takes one row tile x
-// `lpr` 16-byte pieces of columns (lpr lanes side by side, a power of two up to 64; 256 / lpr rows at a time); four rows per
+// `lpr` 16-byte pieces of columns (lpr lanes side by side, a power of two up to 64; 256 / lpr rows at a time); eight rows per
 // lane are requested together.  Bound by HBM: dy and z in, dz out.
 struct DzArgs {
     RowArgs rows;
@@ -362,7 +392,7 @@ struct DzArgs {
 };
 template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs a) {
     typedef typename Elem<T>::Frag Frag;
-    constexpr int V = Elem<T>::EPC, U = 4;
+    constexpr int V = Elem<T>::EPC, U = 8;
     __shared__ float sums[256][V + 1];
     const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
     int g, begin, end;
@@ -407,7 +437,7 @@ template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs
                     for (int e = 0; e < V; ++e) {
                         const float y = (float)dy[u][e], zv = (float)z[u][e], dz = y * dv[e];
                         sb[e] += dz;
-                        ss[e] += zv > 0.0f ? 0.0f : y * zv;
+                        if (a.part_s) ss[e] += zv > 0.0f ? 0.0f : y * zv;
                         d[e] = (T)dz;
                     }
                 } else {
@@ -698,11 +728,11 @@ template <typename K> static int raise_lds(K kernel, int bytes, std::atomic<uint
         static std::atomic<uint64_t> lds_done{0};                                        \
         const int rc__ = raise_lds(KERNEL, LDS, lds_done);                               \
         if (rc__ != FRA_OK) return rc__;                                                 \
-        hipLaunchKernelGGL(KERNEL, dim3((unsigned)(GRID)), dim3(NT), LDS, STREAM, ARGS); \
+        hipLaunchKernelGGL(KERNEL, (GRID), dim3(NT), LDS, STREAM, ARGS); \
         FRA_HIP(hipGetLastError());                                                      \
     } while (0)
 
-typedef Shape<128, 128, 2, 2, 1, 4> Big;
+typedef Shape<128, 128, 4, 2, 2, 2> Big;
 typedef Shape<64, 64, 2, 2, 2, 3> Small;
 
 static int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
@@ -735,6 +765,7 @@ static RowArgs row_args(const fra_linear_desc* d, int tile_rows) {
     r.order = g ? g->order : nullptr;
     r.tiles = g ? (const int4*)g->tiles : nullptr;
     r.offsets = g ? g->offsets : nullptr;
+    r.tile_offsets = g ? g->tile_offsets : nullptr;
     r.n_tiles = g ? g->n_tiles : cdiv(d->M, tile_rows);
     r.M = (int)d->M;
     r.G = g ? g->n_groups : 1;
@@ -749,12 +780,12 @@ static bool big_tiles(int64_t rows, int64_t cols) { return (int64_t)cdiv(rows, 1
 
 template <typename T, typename S> static int launch_forward(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
     a.n_col_tiles = cdiv(d->N, S::BJ);
-    const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
+    const int64_t blocks = ((int64_t)a.rows.n_tiles * a.n_col_tiles + 7) / 8 * 8;
     if (int rc = check_grid(blocks, "fra_linear")) return rc;
     if (dma_ok<T>(d->x, d->ldx, d->K) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K))
-        PJ_LAUNCH((pj_forward_kernel<T, S, true>), blocks, S::NT, S::LDS, s, a);
+        PJ_LAUNCH((pj_forward_kernel<T, S, true>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
     else
-        PJ_LAUNCH((pj_forward_kernel<T, S, false>), blocks, S::NT, S::LDS, s, a);
+        PJ_LAUNCH((pj_forward_kernel<T, S, false>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
     return FRA_OK;
 }
 template <typename T, int MT> static int launch_few_rows(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
@@ -830,9 +861,9 @@ template <typename T> static int launch_pack(const PackArgs& a, hipStream_t s) {
 }
 template <typename T, typename S> static int launch_dx(DxArgs& a, hipStream_t s) {
     a.n_col_tiles = cdiv(a.K, S::BJ);
-    const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
+    const int64_t blocks = ((int64_t)a.rows.n_tiles * a.n_col_tiles + 7) / 8 * 8;
     if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
-    PJ_LAUNCH((pj_dx_kernel<T, S>), blocks, S::NT, S::LDS, s, a);
+    PJ_LAUNCH((pj_dx_kernel<T, S>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
     return FRA_OK;
 }
 template <typename T>
@@ -904,9 +935,9 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         a.rows = row_args(d, 128);
         a.dz = dz; a.dw = p.splits > 1 ? (void*)(ws + p.off_part) : dw; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
         a.n_ti = cdiv(d->N, Big::BI); a.n_tj = cdiv(d->K, Big::BJ); a.splits = p.splits;
-        const int64_t blocks = (int64_t)a.n_ti * a.n_tj * a.splits * G;
-        if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
-        PJ_LAUNCH((pj_dw_kernel<T, Big>), blocks, Big::NT, Big::LDS, s, a);
+        const int64_t blocks = ((int64_t)a.n_ti * a.n_tj + 7) / 8 * 8;
+        if (int rc = check_grid(blocks * a.splits * G, "fra_linear_backward")) return rc;
+        PJ_LAUNCH((pj_dw_kernel<T, Big>), dim3((unsigned)blocks, a.splits * G), Big::NT, Big::LDS, s, a);
         if (p.splits > 1) {
             const int64_t n = (int64_t)G * d->N * d->K, jb = (n + 1023) / 1024;
             if (int rc = check_grid(jb, "fra_linear_backward")) return rc;

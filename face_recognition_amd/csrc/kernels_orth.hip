@@ -99,19 +99,21 @@ template <typename T, bool BK, typename S> __global__ __launch_bounds__(S::NT) v
     const int i0 = rt * S::BI, j0 = ct * S::BJ;
     const int64_t b = blockIdx.y;
     f32x4 acc[S::MI][S::MJ];
-    OperandA<f16, false, S> A;
-    A.order = nullptr; A.ld = a.lda; A.row0 = i0; A.rows = a.I - i0; A.klen = a.K; A.cols = 0;
-    OperandB<f16, BK, S> B;
-    B.order = nullptr; B.ld = a.ldb; B.klen = a.K;
-    B.row0 = BK ? 0 : j0; B.rows = BK ? 0 : a.J - j0; B.cols = BK ? a.J - j0 : 0;
+    Product<f16, false, BK, S, true> p;
+    p.A.order = nullptr; p.A.ld = a.lda; p.A.row0 = i0; p.A.rows = a.I - i0; p.A.klen = a.K; p.A.cols = 0;
+    p.B.order = nullptr; p.B.ld = a.ldb; p.B.klen = a.K;
+    p.B.row0 = BK ? 0 : j0; p.B.rows = BK ? 0 : a.J - j0; p.B.cols = BK ? a.J - j0 : 0;
     const int64_t boff = b * a.sb + (BK ? j0 : 0);
     // the small parts first, so that they are added before the large ones
-    A.base = a.al + b * a.sa; B.base = a.bh + boff;
-    tile_product<f16, false, BK, S, true>(A, B, a.K, lds, acc);
-    A.base = a.ah + b * a.sa; B.base = a.bl + boff;
-    tile_product<f16, false, BK, S, true, true>(A, B, a.K, lds, acc);
-    A.base = a.ah + b * a.sa; B.base = a.bh + boff;
-    tile_product<f16, false, BK, S, true, true>(A, B, a.K, lds, acc);
+    p.A.base = a.al + b * a.sa; p.B.base = a.bh + boff;
+    p.start(a.K, lds);
+    p.run(lds, acc);
+    p.A.base = a.ah + b * a.sa; p.B.base = a.bl + boff;
+    p.start(a.K, lds);
+    p.template run<true>(lds, acc);
+    p.A.base = a.ah + b * a.sa; p.B.base = a.bh + boff;
+    p.start(a.K, lds);
+    p.template run<true>(lds, acc);
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int li = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), lj = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);

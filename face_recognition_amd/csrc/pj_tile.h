@@ -120,7 +120,6 @@ static __device__ __attribute__((aligned(16))) const float pj_zeros[4] = {0.0f, 
 // One operand of a workgroup's tile: where its chunks come from and how a wave reads its fragments.
 //   row-major: `rows` tile rows start at row0 of a row list (`order`, or the rows themselves), each `klen` long from k = 0;
 //   k-major: columns 0 .. cols of `base`, whose rows row0 .. row0 + klen are summed over.
-// Chunks outside are zeros.
 template <typename T, bool KMAJOR, int DIM, int NT, int KS> struct Operand {
     static constexpr int EPC = Elem<T>::EPC, KSTEP = KS * Elem<T>::KG;
     static constexpr int CPR = KMAJOR ? DIM / EPC : 4 * KS;         // chunks per LDS row
@@ -140,8 +139,8 @@ template <typename T, bool KMAJOR, int DIM, int NT, int KS> struct Operand {
     struct Src {
         const T* p[NLD];
     };
-    // row-major: rows >= 1; tile row r stands for list entry row0 + min(r, rows - 1) (rows past the end repeat the last: their
-    // results are not stored)
+    // row-major: rows >= 1; tile row r stands for list entry row0 + min(r, rows - 1).  k-major: a chunk past `cols` stands for the
+    // first one.  (Rows and columns past the end belong to results that are not stored; only k past `klen` has to be zero.)
     __device__ __forceinline__ void init(Src& d, int tid) const {
 #pragma unroll
         for (int j = 0; j < NLD; ++j) {
@@ -150,15 +149,20 @@ template <typename T, bool KMAJOR, int DIM, int NT, int KS> struct Operand {
                 const int at = row0 + (r < rows ? r : rows - 1);
                 d.p[j] = base + (int64_t)(order ? order[at] : at) * ld + swz_row_major<KS>(r, tid % CPR) * EPC;
             } else {
-                d.p[j] = base + (int64_t)(row0 + r) * ld + swz_k_major<T, CPR>(r, tid % CPR) * EPC;
+                const int col = swz_k_major<T, CPR>(r, tid % CPR) * EPC;
+                d.p[j] = base + (int64_t)(row0 + r) * ld + (col < cols ? col : 0);
             }
         }
     }
-    // elements of the lane's chunk of pass j that are inside at `step` (<= 0: none)
+    // elements of the lane's chunk of pass j that are inside at `step` (<= 0: none); k-major: of the chunk it stands for
     __device__ __forceinline__ int valid(int j, int step, int tid) const {
         const int r = j * RPP + tid / CPR;
-        if constexpr (!KMAJOR) return klen - step * KSTEP - swz_row_major<KS>(r, tid % CPR) * EPC;
-        else return step * KSTEP + r < klen ? cols - swz_k_major<T, CPR>(r, tid % CPR) * EPC : 0;
+        if constexpr (!KMAJOR) {
+            return klen - step * KSTEP - swz_row_major<KS>(r, tid % CPR) * EPC;
+        } else {
+            const int col = swz_k_major<T, CPR>(r, tid % CPR) * EPC;
+            return step * KSTEP + r < klen ? cols - (col < cols ? col : 0) : 0;
+        }
     }
     __device__ __forceinline__ int64_t advance(int step) const {
         if constexpr (!KMAJOR) return (int64_t)step * KSTEP;
@@ -176,11 +180,13 @@ template <typename T, bool KMAJOR, int DIM, int NT, int KS> struct Operand {
     }
     // ---- staging by DMA: every chunk is wholly inside or outside (klen or cols, pitch and base multiples of 16 bytes)
     __device__ __forceinline__ void issue(const Src& d, int step, LdsPtr lds, int tid) const {
+        if ((step + 1) * KSTEP <= klen) {
 #pragma unroll
-        for (int j = 0; j < NLD; ++j) {
-            const T* p = d.p[j] + advance(step);
-            if (valid(j, step, tid) <= 0) p = reinterpret_cast<const T*>(pj_zeros);
-            dma16(p, lds + j * (NT * 16));
+            for (int j = 0; j < NLD; ++j) dma16(d.p[j] + advance(step), lds + j * (NT * 16));
+        } else {
+#pragma unroll
+            for (int j = 0; j < NLD; ++j)
+                dma16(valid(j, step, tid) > 0 ? d.p[j] + advance(step) : reinterpret_cast<const T*>(pj_zeros), lds + j * (NT * 16));
         }
     }
     // fragment of the 16 rows / columns from `d0`, k group `ks` of the step
@@ -220,24 +226,42 @@ template <typename T, bool KMAJOR, int DIM, int NT, int KS> struct Operand {
 template <int BI_, int BJ_, int WI_, int WJ_, int KS_, int NB_> struct Shape {
     static constexpr int BI = BI_, BJ = BJ_, WI = WI_, WJ = WJ_, KS = KS_, NB = NB_, NT = 64 * WI * WJ;
     static constexpr int MI = BI / WI / 16, MJ = BJ / WJ / 16;
-    static constexpr int LDS = NB * (BI + BJ) * KS * 64;
+    static constexpr int STEP = (BI + BJ) * KS * 64, LDS = NB * STEP;
+    static constexpr int STRIPS = BI * BJ / MI * 4;     // tile_emit's
+    static constexpr int PER_CU = 163840 / LDS;         // workgroups that share a compute unit's LDS,
+    static constexpr int WAVES = PER_CU * NT / 256;     // and their waves per SIMD, for which the registers have to do
+    static_assert(STRIPS <= LDS, "");
 };
 template <typename T, bool KMAJOR, typename S> using OperandA = Operand<T, KMAJOR, S::BI, S::NT, S::KS>;
 template <typename T, bool KMAJOR, typename S> using OperandB = Operand<T, KMAJOR, S::BJ, S::NT, S::KS>;
 
+// Which tile of n_rt x n_ct a workgroup takes.  Workgroups are dealt out to the eight dies in turn, and each die has an L2 of its
+// own, so die b % 8 gets one consecutive eighth of the tiles, walked in bands of eight row tiles, column by column: what runs on
+// a die at a time is about square and reads each operand's panels once (with tiles dealt out row by row the dies together
+// fetched 105 MB through their L2s for a 4096 x 2048 x 1024 product whose operands are 12 MB).  Launch 8 ceil(tiles / 8)
+// workgroups at least; false: no tile left for this one.
+__device__ __forceinline__ bool tile_of_block(unsigned b, int64_t n_rt, int n_ct, int& rt, int& ct) {
+    const int64_t all = n_rt * n_ct, x = b & 7, i = b >> 3, q = all >> 3, r = all & 7;
+    if (i >= q + (x < r)) return false;
+    const int64_t id = x * q + (x < r ? x : r) + i, band = 8 * (int64_t)n_ct, first = id / band * 8;
+    const int in = (int)(id % band), rows = (int)(n_rt - first < 8 ? n_rt - first : 8);
+    rt = (int)first + in % rows;
+    ct = in / rows;
+    return true;
+}
+
 // Hands a workgroup's results on as 16-byte pieces of rows: a wave turns its accumulators through its own part of LDS, 16 rows
-// at a time (written as a lane's four neighbouring columns, pitch + 16 bytes: no bank conflicts; read as V neighbouring
-// columns, so that eight or sixteen lanes cover a row's whole line), and calls
-//     pre(i, j)           for every piece first (loads that the results wait for go out together), then
+// at a time (written as a lane's four neighbouring columns, chunk c of row r at c ^ r; read as V neighbouring columns, so that
+// the lanes side by side cover a row's whole lines), and calls
+//     pre(i, j)             for every piece first (loads that the results wait for go out together), then
 //     emit(state, i, j, v)  with the V = 16 / sizeof(T) values of row i, columns j .. j + V of the tile.
-// `lds` is free when every wave is past the last step's barrier.
-template <typename T, typename S, typename F> __device__ __forceinline__ void tile_emit(const f32x4 (&acc)[S::MI][S::MJ], char* lds, const F& f) {
-    constexpr int COLS = S::MJ * 16, V = 16 / sizeof(T), LPR = COLS / V, RPP = 64 / LPR, NP = 16 / RPP, PITCH = COLS + 4;
-    static_assert(S::WI * S::WJ * 16 * PITCH * 4 <= S::LDS, "the strips fit the tiles' buffers");
-    static_assert(16 % RPP == 0, "whole passes per strip");
+// `strips`: S::STRIPS bytes that nobody else uses any more.
+template <typename T, typename S, typename F> __device__ __forceinline__ void tile_emit(const f32x4 (&acc)[S::MI][S::MJ], char* strips, const F& f) {
+    constexpr int COLS = S::MJ * 16, CH = COLS / 4, V = 16 / sizeof(T), LPR = COLS / V, RPP = 64 / LPR, NP = 16 / RPP;
+    static_assert(16 % RPP == 0 && (CH & (CH - 1)) == 0, "whole passes per strip");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
-    float* strip = reinterpret_cast<float*>(lds) + wave * (16 * PITCH);
+    f32x4* strip = reinterpret_cast<f32x4*>(strips) + wave * (16 * CH);
     const int r = lane / LPR, c = (lane % LPR) * V;
     typename F::Pre pre[S::MI * NP];
 #pragma unroll
@@ -247,19 +271,19 @@ template <typename T, typename S, typename F> __device__ __forceinline__ void ti
 #pragma unroll
     for (int mi = 0; mi < S::MI; ++mi) {
 #pragma unroll
-        for (int mj = 0; mj < S::MJ; ++mj)
-            *reinterpret_cast<f32x4*>(strip + (lane & 15) * PITCH + 16 * mj + 4 * (lane >> 4)) = acc[mi][mj];
+        for (int mj = 0; mj < S::MJ; ++mj) strip[(lane & 15) * CH + ((4 * mj + (lane >> 4)) ^ (lane & (CH - 1) & 15))] = acc[mi][mj];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
+            const int row = p * RPP + r;
             float v[V];
 #pragma unroll
             for (int q = 0; q < V / 4; ++q) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(strip + (p * RPP + r) * PITCH + c + 4 * q);
+                const f32x4 x = strip[row * CH + ((c / 4 + q) ^ (row & (CH - 1)))];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e];
             }
-            f.emit(pre[mi * NP + p], i0 + 16 * mi + p * RPP + r, j0 + c, v);
+            f.emit(pre[mi * NP + p], i0 + 16 * mi + row, j0 + c, v);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
@@ -284,82 +308,96 @@ __device__ __forceinline__ void tile_step(const char* ta, const char* tb, int i0
     }
 }
 
-// acc[mi][mj][r] = C[i][j] with i = 16 mi + (lane & 15), j = 16 mj + 4 (lane >> 4) + r inside the wave's part: the j side is
-// the MFMA's row operand, so a lane holds four neighbouring j of one i.  klen: the longer of the operands' (an operand's
-// chunks past its own are zeros).  ADD: on top of what acc holds.
-// DMA: the next NB - 1 steps are on their way while one runs; one barrier per step says both that the step has arrived for
-// every wave and that every wave has left the buffer the next load goes to.  Otherwise the next step waits in registers.
-// On return every wave is past its last LDS read.
-template <typename T, bool AK, bool BK, typename S, bool DMA, bool ADD = false>
-__device__ __forceinline__ void tile_product(const OperandA<T, AK, S>& A, const OperandB<T, BK, S>& B, int klen, char* lds,
-                                             f32x4 (&acc)[S::MI][S::MJ]) {
+// The product of a tile in two parts, between which a kernel sends for what it needs afterwards:
+//   start   fetches the addresses and (DMA) issues the first NB - 1 steps; every wave is past its reads of those buffers;
+//   run     acc[mi][mj][r] = C[i][j] with i = 16 mi + (lane & 15), j = 16 mj + 4 (lane >> 4) + r inside the wave's part: the j side
+//           is the MFMA's row operand, so a lane holds four neighbouring j of one i.  ADD: on top of what acc holds.
+//           On return every wave is past its last LDS read.
+// klen: the longer of the operands' (an operand's chunks past its own are zeros).  DMA: the next NB - 1 steps are on their way
+// while one runs; one barrier per step says both that the step has arrived for every wave and that every wave has left the buffer
+// the next load goes to.  Otherwise the next step waits in registers.
+template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
     typedef OperandA<T, AK, S> OA;
     typedef OperandB<T, BK, S> OB;
-    constexpr int BUF = OA::BYTES + OB::BYTES, NB = S::NB;
-    static_assert(BUF * NB == S::LDS && NB >= 2 && NB <= 5, "");
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (!ADD) {
-#pragma unroll
-        for (int mi = 0; mi < S::MI; ++mi)
-#pragma unroll
-            for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
-    }
-    const int steps = (klen + OA::KSTEP - 1) / OA::KSTEP;
-    if (steps == 0) return;
+    static constexpr int NB = S::NB, BUF = S::STEP, NLD = OA::NLD + OB::NLD;
+    static_assert(OA::BYTES + OB::BYTES == BUF && NB >= 2 && NB <= 5, "");
+    OA A;
+    OB B;
     typename OA::Src sa;
     typename OB::Src sb;
-    A.init(sa, tid);
-    B.init(sb, tid);
+    int steps;
 
-    if constexpr (DMA) {
-        constexpr int NLD = OA::NLD + OB::NLD;
-        const LdsPtr dst = (LdsPtr)lds + __builtin_amdgcn_readfirstlane(wave) * 1024;
+    __device__ __forceinline__ static LdsPtr dma_base(char* lds) {
+        return (LdsPtr)lds + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * 1024;
+    }
+    __device__ __forceinline__ void start(int klen, char* lds) {
+        const int tid = threadIdx.x;
+        steps = (klen + OA::KSTEP - 1) / OA::KSTEP;
+        if (steps == 0) return;
+        A.init(sa, tid);
+        B.init(sb, tid);
+        if constexpr (DMA) {
+            const LdsPtr dst = dma_base(lds);
 #pragma unroll
-        for (int t = 0; t < NB - 1; ++t)
-            if (t < steps) {
-                A.issue(sa, t, dst + t * BUF, tid);
-                B.issue(sb, t, dst + t * BUF + OA::BYTES, tid);
-            }
-        int cur = 0, nxt = (NB - 1) * BUF;
-        for (int t = 0; t < steps; ++t) {
-            const int behind = steps - 1 - t;       // steps after this one, at most NB - 2 of them on their way
-            if (behind >= NB - 2) dma_wait_barrier<(NB - 2) * NLD>();
-            else if (NB > 4 && behind == 2) dma_wait_barrier<2 * NLD>();
-            else if (NB > 3 && behind == 1) dma_wait_barrier<NLD>();
-            else dma_wait_barrier<0>();
-            if (t + NB - 1 < steps) {
-                A.issue(sa, t + NB - 1, dst + nxt, tid);
-                B.issue(sb, t + NB - 1, dst + nxt + OA::BYTES, tid);
-            }
-            tile_step<T, AK, BK, S>(lds + cur, lds + cur + OA::BYTES, i0, j0, lane, acc);
-            nxt = cur;
-            cur = cur + BUF == NB * BUF ? 0 : cur + BUF;
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    } else {
-        typename Elem<T>::Frag va[OA::NLD], vb[OB::NLD];
-        A.load(sa, va, 0, tid);
-        B.load(sb, vb, 0, tid);
-        OA::store(lds, va, tid);
-        OB::store(lds + OA::BYTES, vb, tid);
-        __syncthreads();
-        for (int t = 0; t < steps; ++t) {
-            const char* ta = lds + (t & 1) * BUF;
-            if (t + 1 < steps) {
-                A.load(sa, va, t + 1, tid);
-                B.load(sb, vb, t + 1, tid);
-            }
-            tile_step<T, AK, BK, S>(ta, ta + OA::BYTES, i0, j0, lane, acc);
-            if (t + 1 < steps) {
-                char* na = lds + ((t + 1) & 1) * BUF;
-                OA::store(na, va, tid);
-                OB::store(na + OA::BYTES, vb, tid);
-            }
-            __syncthreads();
+            for (int t = 0; t < NB - 1; ++t)
+                if (t < steps) {
+                    A.issue(sa, t, dst + t * BUF, tid);
+                    B.issue(sb, t, dst + t * BUF + OA::BYTES, tid);
+                }
         }
     }
-}
+    template <bool ADD = false> __device__ __forceinline__ void run(char* lds, f32x4 (&acc)[S::MI][S::MJ]) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (!ADD) {
+#pragma unroll
+            for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+                for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
+        }
+        if (steps == 0) return;
+        if constexpr (DMA) {
+            const LdsPtr dst = dma_base(lds);
+            int cur = 0, nxt = (NB - 1) * BUF;
+            for (int t = 0; t < steps; ++t) {
+                const int behind = steps - 1 - t;       // steps after this one, at most NB - 2 of them on their way
+                if (behind >= NB - 2) dma_wait_barrier<(NB - 2) * NLD>();
+                else if (NB > 4 && behind == 2) dma_wait_barrier<2 * NLD>();
+                else if (NB > 3 && behind == 1) dma_wait_barrier<NLD>();
+                else dma_wait_barrier<0>();
+                if (t + NB - 1 < steps) {
+                    A.issue(sa, t + NB - 1, dst + nxt, tid);
+                    B.issue(sb, t + NB - 1, dst + nxt + OA::BYTES, tid);
+                }
+                tile_step<T, AK, BK, S>(lds + cur, lds + cur + OA::BYTES, i0, j0, lane, acc);
+                nxt = cur;
+                cur = cur + BUF == NB * BUF ? 0 : cur + BUF;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        } else {
+            typename Elem<T>::Frag va[OA::NLD], vb[OB::NLD];
+            A.load(sa, va, 0, tid);
+            B.load(sb, vb, 0, tid);
+            OA::store(lds, va, tid);
+            OB::store(lds + OA::BYTES, vb, tid);
+            __syncthreads();
+            for (int t = 0; t < steps; ++t) {
+                const char* ta = lds + (t & 1) * BUF;
+                if (t + 1 < steps) {
+                    A.load(sa, va, t + 1, tid);
+                    B.load(sb, vb, t + 1, tid);
+                }
+                tile_step<T, AK, BK, S>(ta, ta + OA::BYTES, i0, j0, lane, acc);
+                if (t + 1 < steps) {
+                    char* na = lds + ((t + 1) & 1) * BUF;
+                    OA::store(na, va, tid);
+                    OB::store(na + OA::BYTES, vb, tid);
+                }
+                __syncthreads();
+            }
+        }
+    }
+};
 
 }  // namespace fra
