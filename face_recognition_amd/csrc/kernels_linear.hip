@@ -91,81 +91,71 @@ struct FwdArgs {
     int K, N, act, bias_f32, slope_f32, n_col_tiles;
 };
 
-// A lane's columns are the same in all its pieces, so bias and slope sit in registers.  FULL: the tile's columns are all inside
-// and ACT is the activation, so that the pieces are straight-line code whose loads and arithmetic overlap (with a guard around
-// every access and the activation chosen per piece a 262144 x 512 x 512 product took 316 us, see pj_forward_kernel); otherwise
-// everything is checked, and ACT is not used.
-template <typename T> struct LaneParams {
+// A lane's columns are the same in all its pieces, so bias and slope sit in registers, sent for before the product (as they lie
+// in memory: a conversion there would wait for them) and converted after it.
+template <typename T> struct LaneParam {
     static constexpr int V = 16 / sizeof(T);
-    float bi[V], sl[V];
-    __device__ __forceinline__ void load(const FwdArgs& a, int64_t at, int left, bool live) {
+    f32x4 raw[V / 4];
+    __device__ __forceinline__ void load(const void* p, int is_f32, int64_t at, int left) {
+        if (is_f32) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) bi[e] = sl[e] = 0.0f;
-        if (a.bias && live) vec(a.bias, a.bias_f32, at, left, bi);
-        if (a.slope && live) vec(a.slope, a.slope_f32, at, left, sl);
-    }
-    __device__ __forceinline__ static void vec(const void* p, int is_f32, int64_t at, int left, float (&o)[V]) {
-#pragma unroll
-        for (int q = 0; q < V; q += 4) {
-            float t[4];
-            load_param4<T>(p, is_f32, at + q, left - q, t);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[q + e] = t[e];
+            for (int q = 0; q < V / 4; ++q) raw[q] = load_chunk<float>((const float*)p + at + 4 * q, left - 4 * q);
+        } else {
+            raw[0] = __builtin_bit_cast(f32x4, load_chunk<T>((const T*)p + at, left));
         }
+    }
+    __device__ __forceinline__ void get(bool there, int is_f32, float (&o)[V]) const {
+        const typename Elem<T>::Frag h = __builtin_bit_cast(typename Elem<T>::Frag, raw[0]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = !there ? 0.0f : is_f32 ? raw[e / 4][e % 4] : (float)h[e];
     }
 };
+// FULL: the tile's columns are all inside and ACT is the activation, so that the pieces are straight-line code whose loads and
+// arithmetic overlap; otherwise everything is checked, and ACT is not used.
 template <typename T, int ACT, bool FULL> struct ForwardEmit {
     static constexpr int V = 16 / sizeof(T);
-    typedef typename Elem<T>::Frag Frag;
-    struct Pre {
-        int row;                    // -1: nothing to store
-        Frag r;
-    };
-    const FwdArgs& a;
-    const LaneParams<T>& par;
-    int begin, count, n0, left;     // left: valid columns from the lane's first
+    typedef typename Elem<T>::Frag Frag, Pre;
+    const T* resid;
+    T *z, *y;
+    int64_t ldr, N;
+    const int* order;
+    int begin, count, n0, left, act;    // left: valid columns from the lane's first
     bool live;
-    __device__ __forceinline__ Pre pre(int i, int j) const {
-        Pre p;
-        if constexpr (FULL) {
-            const int at = begin + (i < count ? i : count - 1);
-            p.row = a.rows.order ? a.rows.order[at] : at;
-            if (a.resid) p.r = load_chunk<T>((const T*)a.resid + (int64_t)p.row * a.ldr + n0 + j, V);
-            if (i >= count) p.row = -1;
-        } else {
-            p.row = -1;
-            if (i < count && left > 0) {
-                p.row = a.rows.order ? a.rows.order[begin + i] : begin + i;
-                if (a.resid) p.r = load_chunk<T>((const T*)a.resid + (int64_t)p.row * a.ldr + n0 + j, left);
-            }
-        }
-        return p;
+    float bi[V], sl[V];
+    // list entry of tile row i, the last row's past the end; -1 - entry where nothing is stored
+    __device__ __forceinline__ int row(int i) const {
+        const int at = begin + (i < count ? i : count - 1);
+        const int r = order ? order[at] : at;
+        return i < count && (FULL || left > 0) ? r : -1 - r;
     }
-    __device__ __forceinline__ void emit(const Pre& p, int, int j, float (&v)[V]) const {
-        const int64_t at = (int64_t)p.row * a.N + n0 + j;
+    __device__ __forceinline__ Frag pre(int row, int j) const {
+        Frag r = {};
+        if (resid) r = load_chunk<T>(resid + (int64_t)(row < 0 ? -1 - row : row) * ldr + n0 + j, FULL ? V : left);
+        return r;
+    }
+    __device__ __forceinline__ void emit(int row, int j, const Frag& r, float (&v)[V]) const {
+        const int64_t at = (int64_t)row * N + n0 + j;
         const int n = FULL ? V : left;
         Frag o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] += par.bi[e];
-        if (a.z && live && p.row >= 0) {
+        for (int e = 0; e < V; ++e) v[e] += bi[e];
+        if (z && live && row >= 0) {
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = (T)v[e];
-            store_chunk<T>((T*)a.z + at, n, o);
+            store_chunk<T>(z + at, n, o);
         }
-        if constexpr (FULL) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = pj_act<T>(ACT, v[e], par.sl[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = live ? pj_act<T>(a.act, v[e], par.sl[e]) : 0.0f;
+        for (int e = 0; e < V; ++e) {
+            if constexpr (FULL) v[e] = pj_act<T>(ACT, v[e], sl[e]);
+            else v[e] = live ? pj_act<T>(act, v[e], sl[e]) : 0.0f;
         }
-        if (a.resid) {
+        if (resid) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] += (float)p.r[e];
+            for (int e = 0; e < V; ++e) v[e] += (float)r[e];
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = (T)v[e];
-        if (p.row >= 0) store_chunk<T>((T*)a.y + at, n, o);
+        if (row >= 0) store_chunk<T>(y + at, n, o);
     }
 };
 // A tile of rows x columns as the product kernels see it
@@ -194,15 +184,25 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT, 
     p.start(t.live ? a.K : 0, lds);
     const int col = (threadIdx.x >> 6) / S::WI * (S::BJ / S::WJ) + (int)(threadIdx.x & 63) % (S::MJ * 16 / V) * V;
     const int left = a.N - t.c0 - col;
-    LaneParams<T> par;                                              // on their way while the product runs
-    par.load(a, (int64_t)t.g * a.N + t.c0 + col, left, t.live);
+    const int64_t at = (int64_t)t.g * a.N + t.c0 + col;
+    const bool has_bias = a.bias && t.live, has_slope = a.slope && t.live;
+    LaneParam<T> bias, slope;
+    if (has_bias) bias.load(a.bias, a.bias_f32, at, left);
+    if (has_slope) slope.load(a.slope, a.slope_f32, at, left);
     p.run(lds, acc);
+    auto finish = [&](auto f) {
+        f.resid = (const T*)a.resid; f.z = (T*)a.z; f.y = (T*)a.y; f.ldr = a.ldr; f.N = a.N; f.order = a.rows.order;
+        f.begin = t.begin; f.count = t.end - t.begin; f.n0 = t.c0; f.left = left; f.act = a.act; f.live = t.live;
+        bias.get(has_bias, a.bias_f32, f.bi);
+        slope.get(has_slope, a.slope_f32, f.sl);
+        tile_emit<T, S>(acc, lds, f);
+    };
     switch (t.live && t.c0 + S::BJ <= a.N ? a.act : -1) {
 #define PJ_CASE(A) \
-    case A: tile_emit<T, S>(acc, lds, ForwardEmit<T, A, true>{a, par, t.begin, t.end - t.begin, t.c0, left, true}); break;
+    case A: finish(ForwardEmit<T, A, true>()); break;
         PJ_CASE(PJ_NONE) PJ_CASE(PJ_RELU) PJ_CASE(PJ_PRELU) PJ_CASE(PJ_SILU) PJ_CASE(PJ_GELU_TANH)
 #undef PJ_CASE
-        default: tile_emit<T, S>(acc, lds, ForwardEmit<T, 0, false>{a, par, t.begin, t.end - t.begin, t.c0, left, t.live});
+        default: finish(ForwardEmit<T, 0, false>());
     }
 }
 
@@ -284,11 +284,12 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef Product<T, false, true, S, true> P;
     struct Emit {
-        typedef int Pre;
+        struct Pre {};
         const DxArgs& a;
         Tile t;
-        __device__ __forceinline__ int pre(int i, int) const { return t.begin + i < t.end ? (a.rows.order ? a.rows.order[t.begin + i] : t.begin + i) : -1; }
-        __device__ __forceinline__ void emit(int row, int, int j, float (&v)[16 / sizeof(T)]) const {
+        __device__ __forceinline__ int row(int i) const { return t.begin + i < t.end ? (a.rows.order ? a.rows.order[t.begin + i] : t.begin + i) : -1; }
+        __device__ __forceinline__ Pre pre(int, int) const { return {}; }
+        __device__ __forceinline__ void emit(int row, int j, Pre, float (&v)[16 / sizeof(T)]) const {
             const int left = a.K - t.c0 - j;
             if (row < 0 || left <= 0) return;
             typename Elem<T>::Frag o;
@@ -318,12 +319,13 @@ struct DwArgs {
     int K, Kp, N, Np, n_ti, n_tj, splits;
 };
 template <typename O> struct DwEmit {
-    typedef int Pre;
+    struct Pre {};
     O* out;
     int N, K, n0, k0;
-    __device__ __forceinline__ int pre(int, int) const { return 0; }
-    __device__ __forceinline__ void emit(int, int i, int j, float (&v)[16 / sizeof(O)]) const {
-        const int n = n0 + i, left = K - k0 - j;
+    __device__ __forceinline__ int row(int i) const { return n0 + i; }
+    __device__ __forceinline__ Pre pre(int, int) const { return {}; }
+    __device__ __forceinline__ void emit(int n, int j, Pre, float (&v)[16 / sizeof(O)]) const {
+        const int left = K - k0 - j;
         if (n >= N || left <= 0) return;
         typename Elem<O>::Frag o;
 #pragma unroll

@@ -240,21 +240,22 @@ template <typename T, bool KMAJOR, typename S> using OperandB = Operand<T, KMAJO
 // a die at a time is about square and reads each operand's panels once (with tiles dealt out row by row the dies together
 // fetched 105 MB through their L2s for a 4096 x 2048 x 1024 product whose operands are 12 MB).  Launch 8 ceil(tiles / 8)
 // workgroups at least; false: no tile left for this one.
-__device__ __forceinline__ bool tile_of_block(unsigned b, int64_t n_rt, int n_ct, int& rt, int& ct) {
-    const int64_t all = n_rt * n_ct, x = b & 7, i = b >> 3, q = all >> 3, r = all & 7;
+__device__ __forceinline__ bool tile_of_block(unsigned b, unsigned n_rt, unsigned n_ct, int& rt, int& ct) {
+    const unsigned all = n_rt * n_ct, x = b & 7, i = b >> 3, q = all >> 3, r = all & 7;         // below 2^31 (the launchers check)
     if (i >= q + (x < r)) return false;
-    const int64_t id = x * q + (x < r ? x : r) + i, band = 8 * (int64_t)n_ct, first = id / band * 8;
-    const int in = (int)(id % band), rows = (int)(n_rt - first < 8 ? n_rt - first : 8);
-    rt = (int)first + in % rows;
-    ct = in / rows;
+    const unsigned id = x * q + (x < r ? x : r) + i, band = 8 * n_ct, first = id / band * 8;
+    const unsigned in = id - first * n_ct, rows = n_rt - first < 8 ? n_rt - first : 8;
+    ct = (int)(in / rows);
+    rt = (int)(first + in - ct * rows);
     return true;
 }
 
 // Hands a workgroup's results on as 16-byte pieces of rows: a wave turns its accumulators through its own part of LDS, 16 rows
 // at a time (written as a lane's four neighbouring columns, chunk c of row r at c ^ r; read as V neighbouring columns, so that
 // the lanes side by side cover a row's whole lines), and calls
-//     pre(i, j)             for every piece first (loads that the results wait for go out together), then
-//     emit(state, i, j, v)  with the V = 16 / sizeof(T) values of row i, columns j .. j + V of the tile.
+//     row(i)              where row i of the tile goes, for the pieces of two strips first, then
+//     pre(row, j)         for the same pieces, so that loads that the results wait for go out together, then
+//     emit(row, j, state, v)  with the V = 16 / sizeof(T) values of columns j .. j + V of the tile.
 // `strips`: S::STRIPS bytes that nobody else uses any more.
 template <typename T, typename S, typename F> __device__ __forceinline__ void tile_emit(const f32x4 (&acc)[S::MI][S::MJ], char* strips, const F& f) {
     constexpr int COLS = S::MJ * 16, CH = COLS / 4, V = 16 / sizeof(T), LPR = COLS / V, RPP = 64 / LPR, NP = 16 / RPP;
@@ -263,64 +264,72 @@ template <typename T, typename S, typename F> __device__ __forceinline__ void ti
     const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
     f32x4* strip = reinterpret_cast<f32x4*>(strips) + wave * (16 * CH);
     const int r = lane / LPR, c = (lane % LPR) * V;
-    typename F::Pre pre[S::MI * NP];
+    constexpr int MG = S::MI < 2 ? S::MI : 2;                       // strips whose loads go out together
+    static_assert(S::MI % MG == 0, "");
 #pragma unroll
-    for (int mi = 0; mi < S::MI; ++mi)
+    for (int m0 = 0; m0 < S::MI; m0 += MG) {
+        int rows[MG * NP];
+        typename F::Pre pre[MG * NP];
 #pragma unroll
-        for (int p = 0; p < NP; ++p) pre[mi * NP + p] = f.pre(i0 + 16 * mi + p * RPP + r, j0 + c);
+        for (int k = 0; k < MG * NP; ++k) rows[k] = f.row(i0 + 16 * m0 + k * RPP + r);
 #pragma unroll
-    for (int mi = 0; mi < S::MI; ++mi) {
+        for (int k = 0; k < MG * NP; ++k) pre[k] = f.pre(rows[k], j0 + c);
 #pragma unroll
-        for (int mj = 0; mj < S::MJ; ++mj) strip[(lane & 15) * CH + ((4 * mj + (lane >> 4)) ^ (lane & (CH - 1) & 15))] = acc[mi][mj];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int mi = 0; mi < MG; ++mi) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            const int row = p * RPP + r;
-            float v[V];
+            for (int mj = 0; mj < S::MJ; ++mj) strip[(lane & 15) * CH + ((4 * mj + (lane >> 4)) ^ (lane & (CH - 1) & 15))] = acc[m0 + mi][mj];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-            for (int q = 0; q < V / 4; ++q) {
-                const f32x4 x = strip[row * CH + ((c / 4 + q) ^ (row & (CH - 1)))];
+            for (int p = 0; p < NP; ++p) {
+                const int row = p * RPP + r;
+                float v[V];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e];
+                for (int q = 0; q < V / 4; ++q) {
+                    const f32x4 x = strip[row * CH + ((c / 4 + q) ^ (row & (CH - 1)))];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[4 * q + e] = x[e];
+                }
+                f.emit(rows[mi * NP + p], j0 + c, pre[mi * NP + p], v);
             }
-            f.emit(pre[mi * NP + p], i0 + 16 * mi + row, j0 + c, v);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
-// The MFMAs of one step on the tiles in LDS.
-template <typename T, bool AK, bool BK, typename S>
-__device__ __forceinline__ void tile_step(const char* ta, const char* tb, int i0, int j0, int lane, f32x4 (&acc)[S::MI][S::MJ]) {
-    typedef OperandA<T, AK, S> OA;
-    typedef OperandB<T, BK, S> OB;
+// A wave's operands of one group of k, and the MFMAs on them.
+template <typename T, bool AK, bool BK, typename S> struct Frags {
+    typename Elem<T>::Frag a[S::MI], b[S::MJ];
+    __device__ __forceinline__ void read(const char* step, int ks, int i0, int j0, int lane) {
+        typedef OperandA<T, AK, S> OA;
+        typedef OperandB<T, BK, S> OB;
 #pragma unroll
-    for (int ks = 0; ks < S::KS; ++ks) {
-        typename Elem<T>::Frag fa[S::MI], fb[S::MJ];
+        for (int mi = 0; mi < S::MI; ++mi) a[mi] = OA::frag(step, i0 + 16 * mi, ks, lane);
 #pragma unroll
-        for (int mi = 0; mi < S::MI; ++mi) fa[mi] = OA::frag(ta, i0 + 16 * mi, ks, lane);
-#pragma unroll
-        for (int mj = 0; mj < S::MJ; ++mj) fb[mj] = OB::frag(tb, j0 + 16 * mj, ks, lane);
+        for (int mj = 0; mj < S::MJ; ++mj) b[mj] = OB::frag(step + OA::BYTES, j0 + 16 * mj, ks, lane);
+    }
+    __device__ __forceinline__ void mma(f32x4 (&acc)[S::MI][S::MJ]) const {
 #pragma unroll
         for (int mi = 0; mi < S::MI; ++mi)
 #pragma unroll
-            for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = pj_mma<T>(fb[mj], fa[mi], acc[mi][mj]);
+            for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = pj_mma<T>(b[mj], a[mi], acc[mi][mj]);
     }
-}
+};
 
 // The product of a tile in two parts, between which a kernel sends for what it needs afterwards:
-//   start   fetches the addresses and (DMA) issues the first NB - 1 steps; every wave is past its reads of those buffers;
+//   start   fetches the addresses and (DMA) issues the first NB steps; every wave is past its reads of those buffers;
 //   run     acc[mi][mj][r] = C[i][j] with i = 16 mi + (lane & 15), j = 16 mj + 4 (lane >> 4) + r inside the wave's part: the j side
 //           is the MFMA's row operand, so a lane holds four neighbouring j of one i.  ADD: on top of what acc holds.
 //           On return every wave is past its last LDS read.
-// klen: the longer of the operands' (an operand's chunks past its own are zeros).  DMA: the next NB - 1 steps are on their way
-// while one runs; one barrier per step says both that the step has arrived for every wave and that every wave has left the buffer
-// the next load goes to.  Otherwise the next step waits in registers.
+// klen: the longer of the operands' (an operand's chunks past its own are zeros).
+// DMA: steps are NB deep in LDS.  A wave reads the second half of a step while the matrix cores work on the first, and the first
+// half of the next step while they work on the second; between the two lies the one barrier of a step, which says that the next
+// step has arrived for every wave and that every wave has read all of this one, whose buffer the load of step t + NB then takes.
+// Otherwise the next step waits in registers.
 template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
     typedef OperandA<T, AK, S> OA;
     typedef OperandB<T, BK, S> OB;
     static constexpr int NB = S::NB, BUF = S::STEP, NLD = OA::NLD + OB::NLD;
-    static_assert(OA::BYTES + OB::BYTES == BUF && NB >= 2 && NB <= 5, "");
+    static_assert(OA::BYTES + OB::BYTES == BUF && NB >= 2 && NB <= 4 && S::KS == 2, "");
     OA A;
     OB B;
     typename OA::Src sa;
@@ -339,12 +348,20 @@ template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
         if constexpr (DMA) {
             const LdsPtr dst = dma_base(lds);
 #pragma unroll
-            for (int t = 0; t < NB - 1; ++t)
+            for (int t = 0; t < NB; ++t)
                 if (t < steps) {
                     A.issue(sa, t, dst + t * BUF, tid);
                     B.issue(sb, t, dst + t * BUF + OA::BYTES, tid);
                 }
         }
+    }
+    // the oldest step on its way has arrived for every wave: at most Y younger ones are still out, fewer if fewer than that
+    // (`behind`) come after it
+    template <int Y> __device__ __forceinline__ static void arrived(int behind) {
+        if (behind >= Y) dma_wait_barrier<Y * NLD>();
+        else if (Y > 2 && behind == 2) dma_wait_barrier<2 * NLD>();
+        else if (Y > 1 && behind == 1) dma_wait_barrier<NLD>();
+        else dma_wait_barrier<0>();
     }
     template <bool ADD = false> __device__ __forceinline__ void run(char* lds, f32x4 (&acc)[S::MI][S::MJ]) const {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -359,20 +376,28 @@ template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
         if (steps == 0) return;
         if constexpr (DMA) {
             const LdsPtr dst = dma_base(lds);
-            int cur = 0, nxt = (NB - 1) * BUF;
+            Frags<T, AK, BK, S> f0, f1;
+            arrived<NB - 1>(steps - 1);
+            f0.read(lds, 0, i0, j0, lane);
+            int cur = 0;
             for (int t = 0; t < steps; ++t) {
-                const int behind = steps - 1 - t;       // steps after this one, at most NB - 2 of them on their way
-                if (behind >= NB - 2) dma_wait_barrier<(NB - 2) * NLD>();
-                else if (NB > 4 && behind == 2) dma_wait_barrier<2 * NLD>();
-                else if (NB > 3 && behind == 1) dma_wait_barrier<NLD>();
-                else dma_wait_barrier<0>();
-                if (t + NB - 1 < steps) {
-                    A.issue(sa, t + NB - 1, dst + nxt, tid);
-                    B.issue(sb, t + NB - 1, dst + nxt + OA::BYTES, tid);
+                f1.read(lds + cur, 1, i0, j0, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                f0.mma(acc);
+                __builtin_amdgcn_sched_barrier(0);
+                const int nxt = cur + BUF == NB * BUF ? 0 : cur + BUF;
+                if (t + 1 < steps) {
+                    arrived<NB - 2>(steps - 2 - t);
+                    if (t + NB < steps) {
+                        A.issue(sa, t + NB, dst + cur, tid);
+                        B.issue(sb, t + NB, dst + cur + OA::BYTES, tid);
+                    }
+                    f0.read(lds + nxt, 0, i0, j0, lane);
                 }
-                tile_step<T, AK, BK, S>(lds + cur, lds + cur + OA::BYTES, i0, j0, lane, acc);
-                nxt = cur;
-                cur = cur + BUF == NB * BUF ? 0 : cur + BUF;
+                __builtin_amdgcn_sched_barrier(0);
+                f1.mma(acc);
+                __builtin_amdgcn_sched_barrier(0);
+                cur = nxt;
             }
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         } else {
@@ -388,7 +413,12 @@ template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
                     A.load(sa, va, t + 1, tid);
                     B.load(sb, vb, t + 1, tid);
                 }
-                tile_step<T, AK, BK, S>(ta, ta + OA::BYTES, i0, j0, lane, acc);
+                Frags<T, AK, BK, S> f;
+#pragma unroll
+                for (int ks = 0; ks < S::KS; ++ks) {
+                    f.read(ta, ks, i0, j0, lane);
+                    f.mma(acc);
+                }
                 if (t + 1 < steps) {
                     char* na = lds + ((t + 1) & 1) * BUF;
                     OA::store(na, va, tid);
