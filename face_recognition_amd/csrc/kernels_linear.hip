@@ -50,18 +50,6 @@ template <typename T> __device__ __forceinline__ float pj_act_grad(int act, floa
     }
 }
 
-template <typename T, int V> __device__ __forceinline__ void pj_act_grad_all(int act, typename Elem<T>::Frag z, const float (&s)[V], float (&d)[V]) {
-    switch (act) {
-#define PJ_CASE(A)                                                \
-    case A:                                                       \
-        _Pragma("unroll") for (int e = 0; e < V; ++e) d[e] = pj_act_grad<T>(A, (float)z[e], s[e]); \
-        break;
-        PJ_CASE(PJ_RELU) PJ_CASE(PJ_PRELU) PJ_CASE(PJ_SILU) PJ_CASE(PJ_GELU_TANH)
-#undef PJ_CASE
-        default: break;
-    }
-}
-
 // what every product kernel knows about its rows
 struct RowArgs {
     const int* order;           // nullptr: the rows themselves
@@ -382,8 +370,8 @@ template <typename T> __global__ __launch_bounds__(256) void pj_join_kernel(cons
 }
 
 // dz = dy act'(z) in list order and, per row tile, the column sums of dz and of dy min(z, 0).  A workgroup takes one row tile x
-// `lpr` 16-byte pieces of columns (lpr lanes side by side, a power of two up to 64; 256 / lpr rows at a time); eight rows per
-// lane are requested together.  Bound by HBM: dy and z in, dz out.
+// `lpr` 16-byte pieces of columns (lpr lanes side by side, a power of two up to 16, so that narrow pieces make many workgroups;
+// 256 / lpr rows at a time); four rows per lane are requested together.  Bound by HBM: dy and z in, dz out.
 struct DzArgs {
     RowArgs rows;
     const void *dy, *z, *slope;
@@ -392,62 +380,71 @@ struct DzArgs {
     int64_t lddy;
     int N, Np, act, slope_f32, tile_rows, n_col_tiles, lpr_log2;
 };
-template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs a) {
+// ACT: the activation; FULL: every piece is whole (N = Np)
+template <typename T, int ACT, bool FULL> __device__ __forceinline__ void dz_rows(const DzArgs& a, int g, int begin, int end, int n, int sub, int nsub,
+                                                                                float (&sb)[Elem<T>::EPC], float (&ss)[Elem<T>::EPC]) {
     typedef typename Elem<T>::Frag Frag;
-    constexpr int V = Elem<T>::EPC, U = 8;
+    constexpr int V = Elem<T>::EPC, U = 4;
+    const int have = FULL ? V : a.N - n;
+    LaneParam<T> slope;
+    float sl[V];
+    if (ACT == PJ_PRELU) slope.load(a.slope, a.slope_f32, (int64_t)g * a.N + n, have);
+    for (int at0 = begin + sub; at0 < end; at0 += nsub * U) {
+        Frag dy[U], z[U];
+        int row[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = at0 + u * nsub;
+            row[u] = at < end ? at : at0;                           // rows past the end repeat the first, unused
+        }
+        if (a.rows.order) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) row[u] = a.rows.order[row[u]];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            dy[u] = load_chunk<T>((const T*)a.dy + (int64_t)row[u] * a.lddy + n, have);
+            if (ACT != PJ_NONE) z[u] = load_chunk<T>((const T*)a.z + (int64_t)row[u] * a.N + n, have);
+        }
+        if (ACT == PJ_PRELU) slope.get(true, a.slope_f32, sl);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = at0 + u * nsub;
+            if (at >= end) continue;
+            Frag d = dy[u];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float y = (float)dy[u][e], zv = ACT != PJ_NONE ? (float)z[u][e] : 0.0f;
+                const float dz = ACT != PJ_NONE ? y * pj_act_grad<T>(ACT, zv, sl[e]) : y;
+                sb[e] += dz;
+                if (ACT == PJ_PRELU) ss[e] += zv > 0.0f ? 0.0f : y * zv;
+                if (ACT != PJ_NONE) d[e] = (T)dz;
+            }
+            if (a.dz) *reinterpret_cast<Frag*>((T*)a.dz + (int64_t)at * a.Np + n) = d;
+        }
+    }
+}
+template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs a) {
+    constexpr int V = Elem<T>::EPC;
     __shared__ float sums[256][V + 1];
     const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
     int g, begin, end;
     if (!row_tile(a.rows, rt, a.tile_rows, g, begin, end) || g >= a.rows.G) return;     // the same for the whole workgroup
     const int lpr = 1 << a.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> a.lpr_log2, nsub = 256 >> a.lpr_log2;
-    const int n = (ct * lpr + lane) * V, left = a.N - n;
-    float sb[V], ss[V], sl[V];
+    const int n = (ct * lpr + lane) * V;
+    float sb[V], ss[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) sb[e] = ss[e] = sl[e] = 0.0f;
+    for (int e = 0; e < V; ++e) sb[e] = ss[e] = 0.0f;
     if (n < a.Np) {
-        if (a.slope) {
-#pragma unroll
-            for (int q = 0; q < V; q += 4) {
-                float s4[4];
-                load_param4<T>(a.slope, a.slope_f32, (int64_t)g * a.N + n + q, left - q, s4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sl[q + e] = s4[e];
-            }
-        }
-        for (int at0 = begin + sub; at0 < end; at0 += nsub * U) {
-            Frag dy[U], z[U];
-            int64_t row[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int at = at0 + u * nsub;
-                row[u] = at >= end ? -1 : a.rows.order ? a.rows.order[at] : at;
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int have = row[u] >= 0 ? left : 0;
-                dy[u] = load_chunk<T>((const T*)a.dy + (have > 0 ? row[u] * a.lddy + n : 0), have);
-                if (a.act != PJ_NONE) z[u] = load_chunk<T>((const T*)a.z + (have > 0 ? row[u] * a.N + n : 0), have);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (row[u] < 0) continue;
-                Frag d = dy[u];
-                if (a.act != PJ_NONE) {
-                    float dv[V];
-                    pj_act_grad_all<T, V>(a.act, z[u], sl, dv);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float y = (float)dy[u][e], zv = (float)z[u][e], dz = y * dv[e];
-                        sb[e] += dz;
-                        if (a.part_s) ss[e] += zv > 0.0f ? 0.0f : y * zv;
-                        d[e] = (T)dz;
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) sb[e] += (float)dy[u][e];
-                }
-                if (a.dz) *reinterpret_cast<Frag*>((T*)a.dz + (int64_t)(at0 + u * nsub) * a.Np + n) = d;
-            }
+        const bool full = a.N == a.Np;
+        switch (a.act) {
+#define PJ_CASE(A)                                                               \
+    case A:                                                                      \
+        if (full) dz_rows<T, A, true>(a, g, begin, end, n, sub, nsub, sb, ss);   \
+        else dz_rows<T, A, false>(a, g, begin, end, n, sub, nsub, sb, ss);       \
+        break;
+            PJ_CASE(PJ_NONE) PJ_CASE(PJ_RELU) PJ_CASE(PJ_PRELU) PJ_CASE(PJ_SILU) PJ_CASE(PJ_GELU_TANH)
+#undef PJ_CASE
         }
     }
 #pragma unroll
@@ -734,8 +731,10 @@ template <typename K> static int raise_lds(K kernel, int bytes, std::atomic<uint
         FRA_HIP(hipGetLastError());                                                      \
     } while (0)
 
+typedef Shape<256, 256, 2, 4, 2, 2> Huge;       // 16-bit types only
 typedef Shape<128, 128, 4, 2, 2, 2> Big;
 typedef Shape<64, 64, 2, 2, 2, 3> Small;
+typedef Shape<32, 32, 2, 1, 2, 4> Tiny;
 
 static int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
@@ -777,8 +776,16 @@ static int check_grid(int64_t blocks, const char* what) {
     FRA_REQUIRE(blocks < 2147483647LL, FRA_ERR_ARG, "%s: %lld workgroups", what, (long long)blocks);
     return FRA_OK;
 }
-// 128 x 128 tiles once they fill the 256 compute units, else 64 x 64
-static bool big_tiles(int64_t rows, int64_t cols) { return (int64_t)cdiv(rows, 128) * cdiv(cols, 128) >= 256; }
+// The side of a product's tiles.  256 x 256 moves half the bytes per product of 128 x 128 through the caches (8192 x 8192 x 8192:
+// 826 against 977 us) but holds one workgroup per compute unit, so it takes rounds that are nearly full (4096 x 2048 x 1024, half a
+// round: 37 against 24 us); 128 from one tile per unit on, 64 from three quarters of that on, below it 32 (1000 x 301 x 500 in fp32
+// is 80 tiles of 64 on 256 units).
+static int tile_side(int64_t rows, int64_t cols, bool f32) {
+    auto tiles = [&](int side) { return (int64_t)cdiv(rows, side) * cdiv(cols, side); };
+    const int64_t huge = tiles(256);
+    if (!f32 && huge >= 512 && huge * 10 >= (huge + 255) / 256 * 256 * 9) return 256;
+    return tiles(128) >= 256 ? 128 : tiles(64) >= 192 ? 64 : 32;
+}
 
 template <typename T, typename S> static int launch_forward(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
     a.n_col_tiles = cdiv(d->N, S::BJ);
@@ -801,22 +808,23 @@ template <typename T, int MT> static int launch_few_rows(const fra_linear_desc* 
 template <typename T> static int forward_t(const fra_linear_desc* d, void* z, void* y, hipStream_t s) {
     FwdArgs a;
     // up to 64 rows: the kernel for few rows; then by the number of tiles
-    const int bi = d->groups ? d->groups->tile_rows : d->M <= 16 ? 16 : d->M <= 32 ? 32 : d->M <= 64 ? 64 : big_tiles(d->M, d->N) ? 128 : 64;
+    const bool few = d->groups ? d->groups->tile_rows == 16 : d->M <= 64;
+    const int bi = d->groups ? d->groups->tile_rows : few ? (d->M <= 16 ? 16 : d->M <= 32 ? 32 : 64) : tile_side(d->M, d->N, sizeof(T) == 4);
     a.rows = row_args(d, bi);
     a.x = d->x; a.w = d->w; a.bias = d->bias; a.slope = d->slope; a.resid = d->resid; a.z = z; a.y = y;
     a.ldx = d->ldx; a.ldw = d->ldw; a.wg = d->w_group_stride; a.ldr = d->ldr;
     a.K = d->K; a.N = d->N; a.act = d->act; a.bias_f32 = d->bias_dtype == FRA_F32; a.slope_f32 = d->slope_dtype == FRA_F32;
-    if (bi == 16) return launch_few_rows<T, 1>(d, a, s);
-    if (bi == 32) return launch_few_rows<T, 2>(d, a, s);
-    if (bi == 64 && !d->groups && d->M <= 64) return launch_few_rows<T, 4>(d, a, s);
-    if (bi == 64) return launch_forward<T, Small>(d, a, s);
-    return launch_forward<T, Big>(d, a, s);
+    if (few) return bi == 16 ? launch_few_rows<T, 1>(d, a, s) : bi == 32 ? launch_few_rows<T, 2>(d, a, s) : launch_few_rows<T, 4>(d, a, s);
+    if constexpr (sizeof(T) == 2) {
+        if (bi == 256) return launch_forward<T, Huge>(d, a, s);
+    }
+    return bi == 128 ? launch_forward<T, Big>(d, a, s) : bi == 64 ? launch_forward<T, Small>(d, a, s) : launch_forward<T, Tiny>(d, a, s);
 }
 
 // ---- backward: what goes where in the workspace
 struct BackwardPlan {
     bool need_dz, need_sums, pack_x, pack_w;
-    int dz_rows, n_tiles, splits, Np, Kp;
+    int dz_rows, n_tiles, splits, dw_side, Np, Kp;
     size_t off_dz, off_x, off_w, off_b, off_s, off_part, bytes;
 };
 template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc* d, bool dx, bool dw, bool db, bool ds) {
@@ -835,10 +843,13 @@ template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc*
     p.pack_w = dx && !dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
     p.dz_rows = g ? g->tile_rows : 64;
     p.n_tiles = g ? g->n_tiles : cdiv(d->M, p.dz_rows);
-    // workgroups of dW: enough to fill the chip twice, each with at least 256 rows of its group's average share
-    const int64_t tiles = (int64_t)cdiv(d->N, Big::BI) * cdiv(d->K, Big::BJ) * G;
+    // dW: enough workgroups to fill the chip twice, each with at least 128 rows of its group's average share; tiles of 64 where
+    // tiles of 128 cannot be that many
+    const int64_t share = d->M / G / 128 > 1 ? d->M / G / 128 : 1;
+    p.dw_side = (int64_t)cdiv(d->N, 128) * cdiv(d->K, 128) * G * share >= 256 ? 128 : 64;
+    const int64_t tiles = (int64_t)cdiv(d->N, p.dw_side) * cdiv(d->K, p.dw_side) * G;
     int64_t sp = (512 + tiles - 1) / tiles;
-    if (sp > d->M / G / 256) sp = d->M / G / 256;
+    if (sp > share) sp = share;
     p.splits = dw && sp > 1 ? (int)sp : 1;
     size_t at = 0;
     p.off_dz = at; if (p.need_dz) at += up((size_t)d->M * p.Np * es);
@@ -887,7 +898,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         a.tile_rows = p.dz_rows;
         const int pieces = p.Np / Elem<T>::EPC;
         a.lpr_log2 = 0;
-        while (a.lpr_log2 < 6 && (1 << a.lpr_log2) < pieces) ++a.lpr_log2;
+        while (a.lpr_log2 < 4 && (1 << a.lpr_log2) < pieces) ++a.lpr_log2;
         a.n_col_tiles = cdiv(pieces, 1 << a.lpr_log2);
         const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
         if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
@@ -919,10 +930,15 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
             if (int rc = launch_pack<T>(k, s)) return rc;
             a.w = k.dst; a.ldw = p.Kp; a.wg = (int64_t)d->N * p.Kp;
         }
-        const bool big = g ? g->tile_rows == 128 : big_tiles(d->M, d->K);
-        a.rows = row_args(d, big ? 128 : 64);
+        const int bi = g ? g->tile_rows : tile_side(d->M, d->K, sizeof(T) == 4);
+        a.rows = row_args(d, bi);
         a.dz = dz; a.dx = dx; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
-        if (int rc = big ? launch_dx<T, Big>(a, s) : launch_dx<T, Small>(a, s)) return rc;
+        int rc = FRA_OK;
+        if constexpr (sizeof(T) == 2) {
+            if (bi == 256) rc = launch_dx<T, Huge>(a, s);
+        }
+        if (bi != 256) rc = bi == 128 ? launch_dx<T, Big>(a, s) : bi == 64 ? launch_dx<T, Small>(a, s) : launch_dx<T, Tiny>(a, s);
+        if (rc != FRA_OK) return rc;
     }
     if (dw) {
         DwArgs a;
@@ -936,10 +952,12 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         }
         a.rows = row_args(d, 128);
         a.dz = dz; a.dw = p.splits > 1 ? (void*)(ws + p.off_part) : dw; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
-        a.n_ti = cdiv(d->N, Big::BI); a.n_tj = cdiv(d->K, Big::BJ); a.splits = p.splits;
+        a.n_ti = cdiv(d->N, p.dw_side); a.n_tj = cdiv(d->K, p.dw_side); a.splits = p.splits;
         const int64_t blocks = ((int64_t)a.n_ti * a.n_tj + 7) / 8 * 8;
         if (int rc = check_grid(blocks * a.splits * G, "fra_linear_backward")) return rc;
-        PJ_LAUNCH((pj_dw_kernel<T, Big>), dim3((unsigned)blocks, a.splits * G), Big::NT, Big::LDS, s, a);
+        const dim3 grid((unsigned)blocks, a.splits * G);
+        if (p.dw_side == 128) PJ_LAUNCH((pj_dw_kernel<T, Big>), grid, Big::NT, Big::LDS, s, a);
+        else PJ_LAUNCH((pj_dw_kernel<T, Small>), grid, Small::NT, Small::LDS, s, a);
         if (p.splits > 1) {
             const int64_t n = (int64_t)G * d->N * d->K, jb = (n + 1023) / 1024;
             if (int rc = check_grid(jb, "fra_linear_backward")) return rc;

@@ -8,8 +8,9 @@
 //   row-major  [DIM rows][4 KS chunks of k]; chunk c of row r at slot c ^ (r & 7) (KS = 2) or c ^ (r >> 1 & 3) (KS = 1): the eight
 //              rows of a read's phase are on different banks;
 //   k-major    [step's rows of k][DIM], 16 bit: chunk pair p of row k at p ^ ((k & 3) | (k >> 1 & 4)) (128 columns and more; with
-//              64, two rows of k fill a row of banks: p ^ ((k >> 1 & 1) | (k >> 2 & 2))), so the eight 32-byte pieces that half a
-//              wave's transposing read (ds_read_b64_tr_b16) takes are on different banks; float: chunk c at c ^ 4 (k >> 2 & 3).
+//              64, two rows of k fill a row of banks: p ^ ((k >> 1 & 1) | (k >> 2 & 2)); with 32, four: p ^ (k >> 3 & 1)), so the
+//              eight 32-byte pieces that half a wave's transposing read (ds_read_b64_tr_b16) takes are on different banks; float:
+//              chunk c at c ^ 4 (k >> 2 & 3) (with 32 columns 4 (k >> 2 & 1), two lanes to a bank).
 #pragma once
 
 #include "common.h"
@@ -96,9 +97,10 @@ template <typename T> __device__ __forceinline__ void load_param4(const void* p,
 
 template <int KS> __device__ __forceinline__ int swz_row_major(int row, int c) { return KS == 2 ? c ^ (row & 7) : c ^ ((row >> 1) & 3); }
 template <typename T, int CPR> __device__ __forceinline__ int swz_k_major(int k, int c) {
-    if constexpr (sizeof(T) == 4) return c ^ (((k >> 2) & 3) << 2);
+    if constexpr (sizeof(T) == 4) return c ^ ((((k >> 2) & 3) << 2) & (CPR - 1));
     else if constexpr (CPR >= 16) return c ^ (((k & 3) | ((k >> 1) & 4)) << 1);
-    else return c ^ ((((k >> 1) & 1) | ((k >> 2) & 2)) << 1);       // two rows of k share a row of banks
+    else if constexpr (CPR == 8) return c ^ ((((k >> 1) & 1) | ((k >> 2) & 2)) << 1);       // two rows of k share a row of banks
+    else return c ^ (((k >> 3) & 1) << 1);                                                  // four do
 }
 
 // 16 bytes per lane from global memory into LDS at `lds` + 16 lane, without passing through registers.  Written out (the

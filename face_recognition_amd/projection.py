@@ -28,6 +28,11 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "prelu": 2, "silu": 3, "gelu_tanh"
 MAX_GROUPS = 4096
 
 
+def _stream(device: torch.device) -> int:
+    """The current stream's handle, without building a ``torch.cuda.Stream`` for it (2 us of a call's 13)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 class _on_device:
     """``torch.cuda.device`` that costs nothing when the device is the current one already."""
     __slots__ = ("index", "prev")
@@ -85,7 +90,7 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
         ws = torch.empty(need.value, dtype=torch.uint8, device=ids.device) if need.value else None
         _lib.check(lib.fra_group_rows(ids.data_ptr(), int(ids.dtype == torch.int64), C.byref(g._desc),
                                       ws.data_ptr() if ws is not None else None, need.value,
-                                      _lib.current_stream_ptr(ids.device)), "fra_group_rows")
+                                      _stream(ids.device)), "fra_group_rows")
     return g
 
 
@@ -128,13 +133,13 @@ def _forward(x, weight, bias, slope, residual, act, groups, want_preact):
         bias = bias.contiguous()
     if slope is not None:
         slope = slope.contiguous()
-    out = torch.empty((x.shape[0], weight.shape[-2]), dtype=x.dtype, device=x.device)
+    out = x.new_empty((x.shape[0], weight.shape[-2]))
     z = torch.empty_like(out) if want_preact else None
     if out.shape[0]:
         d = _desc(x, ldx, weight, ldw, wg, bias, slope, residual, ldr, act, groups)
         with _on_device(x.device):
             _lib.check(_lib.load().fra_linear(C.byref(d), z.data_ptr() if z is not None else None, out.data_ptr(),
-                                              _lib.current_stream_ptr(x.device)), "fra_linear")
+                                              _stream(x.device)), "fra_linear")
     return out, z
 
 
@@ -155,11 +160,11 @@ class _Linear(torch.autograd.Function):
         x, weight, slope, z = ctx.saved_tensors
         need = ctx.needs_input_grad
         dev = x.device
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need[1] else None
+        dx = x.new_empty(x.shape) if need[0] else None
+        dw = x.new_empty(weight.shape) if need[1] else None
         par = weight.shape[:-1]
-        db = torch.empty(par, dtype=ctx.bias_dtype, device=dev) if need[2] else None
-        ds = torch.empty(par, dtype=slope.dtype, device=dev) if need[3] else None
+        db = x.new_empty(par, dtype=ctx.bias_dtype) if need[2] else None
+        ds = x.new_empty(par, dtype=slope.dtype) if need[3] else None
         if any(need[:4]):
             lib = _lib.load()
             g, lddy = _rows(dy)
@@ -177,37 +182,42 @@ class _Linear(torch.autograd.Function):
                 ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
                 ptr = [t.data_ptr() if t is not None else None for t in (dx, dw, db, ds)]
                 _lib.check(lib.fra_linear_backward(C.byref(d), z.data_ptr() if z is not None else None, g.data_ptr(), lddy,
-                                                   *ptr, ws.data_ptr(), nbytes.value, _lib.current_stream_ptr(dev)),
+                                                   *ptr, ws.data_ptr(), nbytes.value, _stream(dev)),
                            "fra_linear_backward")
         return dx, dw, db, ds, (dy if need[4] else None), None, None
 
 
 def _check(what, x, weight, bias, activation, slope, residual, lead):
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation, -1) if activation is None or isinstance(activation, str) else -1
+    if act < 0:
         raise RuntimeError(f"{what}: activation {activation!r} is none of {sorted(k for k in ACTIVATIONS if k)}")
-    act = ACTIVATIONS[activation]
-    if x.dtype not in _DTYPES:
-        raise RuntimeError(f"{what}: {x.dtype} is not supported (float32, float16, bfloat16)")
+    dt = x.dtype
+    if dt not in _DTYPES:
+        raise RuntimeError(f"{what}: {dt} is not supported (float32, float16, bfloat16)")
     if not x.is_cuda:
         raise RuntimeError(f"{what}: tensors live on the HIP device ('cuda'); there is no CPU path")
-    if weight.dim() != 2 + len(lead) or tuple(weight.shape[:len(lead)]) != lead:
-        raise RuntimeError(f"{what}: weight must be [{', '.join([str(v) for v in lead] + ['N', 'K'])}], got {tuple(weight.shape)}")
-    n, k = weight.shape[-2:]
-    if n == 0 or k == 0 or x.dim() < 1 or x.shape[-1] != k:
-        raise RuntimeError(f"{what}: x {tuple(x.shape)} does not go with weight {tuple(weight.shape)}")
+    ws = weight.shape
+    if len(ws) != 2 + len(lead) or ws[:-2] != lead:
+        raise RuntimeError(f"{what}: weight must be [{', '.join([str(v) for v in lead] + ['N', 'K'])}], got {tuple(ws)}")
+    n, k = ws[-2:]
+    xs = x.shape
+    if n == 0 or k == 0 or len(xs) < 1 or xs[-1] != k:
+        raise RuntimeError(f"{what}: x {tuple(xs)} does not go with weight {tuple(ws)}")
     if (act == 2) != (slope is not None):
         raise RuntimeError(f"{what}: slope goes with activation 'prelu', and only with it")
+    par = lead + (n,)
     for name, t in (("bias", bias), ("slope", slope)):
-        if t is not None and (tuple(t.shape) != lead + (n,) or t.dtype not in (x.dtype, torch.float32)):
-            raise RuntimeError(f"{what}: {name} must be {list(lead + (n,))} in {x.dtype} or float32, got {list(t.shape)} {t.dtype}")
-    if residual is not None and tuple(residual.shape) != tuple(x.shape[:-1]) + (n,):
-        raise RuntimeError(f"{what}: residual must be {list(x.shape[:-1]) + [n]}, got {list(residual.shape)}")
+        if t is not None and (t.shape != par or (t.dtype != dt and t.dtype != torch.float32)):
+            raise RuntimeError(f"{what}: {name} must be {list(par)} in {dt} or float32, got {list(t.shape)} {t.dtype}")
+    if residual is not None and residual.shape != xs[:-1] + (n,):
+        raise RuntimeError(f"{what}: residual must be {list(xs[:-1]) + [n]}, got {list(residual.shape)}")
     for name, t in (("weight", weight), ("residual", residual)):
-        if t is not None and t.dtype != x.dtype:
-            raise RuntimeError(f"{what}: {name} is {t.dtype}, x is {x.dtype}")
+        if t is not None and t.dtype != dt:
+            raise RuntimeError(f"{what}: {name} is {t.dtype}, x is {dt}")
+    dev = x.device
     for name, t in (("weight", weight), ("bias", bias), ("slope", slope), ("residual", residual)):
-        if t is not None and t.device != x.device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, x on {x.device}")
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, x on {dev}")
     return act
 
 
@@ -285,5 +295,5 @@ def orthogonalize(matrix: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4
         _lib.check(lib.fra_orthogonalize(_DTYPES[g.dtype], g.data_ptr(), s0 if rows > 1 else cols,
                                          g.stride(0) if g.dim() == 3 else 0, batch, rows, cols, int(steps),
                                          *[float(v) for v in coefficients], out.data_ptr(), ws.data_ptr(), need.value,
-                                         _lib.current_stream_ptr(matrix.device)), "fra_orthogonalize")
+                                         _stream(matrix.device)), "fra_orthogonalize")
     return out

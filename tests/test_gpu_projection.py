@@ -309,6 +309,26 @@ def test_gradients_against_differences(device, act):
     assert abs(got - want) <= sum(err) / (2 * h) + curve + grad_err
 
 
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_a_row_does_not_depend_on_the_rows_beside_it(device, dt):
+    """Beyond the kernel for few rows a value is the same sum in the same order whatever tiles the batch's size asks for: the rows
+    of a large ragged batch (512 tiles of 256 rows) equal those of its parts, forward and back."""
+    m, k, n = 130900, 136, 250
+    t = make(m, k, n, dt, device, 91, act="silu")
+
+    def y_dx(rows):
+        x = t["x"][rows].clone().requires_grad_(True)
+        y = projection.linear(x, t["w"], t["b"], "silu", residual=t["r"][rows])
+        return y.detach(), torch.autograd.grad(y, x, t["dy"][rows])[0]
+
+    y, dx = y_dx(slice(None))
+    for rows in (slice(0, 100), slice(50000, 57000), slice(m - 65, m)):
+        part_y, part_dx = y_dx(rows)
+        assert torch.equal(part_y, y[rows]) and torch.equal(part_dx, dx[rows])
+    rows = slice(m - 300, m)
+    check({"y": y[rows], "dx": dx[rows]}, reference({name: v[rows] if name in ("x", "r", "dy") else v for name, v in t.items()}, "silu"))
+
+
 def test_repeated_runs_are_the_same_bits(device):
     t = make(3000, 130, 200, torch.bfloat16, device, 41, lead=(7,), act="prelu")
     rg = projection.group_rows(torch.arange(3000, device=device) * 7919 % 8, 7)
