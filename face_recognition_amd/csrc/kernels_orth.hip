@@ -45,43 +45,62 @@ __device__ __forceinline__ void split16(float v, f16& hi, f16& lo) {
     lo = (f16)(v - (float)hi);
 }
 
-// G -> X hi / lo [m][np], normalised, transposed if need be, zeros in columns n .. np: 64 x 64 tiles through LDS
+// G -> X hi / lo [m][np], normalised, transposed if need be, zeros in columns n .. np: 64 x 64 tiles through LDS, four neighbours
+// at a time on both sides.  The tile's values are requested before the norm's partial sums are added.
 template <typename T> __global__ __launch_bounds__(256) void orth_split_kernel(const T* g, int64_t ldg, int64_t bs, OrthDims d, const double* part,
                                                                               int n_part, f16* xh, f16* xl) {
     __shared__ float tile[64][65];
     __shared__ double factor;                                       // fp64: OR_SCALE / norm leaves fp32's range for a tiny matrix
     const int b = blockIdx.z, i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
-    if (threadIdx.x < 64) {
-        double v = 0.0;
-        for (int p = threadIdx.x; p < n_part; p += 64) v += part[(int64_t)b * n_part + p];
+    const T* p = g + (int64_t)b * bs;
+    const int r0 = threadIdx.x >> 4, c = (threadIdx.x & 15) * 4;
+    // source rows: X's rows, or (transposed) X's columns
+    const int sr0 = d.transposed ? j0 : i0, sc = (d.transposed ? i0 : j0) + c, nr = d.transposed ? d.n : d.m, nc = d.transposed ? d.m : d.n;
+    float v[4][4];
 #pragma unroll
-        for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s, 64);
-        if (threadIdx.x == 0) factor = v == 0.0 ? 0.0 : (double)OR_SCALE / sqrt(v);        // a matrix of zeros stays one
+    for (int q = 0; q < 4; ++q) {
+        const int r = sr0 + r0 + 16 * q, left = r < nr ? nc - sc : 0;
+        load_four<T>(p + (left > 0 ? (int64_t)r * ldg + sc : 0), left, v[q]);
+    }
+    if (threadIdx.x < 64) {
+        double s = 0.0;
+        for (int k = threadIdx.x; k < n_part; k += 64) s += part[(int64_t)b * n_part + k];
+#pragma unroll
+        for (int k = 32; k; k >>= 1) s += __shfl_xor(s, k, 64);
+        if (threadIdx.x == 0) factor = s == 0.0 ? 0.0 : (double)OR_SCALE / sqrt(s);        // a matrix of zeros stays one
     }
     __syncthreads();
     const double f = factor;
-    const T* p = g + (int64_t)b * bs;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int r = wave; r < 64; r += 4) {
-        // source rows: X's rows, or (transposed) X's columns
-        const int sr = (d.transposed ? j0 : i0) + r, sc = (d.transposed ? i0 : j0) + lane;
-        const bool in = sr < (d.transposed ? d.n : d.m) && sc < (d.transposed ? d.m : d.n);
-        const float v = in ? (float)((double)(float)p[(int64_t)sr * ldg + sc] * f) : 0.0f;
-        if (d.transposed) tile[lane][r] = v;
-        else tile[r][lane] = v;
-    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = (float)((double)v[q][e] * f);
+            if (d.transposed) tile[c + e][r0 + 16 * q] = x;
+            else tile[r0 + 16 * q][c + e] = x;
+        }
     __syncthreads();
     const int64_t base = (int64_t)b * d.m * d.np;
-    for (int r = wave; r < 64; r += 4) {
-        if (i0 + r >= d.m || j0 + lane >= d.np) continue;
-        f16 hi, lo;
-        split16(tile[r][lane], hi, lo);
-        xh[base + (int64_t)(i0 + r) * d.np + j0 + lane] = hi;
-        xl[base + (int64_t)(i0 + r) * d.np + j0 + lane] = lo;
+    if (j0 + c >= d.np) return;                                     // np is a multiple of 8: four neighbours are all in or all out
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int i = r0 + 16 * q;
+        if (i0 + i >= d.m) continue;
+        vec4<f16>::type hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            f16 h, l;
+            split16(tile[i][c + e], h, l);
+            hi[e] = h;
+            lo[e] = l;
+        }
+        const int64_t at = base + (int64_t)(i0 + i) * d.np + j0 + c;
+        *reinterpret_cast<vec4<f16>::type*>(xh + at) = hi;
+        *reinterpret_cast<vec4<f16>::type*>(xl + at) = lo;
     }
 }
 
-// C = alpha A B^T + beta E (or A B where B is contraction-major), everything hi / lo f16, batch in blockIdx.y
+// C = alpha A B^T + beta E (or A B where B is k-major), everything hi / lo f16, batch in blockIdx.y
 struct OrthArgs {
     const f16 *ah, *al, *bh, *bl, *eh, *el;
     f16 *ch, *cl;               // nullptr: the last product, into out
@@ -91,73 +110,234 @@ struct OrthArgs {
     int64_t ldo;
     int I, J, Jp, K;            // C is [I][J], columns J .. Jp are written as zeros
     float alpha, beta;
-    int n_col_tiles, transposed;
+    int n_row_tiles, n_col_tiles, transposed;
 };
-template <typename T, bool BK, typename S> __global__ __launch_bounds__(S::NT) void orth_product_kernel(OrthArgs a) {
+
+// The product of pairs: a step brings the hi and lo tiles of both operands, four tiles for three products (three products one
+// after the other would bring six).  Everything else is as in Product.
+template <bool BK, typename S> struct PairProduct {
+    typedef OperandA<f16, false, S> OA;
+    typedef OperandB<f16, BK, S> OB;
+    static constexpr int NB = S::NB, BUF = 2 * S::STEP, NLD = 2 * (OA::NLD + OB::NLD), LDS = NB * BUF;
+    static_assert(NB >= 2 && NB <= 4 && S::KS == 2, "");
+    OA A;
+    OB B;
+    typename OA::Src sa;
+    typename OB::Src sb;
+    int64_t a_lo, b_lo;         // elements from an operand's hi part to its lo part
+    int steps;
+
+    __device__ __forceinline__ void issue(int step, LdsPtr dst, int tid) const {
+        A.issue(sa, step, dst, tid);
+        A.issue(sa, step, dst + OA::BYTES, tid, a_lo);
+        B.issue(sb, step, dst + 2 * OA::BYTES, tid);
+        B.issue(sb, step, dst + 2 * OA::BYTES + OB::BYTES, tid, b_lo);
+    }
+    template <int Y> __device__ __forceinline__ static void arrived(int behind) {
+        if (behind >= Y) dma_wait_barrier<Y * NLD>();
+        else if (Y > 2 && behind == 2) dma_wait_barrier<2 * NLD>();
+        else if (Y > 1 && behind == 1) dma_wait_barrier<NLD>();
+        else dma_wait_barrier<0>();
+    }
+    struct PairFrags {
+        typename Elem<f16>::Frag ah[S::MI], al[S::MI], bh[S::MJ], bl[S::MJ];
+        __device__ __forceinline__ void read(const char* step, int ks, int i0, int j0, int lane) {
+#pragma unroll
+            for (int mi = 0; mi < S::MI; ++mi) {
+                ah[mi] = OA::frag(step, i0 + 16 * mi, ks, lane);
+                al[mi] = OA::frag(step + OA::BYTES, i0 + 16 * mi, ks, lane);
+            }
+#pragma unroll
+            for (int mj = 0; mj < S::MJ; ++mj) {
+                bh[mj] = OB::frag(step + 2 * OA::BYTES, j0 + 16 * mj, ks, lane);
+                bl[mj] = OB::frag(step + 2 * OA::BYTES + OB::BYTES, j0 + 16 * mj, ks, lane);
+            }
+        }
+        __device__ __forceinline__ void mma(f32x4 (&acc)[S::MI][S::MJ]) const {
+            // the small parts first
+#pragma unroll
+            for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+                for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = pj_mma<f16>(bh[mj], al[mi], acc[mi][mj]);
+#pragma unroll
+            for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+                for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = pj_mma<f16>(bl[mj], ah[mi], acc[mi][mj]);
+#pragma unroll
+            for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+                for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = pj_mma<f16>(bh[mj], ah[mi], acc[mi][mj]);
+        }
+    };
+    __device__ __forceinline__ void run(int klen, char* lds, f32x4 (&acc)[S::MI][S::MJ]) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+            for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
+        steps = (klen + OA::KSTEP - 1) / OA::KSTEP;
+        A.init(sa, tid);
+        B.init(sb, tid);
+        const LdsPtr dst = (LdsPtr)lds + __builtin_amdgcn_readfirstlane(wave) * 1024;
+#pragma unroll
+        for (int t = 0; t < NB; ++t)
+            if (t < steps) issue(t, dst + t * BUF, tid);
+        PairFrags f0, f1;
+        arrived<NB - 1>(steps - 1);
+        f0.read(lds, 0, i0, j0, lane);
+        int cur = 0;
+        for (int t = 0; t < steps; ++t) {
+            f1.read(lds + cur, 1, i0, j0, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            f0.mma(acc);
+            __builtin_amdgcn_sched_barrier(0);
+            const int nxt = cur + BUF == NB * BUF ? 0 : cur + BUF;
+            if (t + 1 < steps) {
+                arrived<NB - 2>(steps - 2 - t);
+                if (t + NB < steps) issue(t + NB, dst + cur, tid);
+                f0.read(lds + nxt, 0, i0, j0, lane);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            f1.mma(acc);
+            __builtin_amdgcn_sched_barrier(0);
+            cur = nxt;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+};
+
+// A piece is eight neighbours of a row (Jp is a multiple of 8: all in or all out).  T: the pairs' (f16) or the result's type
+template <typename T> struct OrthEmit {
+    static constexpr int V = 16 / sizeof(T);
+    struct Pre {
+        typename Elem<f16>::Frag h, l;
+    };
+    const OrthArgs& a;
+    int64_t b;
+    int i0, j0;
+    __device__ __forceinline__ int row(int i) const { return i0 + i < a.I ? i0 + i : -1; }
+    __device__ __forceinline__ Pre pre(int i, int j) const {
+        Pre p = {};
+        if (a.eh && i >= 0 && j0 + j < a.Jp) {
+            const int64_t at = b * a.se + (int64_t)i * a.lde + ((j0 + j) & ~7);
+            p.h = *reinterpret_cast<const typename Elem<f16>::Frag*>(a.eh + at);
+            p.l = *reinterpret_cast<const typename Elem<f16>::Frag*>(a.el + at);
+        }
+        return p;
+    }
+    __device__ __forceinline__ void emit(int i, int jt, const Pre& p, float (&v)[V]) const {
+        const int j = j0 + jt, from = V == 4 && (j & 4) ? 4 : 0;
+        if (i < 0 || j >= a.Jp) return;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float pe = V == 8 ? (float)p.h[e] + (float)p.l[e] : from ? (float)p.h[(e + 4) & 7] + (float)p.l[(e + 4) & 7] : (float)p.h[e] + (float)p.l[e];
+            v[e] = j + e < a.J ? a.alpha * v[e] + a.beta * pe : 0.0f;
+        }
+        if (a.ch) {
+            if constexpr (V == 8) {
+                typename Elem<f16>::Frag hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f16 h, l;
+                    split16(v[e], h, l);
+                    hi[e] = h;
+                    lo[e] = l;
+                }
+                *reinterpret_cast<typename Elem<f16>::Frag*>(a.ch + b * a.sc + (int64_t)i * a.ldc + j) = hi;
+                *reinterpret_cast<typename Elem<f16>::Frag*>(a.cl + b * a.sc + (int64_t)i * a.ldc + j) = lo;
+            }
+        } else {
+            typename Elem<T>::Frag o;
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = (T)(v[e] * (1.0f / OR_SCALE));
+            store_chunk<T>((T*)a.out + b * a.so + (int64_t)i * a.ldo + j, a.J - j, o);
+        }
+    }
+};
+// the last product of a transposed matrix: out[j][i], a wave's part turned through LDS so that a lane writes V neighbouring i
+template <typename T, typename S> __device__ __forceinline__ void orth_emit_transposed(const OrthArgs& a, int64_t b, int i0, int j0, const f32x4 (&acc)[S::MI][S::MJ], char* lds) {
+    constexpr int V = 16 / sizeof(T), ROWS = S::MI * 16, LPR = ROWS / V, RPP = 64 / LPR, PITCH = ROWS + 4;
+    static_assert(S::WI * S::WJ * S::MJ * 16 * PITCH * 4 <= 2 * S::LDS, "");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wi = i0 + (wave % S::WI) * (S::BI / S::WI), wj = j0 + (wave / S::WI) * (S::BJ / S::WJ);
+    float* strip = reinterpret_cast<float*>(lds) + wave * (S::MJ * 16 * PITCH);
+#pragma unroll
+    for (int mi = 0; mi < S::MI; ++mi) {
+        const int i = wi + 16 * mi + (lane & 15);
+#pragma unroll
+        for (int mj = 0; mj < S::MJ; ++mj) {
+            const int jl = 16 * mj + 4 * (lane >> 4), j = wj + jl;
+            float h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
+            if (i < a.I && j < a.Jp) {
+                load_four<f16>(a.eh + b * a.se + (int64_t)i * a.lde + j, 4, h);
+                load_four<f16>(a.el + b * a.se + (int64_t)i * a.lde + j, 4, l);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                strip[(jl + e) * PITCH + 16 * mi + (lane & 15)] = (a.alpha * acc[mi][mj][e] + a.beta * (h[e] + l[e])) * (1.0f / OR_SCALE);
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int jl = 0; jl < S::MJ * 16; jl += RPP) {
+        const int jr = jl + lane / LPR, j = wj + jr, il = (lane % LPR) * V, i = wi + il;
+        typename Elem<T>::Frag o;
+#pragma unroll
+        for (int q = 0; q < V; q += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(strip + jr * PITCH + il + q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[q + e] = (T)x[e];
+        }
+        if (j < a.J && i < a.I) store_chunk<T>((T*)a.out + b * a.so + (int64_t)j * a.ldo + i, a.I - i, o);
+    }
+}
+// LAST: the last product of the last step, into out (T)
+template <typename T, bool BK, bool LAST, typename S> __global__ __launch_bounds__(S::NT) void orth_product_kernel(OrthArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
+    int rt, ct;
+    if (!tile_of_block(blockIdx.x, a.n_row_tiles, a.n_col_tiles, rt, ct)) return;
     const int i0 = rt * S::BI, j0 = ct * S::BJ;
     const int64_t b = blockIdx.y;
     f32x4 acc[S::MI][S::MJ];
-    Product<f16, false, BK, S, true> p;
-    p.A.order = nullptr; p.A.ld = a.lda; p.A.row0 = i0; p.A.rows = a.I - i0; p.A.klen = a.K; p.A.cols = 0;
-    p.B.order = nullptr; p.B.ld = a.ldb; p.B.klen = a.K;
-    p.B.row0 = BK ? 0 : j0; p.B.rows = BK ? 0 : a.J - j0; p.B.cols = BK ? a.J - j0 : 0;
-    const int64_t boff = b * a.sb + (BK ? j0 : 0);
-    // the small parts first, so that they are added before the large ones
-    p.A.base = a.al + b * a.sa; p.B.base = a.bh + boff;
-    p.start(a.K, lds);
-    p.run(lds, acc);
-    p.A.base = a.ah + b * a.sa; p.B.base = a.bl + boff;
-    p.start(a.K, lds);
-    p.template run<true>(lds, acc);
-    p.A.base = a.ah + b * a.sa; p.B.base = a.bh + boff;
-    p.start(a.K, lds);
-    p.template run<true>(lds, acc);
-
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int li = (wave % S::WI) * (S::BI / S::WI) + (lane & 15), lj = (wave / S::WI) * (S::BJ / S::WJ) + 4 * (lane >> 4);
-#pragma unroll
-    for (int mi = 0; mi < S::MI; ++mi) {
-        const int i = i0 + li + 16 * mi;
-        if (i >= a.I) continue;
-#pragma unroll
-        for (int mj = 0; mj < S::MJ; ++mj) {
-            const int j = j0 + lj + 16 * mj;
-            if (j >= a.Jp) continue;
-            float v[4], eh[4] = {0, 0, 0, 0}, el[4] = {0, 0, 0, 0};
-            if (a.eh) {
-                load_four<f16>(a.eh + b * a.se + (int64_t)i * a.lde + j, 4, eh);
-                load_four<f16>(a.el + b * a.se + (int64_t)i * a.lde + j, 4, el);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = j + e < a.J ? a.alpha * acc[mi][mj][e] + a.beta * (eh[e] + el[e]) : 0.0f;
-            if (a.ch) {
-                float hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    hi[e] = (float)(f16)v[e];
-                    lo[e] = v[e] - hi[e];
-                }
-                store_four<f16>(a.ch + b * a.sc + (int64_t)i * a.ldc + j, 4, hi);
-                store_four<f16>(a.cl + b * a.sc + (int64_t)i * a.ldc + j, 4, lo);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] *= 1.0f / OR_SCALE;
-                T* o = (T*)a.out + b * a.so;
-                if (!a.transposed) {
-                    if (a.J - j > 0) store_four<T>(o + (int64_t)i * a.ldo + j, a.J - j, v);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (j + e < a.J) o[(int64_t)(j + e) * a.ldo + i] = (T)v[e];
-                }
-            }
-        }
+    PairProduct<BK, S> p;
+    p.A.order = nullptr; p.A.ld = a.lda; p.A.row0 = i0; p.A.rows = a.I - i0; p.A.klen = a.K; p.A.cols = 0; p.A.base = a.ah + b * a.sa;
+    p.B.order = nullptr; p.B.ld = a.ldb; p.B.klen = a.K; p.B.base = a.bh + b * a.sb + (BK ? j0 : 0);
+    p.B.row0 = BK ? 0 : j0; p.B.rows = BK ? 0 : a.J - j0; p.B.cols = BK ? a.Jp - j0 : 0;
+    p.a_lo = a.al - a.ah; p.b_lo = a.bl - a.bh;
+    p.run(a.K, lds, acc);
+    if constexpr (!LAST) {
+        tile_emit<f16, S>(acc, lds, OrthEmit<f16>{a, b, i0, j0});
+    } else if (!a.transposed) {
+        tile_emit<T, S>(acc, lds, OrthEmit<T>{a, b, i0, j0});
+    } else {
+        orth_emit_transposed<T, S>(a, b, i0, j0, acc, lds);
     }
 }
 
-typedef Shape<64, 64, 2, 2, 2, 3> OrthTile;
+typedef Shape<128, 128, 4, 2, 2, 2> OrthBig;
+typedef Shape<64, 64, 2, 2, 2, 2> OrthSmall;
+typedef Shape<32, 32, 2, 1, 2, 3> OrthTiny;
+
+template <typename T, bool BK, bool LAST, typename S> static int launch_orth(OrthArgs& a, int batch, hipStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    const int lds = PairProduct<BK, S>::LDS;
+    if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(orth_product_kernel<T, BK, LAST, S>), lds, done)) return rc;
+    a.n_row_tiles = (a.I + S::BI - 1) / S::BI;
+    a.n_col_tiles = (a.Jp + S::BJ - 1) / S::BJ;
+    const int blocks = (a.n_row_tiles * a.n_col_tiles + 7) / 8 * 8;
+    hipLaunchKernelGGL((orth_product_kernel<T, BK, LAST, S>), dim3(blocks, batch), dim3(S::NT), lds, s, a);
+    FRA_HIP(hipGetLastError());
+    return FRA_OK;
+}
+// tiles of 128 from three quarters of the chip's units on, of 64 likewise, else 32
+template <typename T, bool BK, bool LAST> static int product(OrthArgs& a, int batch, hipStream_t s) {
+    auto tiles = [&](int64_t side) { return (a.I + side - 1) / side * ((a.Jp + side - 1) / side) * batch; };
+    if (tiles(128) >= 192) return launch_orth<T, BK, LAST, OrthBig>(a, batch, s);
+    if (tiles(64) >= 192) return launch_orth<T, BK, LAST, OrthSmall>(a, batch, s);
+    return launch_orth<T, BK, LAST, OrthTiny>(a, batch, s);
+}
 
 struct OrthPlan {
     OrthDims d;
@@ -201,9 +381,6 @@ static int orth_t(const OrthPlan& p, const T* g, int64_t ldg, int64_t bs, int st
     hipLaunchKernelGGL((orth_split_kernel<T>), dim3((d.np + 63) / 64, (d.m + 63) / 64, d.batch), dim3(256), 0, s, g, ldg, bs, d, part, p.n_part,
                        xh[0], xh[0] + xlo);
     FRA_HIP(hipGetLastError());
-    constexpr int LDS = OrthTile::LDS;
-    static_assert(LDS <= 65536, "no raised limit needed");
-    const int ti = (d.m + 63) / 64, tp = (d.mp + 63) / 64, tx = (d.np + 63) / 64;
     for (int t = 0; t < steps; ++t) {
         f16 *x = xh[t & 1], *y = xh[(t + 1) & 1];
         OrthArgs a;
@@ -211,25 +388,24 @@ static int orth_t(const OrthPlan& p, const T* g, int64_t ldg, int64_t bs, int st
         // P = X X^T
         a.ah = a.bh = x; a.al = a.bl = x + xlo; a.eh = a.el = nullptr; a.ch = ph; a.cl = ph + qlo;
         a.sa = a.sb = xe; a.se = 0; a.sc = qe; a.lda = a.ldb = d.np; a.lde = 0; a.ldc = d.mp;
-        a.I = d.m; a.J = d.m; a.Jp = d.mp; a.K = d.n; a.alpha = 1.0f / OR_SCALE; a.beta = 0.0f; a.n_col_tiles = tp;
-        hipLaunchKernelGGL((orth_product_kernel<T, false, OrthTile>), dim3(ti * tp, d.batch), dim3(OrthTile::NT), LDS, s, a);
-        FRA_HIP(hipGetLastError());
+        a.I = d.m; a.J = d.m; a.Jp = d.mp; a.K = d.np; a.alpha = 1.0f / OR_SCALE; a.beta = 0.0f;
+        if (int rc = product<f16, false, false>(a, d.batch, s)) return rc;
         // Q = b P + c P P (P is symmetric)
         a.ah = a.bh = a.eh = ph; a.al = a.bl = a.el = ph + qlo; a.ch = qh; a.cl = qh + qlo;
         a.sa = a.sb = a.se = a.sc = qe; a.lda = a.ldb = a.lde = a.ldc = d.mp;
-        a.K = d.m; a.alpha = cc / OR_SCALE; a.beta = cb;
-        hipLaunchKernelGGL((orth_product_kernel<T, false, OrthTile>), dim3(ti * tp, d.batch), dim3(OrthTile::NT), LDS, s, a);
-        FRA_HIP(hipGetLastError());
+        a.K = d.mp; a.alpha = cc / OR_SCALE; a.beta = cb;
+        if (int rc = product<f16, false, false>(a, d.batch, s)) return rc;
         // X <- a X + Q X
         a.ah = qh; a.al = qh + qlo; a.bh = a.eh = x; a.bl = a.el = x + xlo; a.ch = y; a.cl = y + xlo;
         a.sa = qe; a.sb = a.se = a.sc = xe; a.lda = d.mp; a.ldb = a.lde = a.ldc = d.np;
-        a.I = d.m; a.J = d.n; a.Jp = d.np; a.K = d.m; a.alpha = 1.0f / OR_SCALE; a.beta = ca; a.n_col_tiles = tx;
-        if (t == steps - 1) {
+        a.I = d.m; a.J = d.n; a.Jp = d.np; a.K = d.m; a.alpha = 1.0f / OR_SCALE; a.beta = ca;
+        if (t < steps - 1) {
+            if (int rc = product<f16, true, false>(a, d.batch, s)) return rc;
+        } else {
             a.ch = a.cl = nullptr;
             a.out = out; a.so = (int64_t)rows * cols; a.ldo = cols; a.transposed = d.transposed;
+            if (int rc = product<T, true, true>(a, d.batch, s)) return rc;
         }
-        hipLaunchKernelGGL((orth_product_kernel<T, true, OrthTile>), dim3(ti * tx, d.batch), dim3(OrthTile::NT), LDS, s, a);
-        FRA_HIP(hipGetLastError());
     }
     return FRA_OK;
 }

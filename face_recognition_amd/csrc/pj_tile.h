@@ -181,14 +181,16 @@ template <typename T, bool KMAJOR, int DIM, int NT, int KS> struct Operand {
         for (int j = 0; j < NLD; ++j) *reinterpret_cast<Frag*>(tile + (j * NT + tid) * 16) = v[j];
     }
     // ---- staging by DMA: every chunk is wholly inside or outside (klen or cols, pitch and base multiples of 16 bytes)
-    __device__ __forceinline__ void issue(const Src& d, int step, LdsPtr lds, int tid) const {
+    // `plus`: elements added to every address (a second operand of the same layout)
+    __device__ __forceinline__ void issue(const Src& d, int step, LdsPtr lds, int tid, int64_t plus = 0) const {
+        const int64_t at = advance(step) + plus;
         if ((step + 1) * KSTEP <= klen) {
 #pragma unroll
-            for (int j = 0; j < NLD; ++j) dma16(d.p[j] + advance(step), lds + j * (NT * 16));
+            for (int j = 0; j < NLD; ++j) dma16(d.p[j] + at, lds + j * (NT * 16));
         } else {
 #pragma unroll
             for (int j = 0; j < NLD; ++j)
-                dma16(valid(j, step, tid) > 0 ? d.p[j] + advance(step) : reinterpret_cast<const T*>(pj_zeros), lds + j * (NT * 16));
+                dma16(valid(j, step, tid) > 0 ? d.p[j] + at : reinterpret_cast<const T*>(pj_zeros), lds + j * (NT * 16));
         }
     }
     // fragment of the 16 rows / columns from `d0`, k group `ks` of the step
