@@ -100,7 +100,8 @@ template <typename T> __global__ __launch_bounds__(256) void orth_split_kernel(c
     }
 }
 
-// C = alpha A B^T + beta E (or A B where B is k-major), everything hi / lo f16, batch in blockIdx.y
+// C = alpha A B^T + beta E (or A B where B is k-major), everything hi / lo f16, a batch of matrices (a die works on one
+// or on neighbours: spread over all dies, a matrix's panels went through every L2, 4.8 TB/s of misses)
 struct OrthArgs {
     const f16 *ah, *al, *bh, *bl, *eh, *el;
     f16 *ch, *cl;               // nullptr: the last product, into out
@@ -110,7 +111,7 @@ struct OrthArgs {
     int64_t ldo;
     int I, J, Jp, K;            // C is [I][J], columns J .. Jp are written as zeros
     float alpha, beta;
-    int n_row_tiles, n_col_tiles, transposed;
+    int n_row_tiles, n_col_tiles, batch, transposed;
 };
 
 // The product of pairs: a step brings the hi and lo tiles of both operands, four tiles for three products (three products one
@@ -296,10 +297,10 @@ template <typename T, typename S> __device__ __forceinline__ void orth_emit_tran
 // LAST: the last product of the last step, into out (T)
 template <typename T, bool BK, bool LAST, typename S> __global__ __launch_bounds__(S::NT) void orth_product_kernel(OrthArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    int rt, ct;
-    if (!tile_of_block(blockIdx.x, a.n_row_tiles, a.n_col_tiles, rt, ct)) return;
+    int rt, ct, mat;
+    if (!tile_of_block(blockIdx.x, a.n_row_tiles, a.n_col_tiles, rt, ct, a.batch, mat)) return;
     const int i0 = rt * S::BI, j0 = ct * S::BJ;
-    const int64_t b = blockIdx.y;
+    const int64_t b = mat;
     f32x4 acc[S::MI][S::MJ];
     PairProduct<BK, S> p;
     p.A.order = nullptr; p.A.ld = a.lda; p.A.row0 = i0; p.A.rows = a.I - i0; p.A.klen = a.K; p.A.cols = 0; p.A.base = a.ah + b * a.sa;
@@ -326,8 +327,10 @@ template <typename T, bool BK, bool LAST, typename S> static int launch_orth(Ort
     if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(orth_product_kernel<T, BK, LAST, S>), lds, done)) return rc;
     a.n_row_tiles = (a.I + S::BI - 1) / S::BI;
     a.n_col_tiles = (a.Jp + S::BJ - 1) / S::BJ;
-    const int blocks = (a.n_row_tiles * a.n_col_tiles + 7) / 8 * 8;
-    hipLaunchKernelGGL((orth_product_kernel<T, BK, LAST, S>), dim3(blocks, batch), dim3(S::NT), lds, s, a);
+    a.batch = batch;
+    const int64_t blocks = ((int64_t)a.n_row_tiles * a.n_col_tiles * batch + 7) / 8 * 8;
+    FRA_REQUIRE(blocks < 2147483647LL, FRA_ERR_ARG, "fra_orthogonalize: %lld workgroups", (long long)blocks);
+    hipLaunchKernelGGL((orth_product_kernel<T, BK, LAST, S>), dim3((unsigned)blocks), dim3(S::NT), lds, s, a);
     FRA_HIP(hipGetLastError());
     return FRA_OK;
 }

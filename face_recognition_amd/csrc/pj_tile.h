@@ -244,14 +244,25 @@ template <typename T, bool KMAJOR, typename S> using OperandB = Operand<T, KMAJO
 // a die at a time is about square and reads each operand's panels once (with tiles dealt out row by row the dies together
 // fetched 105 MB through their L2s for a 4096 x 2048 x 1024 product whose operands are 12 MB).  Launch 8 ceil(tiles / 8)
 // workgroups at least; false: no tile left for this one.
-__device__ __forceinline__ bool tile_of_block(unsigned b, unsigned n_rt, unsigned n_ct, int& rt, int& ct) {
-    const unsigned all = n_rt * n_ct, x = b & 7, i = b >> 3, q = all >> 3, r = all & 7;         // below 2^31 (the launchers check)
+// With several matrices of tiles the eighths run through them one after the other.
+__device__ __forceinline__ bool tile_of_block(unsigned b, unsigned n_rt, unsigned n_ct, int& rt, int& ct, unsigned n_mat, int& mat) {
+    const unsigned each = n_rt * n_ct, all = n_mat * each, x = b & 7, i = b >> 3, q = all >> 3, r = all & 7;   // below 2^31 (the launchers check)
     if (i >= q + (x < r)) return false;
-    const unsigned id = x * q + (x < r ? x : r) + i, band = 8 * n_ct, first = id / band * 8;
+    unsigned id = x * q + (x < r ? x : r) + i;
+    mat = 0;
+    if (n_mat > 1) {
+        mat = (int)(id / each);
+        id -= mat * each;
+    }
+    const unsigned band = 8 * n_ct, first = id / band * 8;
     const unsigned in = id - first * n_ct, rows = n_rt - first < 8 ? n_rt - first : 8;
     ct = (int)(in / rows);
     rt = (int)(first + in - ct * rows);
     return true;
+}
+__device__ __forceinline__ bool tile_of_block(unsigned b, unsigned n_rt, unsigned n_ct, int& rt, int& ct) {
+    int mat;
+    return tile_of_block(b, n_rt, n_ct, rt, ct, 1, mat);
 }
 
 // Hands a workgroup's results on as 16-byte pieces of rows: a wave turns its accumulators through its own part of LDS, 16 rows
