@@ -57,12 +57,19 @@ struct RowArgs {
     const int* offsets;         // [G + 1] list entries of a group (grouped only)
     const int* tile_offsets;    // [G + 2], the last one the number of tiles in use (grouped only)
     int n_tiles, M, G;
+    int sub;                    // tiles a table entry is cut into (a kernel's tiles may be shorter than the table's)
 };
-__device__ __forceinline__ int tiles_in_use(const RowArgs& a) { return a.tiles ? a.tile_offsets[a.G + 1] : a.n_tiles; }
+__device__ __forceinline__ int tiles_in_use(const RowArgs& a) { return a.tiles ? a.tile_offsets[a.G + 1] * a.sub : a.n_tiles; }
 __device__ __forceinline__ bool row_tile(const RowArgs& a, int t, int bi, int& g, int& begin, int& end) {
     if (a.tiles) {
-        const int4 e = a.tiles[t];
+        const int part = a.sub > 1 ? t % a.sub : 0;
+        const int4 e = a.tiles[a.sub > 1 ? t / a.sub : t];
         g = e.x; begin = e.y; end = e.z;
+        if (a.sub > 1) {
+            begin += part * bi;
+            if (begin >= end) return false;
+            end = end - begin > bi ? begin + bi : end;
+        }
         return g >= 0;                                              // entries past the last tile
     }
     g = 0;
@@ -194,13 +201,13 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT, 
     }
 }
 
-// The same for few rows (tiles of 16 MT): a workgroup takes 16 columns, its four waves every fourth group of k, and their sums
-// meet in LDS, wave 0's first.  Bound by the latency of one trip to memory, or by W's bytes: a column's weights are read once,
+// The same for few rows (tiles of 16 MT): a workgroup takes 16 columns, its eight waves every eighth group of k (K = 512 is one
+// trip to memory), and their sums meet in LDS, added in a fixed order.  Bound by the latency of one trip to memory, or by W's bytes: a column's weights are read once,
 // straight into MFMA operands, in pieces of 64 bytes of sixteen rows whose neighbours the other waves take.
-template <typename T, int MT> __global__ __launch_bounds__(256) void pj_few_rows_kernel(FwdArgs a) {
+template <typename T, int MT> __global__ __launch_bounds__(512) void pj_few_rows_kernel(FwdArgs a) {
     typedef typename Elem<T>::Frag Frag;
-    constexpr int KG = Elem<T>::KG, EPC = Elem<T>::EPC, U = MT == 4 ? 2 : 4;
-    __shared__ float red[4][MT][16][17];
+    constexpr int KG = Elem<T>::KG, EPC = Elem<T>::EPC, U = 4, NW = 8;
+    __shared__ float red[NW][MT][16][17];
     const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
     int g, begin, end;
     if (!row_tile(a.rows, rt, 16 * MT, g, begin, end)) return;
@@ -217,11 +224,11 @@ template <typename T, int MT> __global__ __launch_bounds__(256) void pj_few_rows
             const int at = begin + 16 * i + m < end ? begin + 16 * i + m : end - 1;
             xr[i] = (const T*)a.x + (int64_t)(a.rows.order ? a.rows.order[at] : at) * a.ldx + q * EPC;
         }
-        for (int k0 = wave * KG; k0 < a.K; k0 += 4 * KG * U) {
+        for (int k0 = wave * KG; k0 < a.K; k0 += NW * KG * U) {
             Frag w[U], x[U][MT];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int k = k0 + u * 4 * KG, left = a.K - k - q * EPC;
+                const int k = k0 + u * NW * KG, left = a.K - k - q * EPC;
                 w[u] = load_chunk<T>(wr + k, left);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) x[u][i] = load_chunk<T>(xr[i] + k, left);
@@ -237,19 +244,19 @@ template <typename T, int MT> __global__ __launch_bounds__(256) void pj_few_rows
             for (int e = 0; e < 4; ++e) red[wave][i][m][4 * q + e] = acc[i][e];
     }
     __syncthreads();
-    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, n = n0 + c;
+    const int c = threadIdx.x & 15, r = (threadIdx.x >> 4) & 15, n = n0 + c;
     if (n >= a.N) return;
     float bi = 0.0f, sl = 0.0f;
     if (live && a.bias) bi = a.bias_f32 ? ((const float*)a.bias)[(int64_t)g * a.N + n] : (float)((const T*)a.bias)[(int64_t)g * a.N + n];
     if (live && a.slope) sl = a.slope_f32 ? ((const float*)a.slope)[(int64_t)g * a.N + n] : (float)((const T*)a.slope)[(int64_t)g * a.N + n];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = threadIdx.x >> 8; i < MT; i += 2) {
         const int at = begin + 16 * i + r;
         if (at >= end) continue;
         const int64_t row = a.rows.order ? a.rows.order[at] : at;
         float v = 0.0f;
         if (live) {
-            v = ((red[0][i][r][c] + red[1][i][r][c]) + (red[2][i][r][c] + red[3][i][r][c])) + bi;
+            v = ((red[0][i][r][c] + red[1][i][r][c]) + (red[2][i][r][c] + red[3][i][r][c])) +
+                ((red[4][i][r][c] + red[5][i][r][c]) + (red[6][i][r][c] + red[7][i][r][c])) + bi;
             if (a.z) ((T*)a.z)[row * a.N + n] = (T)v;
             v = pj_act<T>(a.act, v, sl);
         }
@@ -298,7 +305,7 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
 }
 
 // dW[g] = sum over the group's rows of dz^T x: both operands k-major.  `splits` workgroups share a group's rows and leave fp32
-// partial sums [split][G][N][K], which pj_join_kernel adds in order; one split writes dW itself.
+// partial sums [split][G][N][K], which pj_finish_kernel adds in order; one split writes dW itself.
 struct DwArgs {
     RowArgs rows;
     const void *dz, *x;
@@ -353,22 +360,6 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
         tile_emit<T, S>(acc, lds, f);
     }
 }
-// out[e] = sum over splits of part[s][e], s ascending
-template <typename T> __global__ __launch_bounds__(256) void pj_join_kernel(const float* part, T* out, int64_t n, int splits) {
-    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (e >= n) return;
-    float v[4] = {0, 0, 0, 0};
-    const int left = n - e < 4 ? (int)(n - e) : 4;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        float o[4];
-        load_four<float>(part + (int64_t)s * n + e, left, o);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += o[i];
-    }
-    store_four<T>(out + e, left, v);
-}
-
 // dz = dy act'(z) in list order and, per row tile, the column sums of dz and of dy min(z, 0).  A workgroup takes one row tile x
 // `lpr` 16-byte pieces of columns (lpr lanes side by side, a power of two up to 16, so that narrow pieces make many workgroups;
 // 256 / lpr rows at a time); four rows per lane are requested together.  Bound by HBM: dy and z in, dz out.
@@ -464,20 +455,46 @@ template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs
         }
     }
 }
-// out[g][n] = sum of part[t][n] over the group's tiles: 16 waves take every sixteenth tile of 64 columns, their sums are added in
-// order.  blockIdx.y: bias / slope
-struct ColsumArgs {
+// The sums that the passes before left in parts, in one launch:
+//   workgroups 0 .. n_join:  dw[e] = sum over splits of part[s][e], s ascending;
+//   the others:              out[g][n] = sum of part[t][n] over the group's tiles, for bias and slope: 16 waves take every sixteenth
+//                            tile of 64 columns, their sums are added in order.
+struct FinishArgs {
+    const float* dw_part;
+    void* dw;
+    int64_t n_dw;
+    int splits;
+    unsigned n_join;
     const float* part[2];
     void* out[2];
     int out_f32[2];
     const int* tile_offsets;
-    int n_tiles, N, n_col_tiles;
+    int n_tiles, N, n_col_tiles, both;      // both: bias and slope, else the one that is there
 };
-template <typename T> __global__ __launch_bounds__(1024) void pj_colsum_kernel(ColsumArgs a) {
+template <typename T> __global__ __launch_bounds__(1024) void pj_finish_kernel(FinishArgs a) {
     __shared__ float sums[16][64];
-    const int which = blockIdx.y;
-    if (!a.out[which]) return;
-    const int ct = blockIdx.x % a.n_col_tiles, g = blockIdx.x / a.n_col_tiles;
+    if (blockIdx.x < a.n_join) {
+        const int64_t e = ((int64_t)blockIdx.x * 1024 + threadIdx.x) * 4;
+        if (e >= a.n_dw) return;
+        float v[4] = {0, 0, 0, 0};
+        const int left = a.n_dw - e < 4 ? (int)(a.n_dw - e) : 4;
+#pragma unroll 4
+        for (int s = 0; s < a.splits; ++s) {
+            float o[4];
+            load_four<float>(a.dw_part + (int64_t)s * a.n_dw + e, left, o);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += o[i];
+        }
+        store_four<T>((T*)a.dw + e, left, v);
+        return;
+    }
+    unsigned b = blockIdx.x - a.n_join;
+    int which = a.out[0] ? 0 : 1;
+    if (a.both) {
+        which = b & 1;
+        b >>= 1;
+    }
+    const int ct = b % a.n_col_tiles, g = b / a.n_col_tiles;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = ct * 64 + lane;
     const int t0 = a.tile_offsets ? a.tile_offsets[g] : 0, t1 = a.tile_offsets ? a.tile_offsets[g + 1] : a.n_tiles;
     float v = 0.0f;
@@ -624,7 +641,7 @@ template <bool WRITE> __device__ __forceinline__ void group_tables(const GroupAr
 }
 // COUNT: a workgroup's counts; else place (the only workgroup, or after the counts, or after pj_group_scan_kernel)
 template <int NW, bool COUNT> __global__ __launch_bounds__(64 * NW) void pj_group_kernel(GroupArgs a) {
-    extern __shared__ int cnt[];                                    // [NW][keys]; place: + totals[keys], before[keys] (= tofs)
+    extern __shared__ int cnt[];                                    // [NW][keys]; place: + totals[keys], before[keys] (= tofs), not scanned: + counts[nb][keys]
     __shared__ int tmp[NW];
     const int keys = a.G + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = 64 * NW;
     int key[GR_KEYS], rank[GR_KEYS];
@@ -654,10 +671,13 @@ template <int NW, bool COUNT> __global__ __launch_bounds__(64 * NW) void pj_grou
             before[k] = a.counts[(int64_t)blockIdx.x * keys + k];
         }
     } else {
+        int* all = before + keys;                                   // [nb][keys]
+        for (int i = threadIdx.x; i < a.nb * keys; i += nt) all[i] = a.counts[i];
+        __syncthreads();
         for (int k = threadIdx.x; k < keys; k += nt) {
-            int all = 0;
-            for (int b = 0; b < a.nb; ++b) all += a.counts[(int64_t)b * keys + k];
-            totals[k] = all;
+            int sum = 0;
+            for (int b = 0; b < a.nb; ++b) sum += all[b * keys + k];
+            totals[k] = sum;
         }
         __syncthreads();
         if (blockIdx.x == 0) group_tables<true>(a, totals, before, tmp);
@@ -665,7 +685,7 @@ template <int NW, bool COUNT> __global__ __launch_bounds__(64 * NW) void pj_grou
         __syncthreads();
         for (int k = threadIdx.x; k < keys; k += nt) {
             int mine = 0;
-            for (int b = 0; b < (int)blockIdx.x; ++b) mine += a.counts[(int64_t)b * keys + k];
+            for (int b = 0; b < (int)blockIdx.x; ++b) mine += all[b * keys + k];
             before[k] = mine;
         }
     }
@@ -767,7 +787,8 @@ static RowArgs row_args(const fra_linear_desc* d, int tile_rows) {
     r.tiles = g ? (const int4*)g->tiles : nullptr;
     r.offsets = g ? g->offsets : nullptr;
     r.tile_offsets = g ? g->tile_offsets : nullptr;
-    r.n_tiles = g ? g->n_tiles : cdiv(d->M, tile_rows);
+    r.sub = g && g->tile_rows > tile_rows ? g->tile_rows / tile_rows : 1;
+    r.n_tiles = g ? g->n_tiles * r.sub : cdiv(d->M, tile_rows);
     r.M = (int)d->M;
     r.G = g ? g->n_groups : 1;
     return r;
@@ -778,13 +799,15 @@ static int check_grid(int64_t blocks, const char* what) {
 }
 // The side of a product's tiles.  256 x 256 moves half the bytes per product of 128 x 128 through the caches (8192 x 8192 x 8192:
 // 826 against 977 us) but holds one workgroup per compute unit, so it takes rounds that are nearly full (4096 x 2048 x 1024, half a
-// round: 37 against 24 us); 128 from one tile per unit on, 64 from three quarters of that on, below it 32 (1000 x 301 x 500 in fp32
-// is 80 tiles of 64 on 256 units).
-static int tile_side(int64_t rows, int64_t cols, bool f32) {
+// round: 37 against 24 us), and 16-bit operands: fp32 tiles are bound by the matrix cores at any size.  128 from one tile per unit
+// on, 64 from half of that on (2999 x 513 x 250 in fp32: 423 tiles of 64 15.5 us, 1598 of 32 21.3), below it 32 (1000 x 301 x 500 is
+// 80 tiles of 64 on 256 units).  Rows in groups: at most the table's tiles (`most`).
+static int tile_side(int64_t rows, int64_t cols, bool f32, int most = 256) {
     auto tiles = [&](int side) { return (int64_t)cdiv(rows, side) * cdiv(cols, side); };
     const int64_t huge = tiles(256);
-    if (!f32 && huge >= 512 && huge * 10 >= (huge + 255) / 256 * 256 * 9) return 256;
-    return tiles(128) >= 256 ? 128 : tiles(64) >= 192 ? 64 : 32;
+    if (most >= 256 && !f32 && huge >= 512 && huge * 10 >= (huge + 255) / 256 * 256 * 9) return 256;
+    if (most >= 128 && tiles(128) >= 256) return 128;
+    return most >= 64 && tiles(64) >= 128 ? 64 : 32;
 }
 
 template <typename T, typename S> static int launch_forward(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
@@ -801,7 +824,7 @@ template <typename T, int MT> static int launch_few_rows(const fra_linear_desc* 
     a.n_col_tiles = cdiv(d->N, 16);
     const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
     if (int rc = check_grid(blocks, "fra_linear")) return rc;
-    hipLaunchKernelGGL((pj_few_rows_kernel<T, MT>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((pj_few_rows_kernel<T, MT>), dim3((unsigned)blocks), dim3(512), 0, s, a);
     FRA_HIP(hipGetLastError());
     return FRA_OK;
 }
@@ -809,7 +832,8 @@ template <typename T> static int forward_t(const fra_linear_desc* d, void* z, vo
     FwdArgs a;
     // up to 64 rows: the kernel for few rows; then by the number of tiles
     const bool few = d->groups ? d->groups->tile_rows == 16 : d->M <= 64;
-    const int bi = d->groups ? d->groups->tile_rows : few ? (d->M <= 16 ? 16 : d->M <= 32 ? 32 : 64) : tile_side(d->M, d->N, sizeof(T) == 4);
+    const int bi = few ? (d->groups || d->M <= 16 ? 16 : d->M <= 32 ? 32 : 64)
+                       : tile_side(d->M, d->N, sizeof(T) == 4, d->groups ? d->groups->tile_rows : 256);
     a.rows = row_args(d, bi);
     a.x = d->x; a.w = d->w; a.bias = d->bias; a.slope = d->slope; a.resid = d->resid; a.z = z; a.y = y;
     a.ldx = d->ldx; a.ldw = d->ldw; a.wg = d->w_group_stride; a.ldr = d->ldr;
@@ -905,18 +929,6 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         hipLaunchKernelGGL((pj_dz_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
         FRA_HIP(hipGetLastError());
     }
-    if (p.need_sums) {
-        ColsumArgs a;
-        a.part[0] = (const float*)(ws + p.off_b); a.part[1] = (const float*)(ws + p.off_s);
-        a.out[0] = db; a.out[1] = ds;
-        a.out_f32[0] = d->bias_dtype == FRA_F32; a.out_f32[1] = d->slope_dtype == FRA_F32;
-        a.tile_offsets = g ? (const int*)g->tile_offsets : nullptr;
-        a.n_tiles = p.n_tiles; a.N = d->N; a.n_col_tiles = cdiv(d->N, 64);
-        const int64_t blocks = (int64_t)a.n_col_tiles * G;
-        if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
-        hipLaunchKernelGGL((pj_colsum_kernel<T>), dim3((unsigned)blocks, ds ? 2 : 1), dim3(1024), 0, s, a);
-        FRA_HIP(hipGetLastError());
-    }
     const void* dz = p.need_dz ? ws + p.off_dz : dy;
     const int64_t lddz = p.need_dz ? p.Np : lddy;
     if (dx && d->M > 0) {
@@ -930,7 +942,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
             if (int rc = launch_pack<T>(k, s)) return rc;
             a.w = k.dst; a.ldw = p.Kp; a.wg = (int64_t)d->N * p.Kp;
         }
-        const int bi = g ? g->tile_rows : tile_side(d->M, d->K, sizeof(T) == 4);
+        const int bi = tile_side(d->M, d->K, sizeof(T) == 4, g ? g->tile_rows : 256);
         a.rows = row_args(d, bi);
         a.dz = dz; a.dx = dx; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
         int rc = FRA_OK;
@@ -958,12 +970,28 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         const dim3 grid((unsigned)blocks, a.splits * G);
         if (p.dw_side == 128) PJ_LAUNCH((pj_dw_kernel<T, Big>), grid, Big::NT, Big::LDS, s, a);
         else PJ_LAUNCH((pj_dw_kernel<T, Small>), grid, Small::NT, Small::LDS, s, a);
+    }
+    if (p.need_sums || p.splits > 1) {
+        FinishArgs a = {};
+        int64_t blocks = 0;
         if (p.splits > 1) {
-            const int64_t n = (int64_t)G * d->N * d->K, jb = (n + 1023) / 1024;
-            if (int rc = check_grid(jb, "fra_linear_backward")) return rc;
-            hipLaunchKernelGGL((pj_join_kernel<T>), dim3((unsigned)jb), dim3(256), 0, s, (const float*)(ws + p.off_part), (T*)dw, n, p.splits);
-            FRA_HIP(hipGetLastError());
+            a.dw_part = (const float*)(ws + p.off_part); a.dw = dw; a.splits = p.splits;
+            a.n_dw = (int64_t)G * d->N * d->K;
+            blocks = (a.n_dw + 4095) / 4096;
+            if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
+            a.n_join = (unsigned)blocks;
         }
+        if (p.need_sums) {
+            a.part[0] = (const float*)(ws + p.off_b); a.part[1] = (const float*)(ws + p.off_s);
+            a.out[0] = db; a.out[1] = ds;
+            a.out_f32[0] = d->bias_dtype == FRA_F32; a.out_f32[1] = d->slope_dtype == FRA_F32;
+            a.tile_offsets = g ? (const int*)g->tile_offsets : nullptr;
+            a.n_tiles = p.n_tiles; a.N = d->N; a.n_col_tiles = cdiv(d->N, 64); a.both = db && ds;
+            blocks += (int64_t)a.n_col_tiles * G * (a.both ? 2 : 1);
+            if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
+        }
+        hipLaunchKernelGGL((pj_finish_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, s, a);
+        FRA_HIP(hipGetLastError());
     }
     return FRA_OK;
 }
@@ -976,7 +1004,7 @@ static int group_blocks(int64_t M, int n_groups) {
 template <int NW> static int launch_groups(GroupArgs& a, hipStream_t s) {
     const int keys = a.G + 1, most = (NW == 16 ? GR_WIDE_KEYS : GR_MAX_GROUPS + 1) * 4, lds = (NW + 2) * keys * 4;
     static std::atomic<uint64_t> done_count{0}, done_place{0};
-    if (int rc = raise_lds(pj_group_kernel<NW, false>, (NW + 2) * most, done_place)) return rc;
+    if (int rc = raise_lds(pj_group_kernel<NW, false>, (NW + 2) * most + GR_INLINE_SCAN * 4, done_place)) return rc;
     if (a.nb > 1) {
         if (int rc = raise_lds(pj_group_kernel<NW, true>, NW * most, done_count)) return rc;
         hipLaunchKernelGGL((pj_group_kernel<NW, true>), dim3(a.nb), dim3(64 * NW), NW * keys * 4, s, a);
@@ -987,7 +1015,8 @@ template <int NW> static int launch_groups(GroupArgs& a, hipStream_t s) {
             FRA_HIP(hipGetLastError());
         }
     }
-    hipLaunchKernelGGL((pj_group_kernel<NW, false>), dim3(a.nb), dim3(64 * NW), lds, s, a);
+    const int counts = a.nb > 1 && !a.scanned ? a.nb * keys * 4 : 0;
+    hipLaunchKernelGGL((pj_group_kernel<NW, false>), dim3(a.nb), dim3(64 * NW), lds + counts, s, a);
     FRA_HIP(hipGetLastError());
     return FRA_OK;
 }

@@ -17,6 +17,7 @@ captured into a graph.  Capture a backward pass as ``torch.autograd.grad`` on le
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -50,6 +51,15 @@ class _on_device:
             torch.cuda.set_device(self.prev)
 
 
+@lru_cache(maxsize=256)
+def _group_sizes(rows: int, n_groups: int):
+    """(rows of a tile, entries of the tile table, bytes of scratch) of so many rows and groups."""
+    lib = _lib.load()
+    need = C.c_size_t()
+    _lib.check(lib.fra_group_rows_workspace_bytes(rows, n_groups, C.byref(need)), "fra_group_rows_workspace_bytes")
+    return lib.fra_group_tile_rows(rows, n_groups), lib.fra_group_tiles(rows, n_groups), need.value
+
+
 class RowGroups:
     """The rows of a batch sorted by group (``group_rows``).
 
@@ -57,19 +67,24 @@ class RowGroups:
     [n_groups + 1]: group g's rows are ``order[offsets[g]:offsets[g + 1]]``.  Serves any number of products of these rows.
     """
 
-    def __init__(self, rows: int, n_groups: int, device: torch.device):
-        lib = _lib.load()
-        self.rows, self.n_groups, self.device = rows, n_groups, device
-        tile_rows, n_tiles = lib.fra_group_tile_rows(rows, n_groups), lib.fra_group_tiles(rows, n_groups)
+    def __init__(self, rows: int, n_groups: int, ids: torch.Tensor):
+        self.rows, self.n_groups, self.device = rows, n_groups, ids.device
+        tile_rows, n_tiles, _ = _group_sizes(rows, n_groups)
         # one allocation: tiles (16-byte aligned) | order | offsets | tile_offsets
-        buf = torch.empty(4 * n_tiles + rows + 2 * n_groups + 3, dtype=torch.int32, device=device)
-        at = 4 * n_tiles
-        self._buf = buf
-        self.order = buf[at:at + rows]
-        self.offsets = buf[at + rows:at + rows + n_groups + 1]
-        base = buf.data_ptr()
+        self._buf = ids.new_empty(4 * n_tiles + rows + 2 * n_groups + 3, dtype=torch.int32)
+        base, at = self._buf.data_ptr(), 4 * n_tiles
         self._desc = _lib.RowGroupsDesc(rows, n_groups, tile_rows, n_tiles, base + 4 * at, base + 4 * (at + rows), base,
                                         base + 4 * (at + rows + n_groups + 1))
+
+    @property
+    def order(self) -> torch.Tensor:
+        at = 4 * self._desc.n_tiles
+        return self._buf[at:at + self.rows]
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        at = 4 * self._desc.n_tiles + self.rows
+        return self._buf[at:at + self.n_groups + 1]
 
 
 def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
@@ -81,16 +96,14 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
     n_groups = int(n_groups)
     if not 1 <= n_groups <= MAX_GROUPS:
         raise RuntimeError(f"group_rows: {n_groups} groups (1 to {MAX_GROUPS})")
-    lib = _lib.load()
     ids = ids.contiguous()
+    rows = ids.shape[0]
+    need = _group_sizes(rows, n_groups)[2]
     with _on_device(ids.device):
-        g = RowGroups(ids.shape[0], n_groups, ids.device)
-        need = C.c_size_t()
-        _lib.check(lib.fra_group_rows_workspace_bytes(g.rows, n_groups, C.byref(need)), "fra_group_rows_workspace_bytes")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=ids.device) if need.value else None
-        _lib.check(lib.fra_group_rows(ids.data_ptr(), int(ids.dtype == torch.int64), C.byref(g._desc),
-                                      ws.data_ptr() if ws is not None else None, need.value,
-                                      _stream(ids.device)), "fra_group_rows")
+        g = RowGroups(rows, n_groups, ids)
+        ws = ids.new_empty(need, dtype=torch.uint8) if need else None
+        _lib.check(_lib.load().fra_group_rows(ids.data_ptr(), ids.dtype == torch.int64, C.byref(g._desc),
+                                              ws.data_ptr() if need else None, need, _stream(ids.device)), "fra_group_rows")
     return g
 
 
