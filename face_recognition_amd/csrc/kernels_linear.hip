@@ -415,10 +415,9 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void dz_row
         }
     }
 }
-template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs a) {
+template <typename T> __device__ __forceinline__ void dz_tile(const DzArgs& a, unsigned block, float (&sums)[256][Elem<T>::EPC + 1]) {
     constexpr int V = Elem<T>::EPC;
-    __shared__ float sums[256][V + 1];
-    const int ct = blockIdx.x % a.n_col_tiles, rt = blockIdx.x / a.n_col_tiles;
+    const int ct = block % a.n_col_tiles, rt = block / a.n_col_tiles;
     int g, begin, end;
     if (!row_tile(a.rows, rt, a.tile_rows, g, begin, end) || g >= a.rows.G) return;     // the same for the whole workgroup
     const int lpr = 1 << a.lpr_log2, lane = threadIdx.x & (lpr - 1), sub = threadIdx.x >> a.lpr_log2, nsub = 256 >> a.lpr_log2;
@@ -455,6 +454,41 @@ template <typename T> __global__ __launch_bounds__(256) void pj_dz_kernel(DzArgs
         }
     }
 }
+// rows of `src` (through `order`, or row r of group r / per_group) to rows of whole aligned chunks, zeros past `cols`
+struct PackArgs {
+    const void* src;
+    void* dst;
+    const int* order;
+    const int* count;           // rows to copy (device), nullptr: `rows`
+    int64_t ld, gs;
+    int rows, per_group, cols, cpr;     // cpr: chunks per row of dst
+    unsigned blocks;            // workgroups that share the rows, 0: nothing to copy
+};
+template <typename T> __device__ __forceinline__ void pack_rows(const PackArgs& a, unsigned block) {
+    typedef typename Elem<T>::Frag Frag;
+    const int64_t n = (int64_t)(a.count ? *a.count : a.rows) * a.cpr, stride = (int64_t)a.blocks * 256;
+    for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < n; i += stride) {
+        const int r = (int)(i / a.cpr), c = (int)(i - (int64_t)r * a.cpr) * Elem<T>::EPC;
+        const T* p = (const T*)a.src;
+        if (a.order) p += (int64_t)a.order[r] * a.ld;
+        else if (a.per_group) p += (int64_t)(r / a.per_group) * a.gs + (int64_t)(r % a.per_group) * a.ld;
+        else p += (int64_t)r * a.ld;
+        reinterpret_cast<Frag*>(a.dst)[i] = load_chunk<T>(p + c, a.cols - c);
+    }
+}
+// Everything the gradients' products wait for, in one launch: dz and the column sums, x in list order, W in aligned rows.
+struct PrepArgs {
+    DzArgs dz;
+    PackArgs x, w;
+    unsigned dz_blocks;
+};
+template <typename T> __global__ __launch_bounds__(256) void pj_prep_kernel(PrepArgs a) {
+    __shared__ float sums[256][Elem<T>::EPC + 1];
+    if (blockIdx.x < a.dz_blocks) dz_tile<T>(a.dz, blockIdx.x, sums);
+    else if (blockIdx.x < a.dz_blocks + a.x.blocks) pack_rows<T>(a.x, blockIdx.x - a.dz_blocks);
+    else pack_rows<T>(a.w, blockIdx.x - a.dz_blocks - a.x.blocks);
+}
+
 // The sums that the passes before left in parts, in one launch:
 //   workgroups 0 .. n_join:  dw[e] = sum over splits of part[s][e], s ascending;
 //   the others:              out[g][n] = sum of part[t][n] over the group's tiles, for bias and slope: 16 waves take every sixteenth
@@ -512,34 +546,12 @@ template <typename T> __global__ __launch_bounds__(1024) void pj_finish_kernel(F
         else ((T*)a.out[which])[(int64_t)g * a.N + n] = (T)v;
     }
 }
-// rows of `src` (through `order`, or row r of group r / per_group) to rows of whole aligned chunks, zeros past `cols`
-struct PackArgs {
-    const void* src;
-    void* dst;
-    const int* order;
-    const int* count;           // rows to copy (device), nullptr: `rows`
-    int64_t ld, gs;
-    int rows, per_group, cols, cpr;     // cpr: chunks per row of dst
-};
-template <typename T> __global__ __launch_bounds__(256) void pj_pack_kernel(PackArgs a) {
-    typedef typename Elem<T>::Frag Frag;
-    const int64_t n = (int64_t)(a.count ? *a.count : a.rows) * a.cpr, stride = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-        const int r = (int)(i / a.cpr), c = (int)(i - (int64_t)r * a.cpr) * Elem<T>::EPC;
-        const T* p = (const T*)a.src;
-        if (a.order) p += (int64_t)a.order[r] * a.ld;
-        else if (a.per_group) p += (int64_t)(r / a.per_group) * a.gs + (int64_t)(r % a.per_group) * a.ld;
-        else p += (int64_t)r * a.ld;
-        reinterpret_cast<Frag*>(a.dst)[i] = load_chunk<T>(p + c, a.cols - c);
-    }
-}
-
 // ---- rows by group: a stable counting sort --------------------------------------------------------------------------
-// key = id, or G where id is outside [0, G).  A workgroup of NW waves owns NW * 256 consecutive rows, a wave 256 of them, kept
-// as four keys per lane.  Lanes with the same key find each other by ballots over the key's bits, so a row's rank among its
+// key = id, or G where id is outside [0, G).  A workgroup of NW waves owns NW * 512 consecutive rows, a wave 512 of them, kept
+// as eight keys per lane.  Lanes with the same key find each other by ballots over the key's bits, so a row's rank among its
 // wave's rows of the key is the wave's running count plus the equal lanes below: no atomics, and the order does not depend on
 // timing.  One launch for one workgroup; else the counts of all workgroups first.
-constexpr int GR_MAX_GROUPS = 4096, GR_KEYS = 4, GR_WAVE_ROWS = 64 * GR_KEYS;
+constexpr int GR_MAX_GROUPS = 4096, GR_KEYS = 8, GR_WAVE_ROWS = 64 * GR_KEYS;
 constexpr int GR_WIDE_KEYS = 1025;          // up to this many keys sixteen waves' counters fit in LDS, beyond it four waves'
 constexpr int GR_INLINE_SCAN = 8192;        // counters up to which every workgroup adds the others' counts itself
 struct GroupArgs {
@@ -889,13 +901,6 @@ static BackwardPlan backward_plan(const fra_linear_desc* d, bool dx, bool dw, bo
     return d->dtype == FRA_F32 ? backward_plan_t<float>(d, dx, dw, db, ds) : backward_plan_t<f16>(d, dx, dw, db, ds);
 }
 
-template <typename T> static int launch_pack(const PackArgs& a, hipStream_t s) {
-    const int64_t chunks = (int64_t)a.rows * a.cpr, blocks = (chunks + 255) / 256;
-    if (blocks == 0) return FRA_OK;
-    hipLaunchKernelGGL((pj_pack_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a);
-    FRA_HIP(hipGetLastError());
-    return FRA_OK;
-}
 template <typename T, typename S> static int launch_dx(DxArgs& a, hipStream_t s) {
     a.n_col_tiles = cdiv(a.K, S::BJ);
     const int64_t blocks = ((int64_t)a.rows.n_tiles * a.n_col_tiles + 7) / 8 * 8;
@@ -911,8 +916,10 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
     const int G = g ? g->n_groups : 1;
     // without groups or activation an aligned dy is dz
     if (!g && d->act == PJ_NONE && dma_ok<T>(dy, lddy, d->N)) p.need_dz = false;
+    PrepArgs prep = {};
+    int64_t prep_blocks = 0;
     if ((p.need_dz || p.need_sums) && d->M > 0) {
-        DzArgs a;
+        DzArgs& a = prep.dz;
         a.rows = row_args(d, p.dz_rows);
         a.dy = dy; a.z = z; a.slope = d->slope;
         a.dz = p.need_dz ? ws + p.off_dz : nullptr;
@@ -924,9 +931,29 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         a.lpr_log2 = 0;
         while (a.lpr_log2 < 4 && (1 << a.lpr_log2) < pieces) ++a.lpr_log2;
         a.n_col_tiles = cdiv(pieces, 1 << a.lpr_log2);
-        const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
-        if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
-        hipLaunchKernelGGL((pj_dz_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+        prep_blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
+        if (int rc = check_grid(prep_blocks, "fra_linear_backward")) return rc;
+        prep.dz_blocks = (unsigned)prep_blocks;
+    }
+    auto pack_blocks = [](int64_t rows, int cpr) { const int64_t b = (rows * cpr + 255) / 256; return (unsigned)(b < 2048 ? b : 2048); };
+    if (p.pack_x && d->M > 0) {
+        PackArgs& k = prep.x;
+        k.src = d->x; k.dst = ws + p.off_x; k.order = g ? (const int*)g->order : nullptr; k.count = g ? g->offsets + G : nullptr;
+        k.ld = d->ldx; k.rows = (int)d->M; k.cols = d->K; k.cpr = p.Kp / Elem<T>::EPC;
+        k.blocks = pack_blocks(d->M, k.cpr);
+        prep_blocks += k.blocks;
+    }
+    if (p.pack_w && d->M > 0) {
+        PackArgs& k = prep.w;
+        FRA_REQUIRE((int64_t)G * d->N <= 2147483647LL, FRA_ERR_ARG, "fra_linear_backward: %d matrices of %d rows", G, d->N);
+        k.src = d->w; k.dst = ws + p.off_w; k.ld = d->ldw; k.gs = d->w_group_stride;
+        k.rows = G * d->N; k.per_group = d->N; k.cols = d->K; k.cpr = p.Kp / Elem<T>::EPC;
+        k.blocks = pack_blocks(k.rows, k.cpr);
+        prep_blocks += k.blocks;
+    }
+    if (prep_blocks > 0) {
+        if (int rc = check_grid(prep_blocks, "fra_linear_backward")) return rc;
+        hipLaunchKernelGGL((pj_prep_kernel<T>), dim3((unsigned)prep_blocks), dim3(256), 0, s, prep);
         FRA_HIP(hipGetLastError());
     }
     const void* dz = p.need_dz ? ws + p.off_dz : dy;
@@ -935,12 +962,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         DxArgs a;
         a.w = d->w; a.ldw = d->ldw; a.wg = d->w_group_stride;
         if (p.pack_w) {
-            PackArgs k;
-            k.src = d->w; k.dst = ws + p.off_w; k.order = nullptr; k.count = nullptr; k.ld = d->ldw; k.gs = d->w_group_stride;
-            FRA_REQUIRE((int64_t)G * d->N <= 2147483647LL, FRA_ERR_ARG, "fra_linear_backward: %d matrices of %d rows", G, d->N);
-            k.rows = G * d->N; k.per_group = d->N; k.cols = d->K; k.cpr = p.Kp / Elem<T>::EPC;
-            if (int rc = launch_pack<T>(k, s)) return rc;
-            a.w = k.dst; a.ldw = p.Kp; a.wg = (int64_t)d->N * p.Kp;
+            a.w = ws + p.off_w; a.ldw = p.Kp; a.wg = (int64_t)d->N * p.Kp;
         }
         const int bi = tile_side(d->M, d->K, sizeof(T) == 4, g ? g->tile_rows : 256);
         a.rows = row_args(d, bi);
@@ -956,11 +978,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         DwArgs a;
         a.x = d->x; a.ldx = d->ldx;
         if (p.pack_x) {
-            PackArgs k;
-            k.src = d->x; k.dst = ws + p.off_x; k.order = g ? (const int*)g->order : nullptr; k.count = g ? g->offsets + G : nullptr;
-            k.ld = d->ldx; k.gs = 0; k.rows = (int)d->M; k.per_group = 0; k.cols = d->K; k.cpr = p.Kp / Elem<T>::EPC;
-            if (int rc = launch_pack<T>(k, s)) return rc;
-            a.x = k.dst; a.ldx = p.Kp;
+            a.x = ws + p.off_x; a.ldx = p.Kp;
         }
         a.rows = row_args(d, 128);
         a.dz = dz; a.dw = p.splits > 1 ? (void*)(ws + p.off_part) : dw; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;

@@ -120,7 +120,7 @@ template <bool BK, typename S> struct PairProduct {
     typedef OperandA<f16, false, S> OA;
     typedef OperandB<f16, BK, S> OB;
     static constexpr int NB = S::NB, BUF = 2 * S::STEP, NLD = 2 * (OA::NLD + OB::NLD), LDS = NB * BUF;
-    static_assert(NB >= 2 && NB <= 4 && S::KS == 2, "");
+    static_assert(NB >= 2 && S::KS == 2, "");
     OA A;
     OB B;
     typename OA::Src sa;
@@ -133,12 +133,6 @@ template <bool BK, typename S> struct PairProduct {
         A.issue(sa, step, dst + OA::BYTES, tid, a_lo);
         B.issue(sb, step, dst + 2 * OA::BYTES, tid);
         B.issue(sb, step, dst + 2 * OA::BYTES + OB::BYTES, tid, b_lo);
-    }
-    template <int Y> __device__ __forceinline__ static void arrived(int behind) {
-        if (behind >= Y) dma_wait_barrier<Y * NLD>();
-        else if (Y > 2 && behind == 2) dma_wait_barrier<2 * NLD>();
-        else if (Y > 1 && behind == 1) dma_wait_barrier<NLD>();
-        else dma_wait_barrier<0>();
     }
     struct PairFrags {
         typename Elem<f16>::Frag ah[S::MI], al[S::MI], bh[S::MJ], bl[S::MJ];
@@ -186,7 +180,7 @@ template <bool BK, typename S> struct PairProduct {
         for (int t = 0; t < NB; ++t)
             if (t < steps) issue(t, dst + t * BUF, tid);
         PairFrags f0, f1;
-        arrived<NB - 1>(steps - 1);
+        step_arrived<NB - 1, NLD>(steps - 1);
         f0.read(lds, 0, i0, j0, lane);
         int cur = 0;
         for (int t = 0; t < steps; ++t) {
@@ -196,7 +190,7 @@ template <bool BK, typename S> struct PairProduct {
             __builtin_amdgcn_sched_barrier(0);
             const int nxt = cur + BUF == NB * BUF ? 0 : cur + BUF;
             if (t + 1 < steps) {
-                arrived<NB - 2>(steps - 2 - t);
+                step_arrived<NB - 2, NLD>(steps - 2 - t);
                 if (t + NB < steps) issue(t + NB, dst + cur, tid);
                 f0.read(lds + nxt, 0, i0, j0, lane);
             }

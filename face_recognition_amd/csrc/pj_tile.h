@@ -116,6 +116,13 @@ __device__ __forceinline__ void dma16(const void* g, LdsPtr lds) {
 template <int N> __device__ __forceinline__ void dma_wait_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+// the oldest step on its way (NLD loads each) has arrived for every wave: at most Y younger ones are still out, fewer if fewer
+// than that (`behind`) come after it
+template <int Y, int NLD> __device__ __forceinline__ void step_arrived(int behind) {
+    static_assert(Y * NLD < 64, "the counter's range");
+    if (behind >= Y) dma_wait_barrier<Y * NLD>();
+    else if constexpr (Y > 0) step_arrived<Y - 1, NLD>(behind);
+}
 // what a lane reads in place of a chunk outside its operand
 static __device__ __attribute__((aligned(16))) const float pj_zeros[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
@@ -344,7 +351,7 @@ template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
     typedef OperandA<T, AK, S> OA;
     typedef OperandB<T, BK, S> OB;
     static constexpr int NB = S::NB, BUF = S::STEP, NLD = OA::NLD + OB::NLD;
-    static_assert(OA::BYTES + OB::BYTES == BUF && NB >= 2 && NB <= 4 && S::KS == 2, "");
+    static_assert(OA::BYTES + OB::BYTES == BUF && NB >= 2 && S::KS == 2, "");
     OA A;
     OB B;
     typename OA::Src sa;
@@ -370,14 +377,6 @@ template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
                 }
         }
     }
-    // the oldest step on its way has arrived for every wave: at most Y younger ones are still out, fewer if fewer than that
-    // (`behind`) come after it
-    template <int Y> __device__ __forceinline__ static void arrived(int behind) {
-        if (behind >= Y) dma_wait_barrier<Y * NLD>();
-        else if (Y > 2 && behind == 2) dma_wait_barrier<2 * NLD>();
-        else if (Y > 1 && behind == 1) dma_wait_barrier<NLD>();
-        else dma_wait_barrier<0>();
-    }
     template <bool ADD = false> __device__ __forceinline__ void run(char* lds, f32x4 (&acc)[S::MI][S::MJ]) const {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
@@ -392,7 +391,7 @@ template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
         if constexpr (DMA) {
             const LdsPtr dst = dma_base(lds);
             Frags<T, AK, BK, S> f0, f1;
-            arrived<NB - 1>(steps - 1);
+            step_arrived<NB - 1, NLD>(steps - 1);
             f0.read(lds, 0, i0, j0, lane);
             int cur = 0;
             for (int t = 0; t < steps; ++t) {
@@ -402,7 +401,7 @@ template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
                 __builtin_amdgcn_sched_barrier(0);
                 const int nxt = cur + BUF == NB * BUF ? 0 : cur + BUF;
                 if (t + 1 < steps) {
-                    arrived<NB - 2>(steps - 2 - t);
+                    step_arrived<NB - 2, NLD>(steps - 2 - t);
                     if (t + NB < steps) {
                         A.issue(sa, t + NB, dst + cur, tid);
                         B.issue(sb, t + NB, dst + cur + OA::BYTES, tid);
