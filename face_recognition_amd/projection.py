@@ -137,6 +137,7 @@ def _weight(weight):
 
 
 def _forward(x, weight, bias, slope, residual, act, groups, want_preact):
+    """(out, preact, descriptor, (x, weight, slope) as the kernels read them)."""
     x, ldx = _rows(x)
     weight, ldw, wg = _weight(weight)
     ldr = 0
@@ -148,56 +149,67 @@ def _forward(x, weight, bias, slope, residual, act, groups, want_preact):
         slope = slope.contiguous()
     out = x.new_empty((x.shape[0], weight.shape[-2]))
     z = torch.empty_like(out) if want_preact else None
+    d = _desc(x, ldx, weight, ldw, wg, bias, slope, residual, ldr, act, groups)
     if out.shape[0]:
-        d = _desc(x, ldx, weight, ldw, wg, bias, slope, residual, ldr, act, groups)
         with _on_device(x.device):
             _lib.check(_lib.load().fra_linear(C.byref(d), z.data_ptr() if z is not None else None, out.data_ptr(),
                                               _stream(x.device)), "fra_linear")
-    return out, z
+    return out, z, d, (x, weight, slope)
+
+
+def _backward(ctx, dy):
+    x, weight, slope, z = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    d = ctx.desc
+    dx = dw = db = ds = None
+    if need[0] or need[1] or need[2] or need[3]:
+        if need[0]:
+            dx = x.new_empty(x.shape)
+        if need[1]:
+            dw = x.new_empty(weight.shape)
+        if need[2]:
+            db = x.new_empty(weight.shape[:-1], dtype=ctx.bias_dtype)
+        if need[3]:
+            ds = x.new_empty(weight.shape[:-1], dtype=slope.dtype)
+        if x.data_ptr() != d.x or weight.data_ptr() != d.w or (slope is not None and slope.data_ptr() != d.slope):
+            # what was saved came back as other tensors (saved-tensor hooks)
+            x, d.ldx = _rows(x)
+            weight, d.ldw, d.w_group_stride = _weight(weight)
+            slope = slope.contiguous() if slope is not None else None
+            d.x, d.w, d.slope = x.data_ptr(), weight.data_ptr(), slope.data_ptr() if slope is not None else None
+        if z is not None:
+            z = z.contiguous()
+        lib = _lib.load()
+        g, lddy = _rows(dy)
+        with _on_device(x.device):
+            nbytes = C.c_size_t()
+            _lib.check(lib.fra_linear_backward_workspace_bytes(C.byref(d), need[0], need[1], need[2], need[3], C.byref(nbytes)),
+                       "fra_linear_backward_workspace_bytes")
+            ws = x.new_empty(nbytes.value, dtype=torch.uint8)
+            _lib.check(lib.fra_linear_backward(C.byref(d), z.data_ptr() if z is not None else None, g.data_ptr(), lddy,
+                                               dx.data_ptr() if need[0] else None, dw.data_ptr() if need[1] else None,
+                                               db.data_ptr() if need[2] else None, ds.data_ptr() if need[3] else None,
+                                               ws.data_ptr(), nbytes.value, _stream(x.device)), "fra_linear_backward")
+    return dx, dw, db, ds, (dy if need[4] else None), None, None
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, slope, residual, act, groups):
         need = ctx.needs_input_grad
-        want = act != 0 and any(need[:4])
-        out, z = _forward(x, weight, bias, slope, residual, act, groups, want)
-        ctx.save_for_backward(x, weight, slope, z)
-        ctx.act, ctx.groups = act, groups
+        out, z, d, kept = _forward(x, weight, bias, slope, residual, act, groups,
+                                   act != 0 and (need[0] or need[1] or need[2] or need[3]))
+        ctx.save_for_backward(*kept, z)
+        ctx.desc, ctx.groups = d, groups
         ctx.bias_dtype = bias.dtype if bias is not None else None
         return out
 
+    # once differentiable; the wrapper that says so is needed only where a graph of the backward pass is being built
+    _once = staticmethod(torch.autograd.function.once_differentiable(_backward))
+
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, slope, z = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dev = x.device
-        dx = x.new_empty(x.shape) if need[0] else None
-        dw = x.new_empty(weight.shape) if need[1] else None
-        par = weight.shape[:-1]
-        db = x.new_empty(par, dtype=ctx.bias_dtype) if need[2] else None
-        ds = x.new_empty(par, dtype=slope.dtype) if need[3] else None
-        if any(need[:4]):
-            lib = _lib.load()
-            g, lddy = _rows(dy)
-            xr, ldx = _rows(x)
-            w, ldw, wg = _weight(weight)
-            if slope is not None:
-                slope = slope.contiguous()
-            d = _desc(xr, ldx, w, ldw, wg, None, slope, None, 0, ctx.act, ctx.groups)
-            if ctx.bias_dtype is not None:
-                d.bias_dtype = _DTYPES[ctx.bias_dtype]
-            nbytes = C.c_size_t()
-            _lib.check(lib.fra_linear_backward_workspace_bytes(C.byref(d), need[0], need[1], need[2], need[3],
-                                                               C.byref(nbytes)), "fra_linear_backward_workspace_bytes")
-            with _on_device(dev):
-                ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-                ptr = [t.data_ptr() if t is not None else None for t in (dx, dw, db, ds)]
-                _lib.check(lib.fra_linear_backward(C.byref(d), z.data_ptr() if z is not None else None, g.data_ptr(), lddy,
-                                                   *ptr, ws.data_ptr(), nbytes.value, _stream(dev)),
-                           "fra_linear_backward")
-        return dx, dw, db, ds, (dy if need[4] else None), None, None
+        return _Linear._once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def _check(what, x, weight, bias, activation, slope, residual, lead):

@@ -355,6 +355,27 @@ def test_parameters_in_fp32_and_partial_gradients(device):
         assert not call(t, "prelu").requires_grad
 
 
+def test_once_differentiable_and_saved_tensor_hooks(device):
+    t = make(50, 24, 40, torch.float32, device, 55, act="prelu")
+    full = run(t, "prelu")
+    x = t["x"].clone().requires_grad_(True)
+    dx, = torch.autograd.grad(call(dict(t, x=x), "prelu").pow(2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+    # what was saved comes back from elsewhere, and laid out differently
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), lambda v: v.to(device).t().contiguous().t() if v.dim() == 2 else v.to(device)):
+        out = run(t, "prelu")
+    for name, v in full.items():
+        assert torch.equal(out[name], v), name
+    # an input changed between the passes is noticed
+    w = t["w"].clone().requires_grad_(True)
+    y = call(dict(t, w=w), "prelu")
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, w, t["dy"])
+
+
 def test_captured_and_replayed(device):
     m, k, n, groups = 500, 136, 72, 5
     t = make(m, k, n, torch.bfloat16, device, 61, lead=(groups,), act="prelu")
