@@ -114,26 +114,18 @@ struct OrthArgs {
     int n_row_tiles, n_col_tiles, batch, transposed;
 };
 
-// The product of pairs: a step brings the hi and lo tiles of both operands, four tiles for three products (three products one
-// after the other would bring six).  Everything else is as in Product.
-template <bool BK, typename S> struct PairProduct {
+// The product of pairs.  TOGETHER: a step brings the hi and lo tiles of both operands, four tiles for the three products (which
+// one after the other need six); else the three products are one chain of steps, lo hi, hi lo, hi hi, with half the LDS per step,
+// which makes room for tiles of twice the side.
+template <bool BK, typename S, bool TOGETHER> struct PairProduct {
     typedef OperandA<f16, false, S> OA;
     typedef OperandB<f16, BK, S> OB;
-    static constexpr int NB = S::NB, BUF = 2 * S::STEP, NLD = 2 * (OA::NLD + OB::NLD), LDS = NB * BUF;
+    static constexpr int NB = S::NB, BUF = (TOGETHER ? 2 : 1) * S::STEP, NLD = (TOGETHER ? 2 : 1) * (OA::NLD + OB::NLD), LDS = NB * BUF;
     static_assert(NB >= 2 && S::KS == 2, "");
     OA A;
     OB B;
-    typename OA::Src sa;
-    typename OB::Src sb;
     int64_t a_lo, b_lo;         // elements from an operand's hi part to its lo part
-    int steps;
 
-    __device__ __forceinline__ void issue(int step, LdsPtr dst, int tid) const {
-        A.issue(sa, step, dst, tid);
-        A.issue(sa, step, dst + OA::BYTES, tid, a_lo);
-        B.issue(sb, step, dst + 2 * OA::BYTES, tid);
-        B.issue(sb, step, dst + 2 * OA::BYTES + OB::BYTES, tid, b_lo);
-    }
     struct PairFrags {
         typename Elem<f16>::Frag ah[S::MI], al[S::MI], bh[S::MJ], bl[S::MJ];
         __device__ __forceinline__ void read(const char* step, int ks, int i0, int j0, int lane) {
@@ -172,34 +164,29 @@ template <bool BK, typename S> struct PairProduct {
         for (int mi = 0; mi < S::MI; ++mi)
 #pragma unroll
             for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
-        steps = (klen + OA::KSTEP - 1) / OA::KSTEP;
+        const int each = (klen + OA::KSTEP - 1) / OA::KSTEP, steps = TOGETHER ? each : 3 * each;
+        typename OA::Src sa;
+        typename OB::Src sb;
         A.init(sa, tid);
         B.init(sb, tid);
         const LdsPtr dst = (LdsPtr)lds + __builtin_amdgcn_readfirstlane(wave) * 1024;
+        auto issue = [&](int t, LdsPtr to) {
+            if constexpr (TOGETHER) {
+                A.issue(sa, t, to, tid);
+                A.issue(sa, t, to + OA::BYTES, tid, a_lo);
+                B.issue(sb, t, to + 2 * OA::BYTES, tid);
+                B.issue(sb, t, to + 2 * OA::BYTES + OB::BYTES, tid, b_lo);
+            } else {
+                const int part = t >= 2 * each ? 2 : t >= each ? 1 : 0, k = t - part * each;
+                A.issue(sa, k, to, tid, part == 0 ? a_lo : 0);
+                B.issue(sb, k, to + OA::BYTES, tid, part == 1 ? b_lo : 0);
+            }
+        };
 #pragma unroll
         for (int t = 0; t < NB; ++t)
-            if (t < steps) issue(t, dst + t * BUF, tid);
-        PairFrags f0, f1;
-        step_arrived<NB - 1, NLD>(steps - 1);
-        f0.read(lds, 0, i0, j0, lane);
-        int cur = 0;
-        for (int t = 0; t < steps; ++t) {
-            f1.read(lds + cur, 1, i0, j0, lane);
-            __builtin_amdgcn_sched_barrier(0);
-            f0.mma(acc);
-            __builtin_amdgcn_sched_barrier(0);
-            const int nxt = cur + BUF == NB * BUF ? 0 : cur + BUF;
-            if (t + 1 < steps) {
-                step_arrived<NB - 2, NLD>(steps - 2 - t);
-                if (t + NB < steps) issue(t + NB, dst + cur, tid);
-                f0.read(lds + nxt, 0, i0, j0, lane);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            f1.mma(acc);
-            __builtin_amdgcn_sched_barrier(0);
-            cur = nxt;
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (t < steps) issue(t, dst + t * BUF);
+        if constexpr (TOGETHER) run_steps<NB, NLD, BUF, PairFrags>(steps, lds, dst, issue, i0, j0, lane, acc);
+        else run_steps<NB, NLD, BUF, Frags<f16, false, BK, S>>(steps, lds, dst, issue, i0, j0, lane, acc);
     }
 };
 
@@ -251,52 +238,57 @@ template <typename T> struct OrthEmit {
         }
     }
 };
-// the last product of a transposed matrix: out[j][i], a wave's part turned through LDS so that a lane writes V neighbouring i
-template <typename T, typename S> __device__ __forceinline__ void orth_emit_transposed(const OrthArgs& a, int64_t b, int i0, int j0, const f32x4 (&acc)[S::MI][S::MJ], char* lds) {
-    constexpr int V = 16 / sizeof(T), ROWS = S::MI * 16, LPR = ROWS / V, RPP = 64 / LPR, PITCH = ROWS + 4;
-    static_assert(S::WI * S::WJ * S::MJ * 16 * PITCH * 4 <= 2 * S::LDS, "");
+// the last product of a transposed matrix: out[j][i], a wave's part turned through LDS, 32 rows at a time, so that a lane writes V
+// neighbouring i
+template <typename T, typename S, int LDS> __device__ __forceinline__ void orth_emit_transposed(const OrthArgs& a, int64_t b, int i0, int j0, const f32x4 (&acc)[S::MI][S::MJ], char* lds) {
+    constexpr int MG = S::MI < 2 ? S::MI : 2, V = 16 / sizeof(T), ROWS = MG * 16, LPR = ROWS / V, RPP = 64 / LPR, PITCH = ROWS + 4;
+    static_assert(S::WI * S::WJ * S::MJ * 16 * PITCH * 4 <= LDS && S::MI % MG == 0 && (S::MJ * 16) % RPP == 0, "the waves' parts fit");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wi = i0 + (wave % S::WI) * (S::BI / S::WI), wj = j0 + (wave / S::WI) * (S::BJ / S::WJ);
     float* strip = reinterpret_cast<float*>(lds) + wave * (S::MJ * 16 * PITCH);
 #pragma unroll
-    for (int mi = 0; mi < S::MI; ++mi) {
-        const int i = wi + 16 * mi + (lane & 15);
+    for (int m0 = 0; m0 < S::MI; m0 += MG) {
 #pragma unroll
-        for (int mj = 0; mj < S::MJ; ++mj) {
-            const int jl = 16 * mj + 4 * (lane >> 4), j = wj + jl;
-            float h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
-            if (i < a.I && j < a.Jp) {
-                load_four<f16>(a.eh + b * a.se + (int64_t)i * a.lde + j, 4, h);
-                load_four<f16>(a.el + b * a.se + (int64_t)i * a.lde + j, 4, l);
+        for (int mi = 0; mi < MG; ++mi) {
+            const int i = wi + 16 * (m0 + mi) + (lane & 15);
+#pragma unroll
+            for (int mj = 0; mj < S::MJ; ++mj) {
+                const int jl = 16 * mj + 4 * (lane >> 4), j = wj + jl;
+                float h[4] = {0, 0, 0, 0}, l[4] = {0, 0, 0, 0};
+                if (i < a.I && j < a.Jp) {
+                    load_four<f16>(a.eh + b * a.se + (int64_t)i * a.lde + j, 4, h);
+                    load_four<f16>(a.el + b * a.se + (int64_t)i * a.lde + j, 4, l);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    strip[(jl + e) * PITCH + 16 * mi + (lane & 15)] = (a.alpha * acc[m0 + mi][mj][e] + a.beta * (h[e] + l[e])) * (1.0f / OR_SCALE);
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                strip[(jl + e) * PITCH + 16 * mi + (lane & 15)] = (a.alpha * acc[mi][mj][e] + a.beta * (h[e] + l[e])) * (1.0f / OR_SCALE);
         }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int jl = 0; jl < S::MJ * 16; jl += RPP) {
-        const int jr = jl + lane / LPR, j = wj + jr, il = (lane % LPR) * V, i = wi + il;
-        typename Elem<T>::Frag o;
+        for (int jl = 0; jl < S::MJ * 16; jl += RPP) {
+            const int jr = jl + lane / LPR, j = wj + jr, il = (lane % LPR) * V, i = wi + 16 * m0 + il;
+            typename Elem<T>::Frag o;
 #pragma unroll
-        for (int q = 0; q < V; q += 4) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(strip + jr * PITCH + il + q);
+            for (int q = 0; q < V; q += 4) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(strip + jr * PITCH + il + q);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[q + e] = (T)x[e];
+                for (int e = 0; e < 4; ++e) o[q + e] = (T)x[e];
+            }
+            if (j < a.J && i < a.I) store_chunk<T>((T*)a.out + b * a.so + (int64_t)j * a.ldo + i, a.I - i, o);
         }
-        if (j < a.J && i < a.I) store_chunk<T>((T*)a.out + b * a.so + (int64_t)j * a.ldo + i, a.I - i, o);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 // LAST: the last product of the last step, into out (T)
-template <typename T, bool BK, bool LAST, typename S> __global__ __launch_bounds__(S::NT) void orth_product_kernel(OrthArgs a) {
+template <typename T, bool BK, bool LAST, typename S, bool TOGETHER> __global__ __launch_bounds__(S::NT) void orth_product_kernel(OrthArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int rt, ct, mat;
     if (!tile_of_block(blockIdx.x, a.n_row_tiles, a.n_col_tiles, rt, ct, a.batch, mat)) return;
     const int i0 = rt * S::BI, j0 = ct * S::BJ;
     const int64_t b = mat;
     f32x4 acc[S::MI][S::MJ];
-    PairProduct<BK, S> p;
+    PairProduct<BK, S, TOGETHER> p;
     p.A.order = nullptr; p.A.ld = a.lda; p.A.row0 = i0; p.A.rows = a.I - i0; p.A.klen = a.K; p.A.cols = 0; p.A.base = a.ah + b * a.sa;
     p.B.order = nullptr; p.B.ld = a.ldb; p.B.klen = a.K; p.B.base = a.bh + b * a.sb + (BK ? j0 : 0);
     p.B.row0 = BK ? 0 : j0; p.B.rows = BK ? 0 : a.J - j0; p.B.cols = BK ? a.Jp - j0 : 0;
@@ -307,33 +299,36 @@ template <typename T, bool BK, bool LAST, typename S> __global__ __launch_bounds
     } else if (!a.transposed) {
         tile_emit<T, S>(acc, lds, OrthEmit<T>{a, b, i0, j0});
     } else {
-        orth_emit_transposed<T, S>(a, b, i0, j0, acc, lds);
+        orth_emit_transposed<T, S, PairProduct<BK, S, TOGETHER>::LDS>(a, b, i0, j0, acc, lds);
     }
 }
 
+typedef Shape<256, 256, 2, 4, 2, 2> OrthHuge;       // three products in a chain
 typedef Shape<128, 128, 4, 2, 2, 2> OrthBig;
 typedef Shape<64, 64, 2, 2, 2, 2> OrthSmall;
 typedef Shape<32, 32, 2, 1, 2, 3> OrthTiny;
 
-template <typename T, bool BK, bool LAST, typename S> static int launch_orth(OrthArgs& a, int batch, hipStream_t s) {
+template <typename T, bool BK, bool LAST, typename S, bool TOGETHER> static int launch_orth(OrthArgs& a, int batch, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
-    const int lds = PairProduct<BK, S>::LDS;
-    if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(orth_product_kernel<T, BK, LAST, S>), lds, done)) return rc;
+    const int lds = PairProduct<BK, S, TOGETHER>::LDS;
+    if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(orth_product_kernel<T, BK, LAST, S, TOGETHER>), lds, done)) return rc;
     a.n_row_tiles = (a.I + S::BI - 1) / S::BI;
     a.n_col_tiles = (a.Jp + S::BJ - 1) / S::BJ;
     a.batch = batch;
     const int64_t blocks = ((int64_t)a.n_row_tiles * a.n_col_tiles * batch + 7) / 8 * 8;
     FRA_REQUIRE(blocks < 2147483647LL, FRA_ERR_ARG, "fra_orthogonalize: %lld workgroups", (long long)blocks);
-    hipLaunchKernelGGL((orth_product_kernel<T, BK, LAST, S>), dim3((unsigned)blocks), dim3(S::NT), lds, s, a);
+    hipLaunchKernelGGL((orth_product_kernel<T, BK, LAST, S, TOGETHER>), dim3((unsigned)blocks), dim3(S::NT), lds, s, a);
     FRA_HIP(hipGetLastError());
     return FRA_OK;
 }
-// tiles of 128 from three quarters of the chip's units on, of 64 likewise, else 32
+// rounds of one workgroup per compute unit that are at least nine tenths full
+static bool full_rounds(int64_t tiles) { return tiles >= 230 && tiles * 10 >= (tiles + 255) / 256 * 256 * 9; }
 template <typename T, bool BK, bool LAST> static int product(OrthArgs& a, int batch, hipStream_t s) {
-    auto tiles = [&](int64_t side) { return (a.I + side - 1) / side * ((a.Jp + side - 1) / side) * batch; };
-    if (tiles(128) >= 192) return launch_orth<T, BK, LAST, OrthBig>(a, batch, s);
-    if (tiles(64) >= 192) return launch_orth<T, BK, LAST, OrthSmall>(a, batch, s);
-    return launch_orth<T, BK, LAST, OrthTiny>(a, batch, s);
+    auto tiles = [&](int64_t bi, int64_t bj) { return (a.I + bi - 1) / bi * ((a.Jp + bj - 1) / bj) * batch; };
+    if (full_rounds(tiles(256, 256))) return launch_orth<T, BK, LAST, OrthHuge, false>(a, batch, s);
+    if (tiles(128, 128) >= 192) return launch_orth<T, BK, LAST, OrthBig, true>(a, batch, s);
+    if (tiles(64, 64) >= 192) return launch_orth<T, BK, LAST, OrthSmall, true>(a, batch, s);
+    return launch_orth<T, BK, LAST, OrthTiny, true>(a, batch, s);
 }
 
 struct OrthPlan {

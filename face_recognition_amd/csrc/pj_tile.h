@@ -337,16 +337,43 @@ template <typename T, bool AK, bool BK, typename S> struct Frags {
     }
 };
 
+// `steps` steps through LDS, NB deep, the first NB already on their way.  issue(t, dst): sends for step t (NLD loads per wave).  A
+// wave reads the second half of a step while the matrix cores work on the first, and the first half of the next step while they
+// work on the second; between the two lies the one barrier of a step, which says that the next step has arrived for every wave and
+// that every wave has read all of this one, whose buffer the load of step t + NB then takes.  On return every wave is past its last
+// LDS read.
+template <int NB, int NLD, int BUF, typename F, typename Issue, typename Acc>
+__device__ __forceinline__ void run_steps(int steps, char* lds, LdsPtr dst, const Issue& issue, int i0, int j0, int lane, Acc& acc) {
+    F f0, f1;
+    step_arrived<NB - 1, NLD>(steps - 1);
+    f0.read(lds, 0, i0, j0, lane);
+    int cur = 0;
+    for (int t = 0; t < steps; ++t) {
+        f1.read(lds + cur, 1, i0, j0, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        f0.mma(acc);
+        __builtin_amdgcn_sched_barrier(0);
+        const int nxt = cur + BUF == NB * BUF ? 0 : cur + BUF;
+        if (t + 1 < steps) {
+            step_arrived<NB - 2, NLD>(steps - 2 - t);
+            if (t + NB < steps) issue(t + NB, dst + cur);
+            f0.read(lds + nxt, 0, i0, j0, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        f1.mma(acc);
+        __builtin_amdgcn_sched_barrier(0);
+        cur = nxt;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // The product of a tile in two parts, between which a kernel sends for what it needs afterwards:
 //   start   fetches the addresses and (DMA) issues the first NB steps; every wave is past its reads of those buffers;
 //   run     acc[mi][mj][r] = C[i][j] with i = 16 mi + (lane & 15), j = 16 mj + 4 (lane >> 4) + r inside the wave's part: the j side
-//           is the MFMA's row operand, so a lane holds four neighbouring j of one i.  ADD: on top of what acc holds.
+//           is the MFMA's row operand, so a lane holds four neighbouring j of one i.
 //           On return every wave is past its last LDS read.
 // klen: the longer of the operands' (an operand's chunks past its own are zeros).
-// DMA: steps are NB deep in LDS.  A wave reads the second half of a step while the matrix cores work on the first, and the first
-// half of the next step while they work on the second; between the two lies the one barrier of a step, which says that the next
-// step has arrived for every wave and that every wave has read all of this one, whose buffer the load of step t + NB then takes.
-// Otherwise the next step waits in registers.
+// DMA: by run_steps; otherwise the next step waits in registers.
 template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
     typedef OperandA<T, AK, S> OA;
     typedef OperandB<T, BK, S> OB;
@@ -377,43 +404,20 @@ template <typename T, bool AK, bool BK, typename S, bool DMA> struct Product {
                 }
         }
     }
-    template <bool ADD = false> __device__ __forceinline__ void run(char* lds, f32x4 (&acc)[S::MI][S::MJ]) const {
+    __device__ __forceinline__ void run(char* lds, f32x4 (&acc)[S::MI][S::MJ]) const {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         const int i0 = (wave % S::WI) * (S::BI / S::WI), j0 = (wave / S::WI) * (S::BJ / S::WJ);
         const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (!ADD) {
 #pragma unroll
-            for (int mi = 0; mi < S::MI; ++mi)
+        for (int mi = 0; mi < S::MI; ++mi)
 #pragma unroll
-                for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
-        }
+            for (int mj = 0; mj < S::MJ; ++mj) acc[mi][mj] = zero;
         if (steps == 0) return;
         if constexpr (DMA) {
-            const LdsPtr dst = dma_base(lds);
-            Frags<T, AK, BK, S> f0, f1;
-            step_arrived<NB - 1, NLD>(steps - 1);
-            f0.read(lds, 0, i0, j0, lane);
-            int cur = 0;
-            for (int t = 0; t < steps; ++t) {
-                f1.read(lds + cur, 1, i0, j0, lane);
-                __builtin_amdgcn_sched_barrier(0);
-                f0.mma(acc);
-                __builtin_amdgcn_sched_barrier(0);
-                const int nxt = cur + BUF == NB * BUF ? 0 : cur + BUF;
-                if (t + 1 < steps) {
-                    step_arrived<NB - 2, NLD>(steps - 2 - t);
-                    if (t + NB < steps) {
-                        A.issue(sa, t + NB, dst + cur, tid);
-                        B.issue(sb, t + NB, dst + cur + OA::BYTES, tid);
-                    }
-                    f0.read(lds + nxt, 0, i0, j0, lane);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                f1.mma(acc);
-                __builtin_amdgcn_sched_barrier(0);
-                cur = nxt;
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            run_steps<NB, NLD, BUF, Frags<T, AK, BK, S>>(steps, lds, dma_base(lds), [&](int t, LdsPtr to) {
+                A.issue(sa, t, to, tid);
+                B.issue(sb, t, to + OA::BYTES, tid);
+            }, i0, j0, lane, acc);
         } else {
             typename Elem<T>::Frag va[OA::NLD], vb[OB::NLD];
             A.load(sa, va, 0, tid);

@@ -174,3 +174,24 @@ def test_a_training_step_of_grouped_projections(device):
     for got, want in ((y, y64), (dw, dw64), (dh, dh64)):
         assert (got.detach().cpu().double() - want.detach()).norm() <= 8 * 700 * 2.0 ** -24 * want.norm()
     check(step, dw, 5, USUAL)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", [(1, 4090, 4100), (60, 500, 505), (60, 505, 500), (9, 1050, 1010)], ids=str)
+def test_large_batches(device, shape, dt):
+    """Enough tiles for the products' widest kinds (256 x 256, forward and turned, and 128 x 128), none of the sides a multiple of a tile, both ways
+    round.  One step, in 64 bits on the device: the bound of the first step."""
+    g = matrix(shape, dt, device, 3)
+    a, b, c = USUAL
+    y = projection.orthogonalize(g, steps=1)
+    for i in (0, shape[0] - 1):
+        x = g[i].double()
+        x = x / torch.linalg.matrix_norm(x)
+        tall = x.shape[0] > x.shape[1]
+        x = x.mT if tall else x
+        p = x @ x.mT
+        want = a * x + (b * p + c * (p @ p)) @ x
+        want = want.mT if tall else want
+        err = torch.linalg.matrix_norm(y[i].double() - want).item()
+        assert err <= allowed([1.0], want, USUAL, dt)
+        assert (y[i].double() - want).abs().max() <= 2.0 ** -7 * want.abs().max()       # no value out of place
