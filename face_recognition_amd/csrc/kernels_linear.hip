@@ -304,14 +304,25 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
     tile_emit<T, S>(acc, lds, Emit{a, t});
 }
 
-// dW[g] = sum over the group's rows of dz^T x: both operands k-major.  `splits` workgroups share a group's rows and leave fp32
-// partial sums [split][G][N][K], which pj_finish_kernel adds in order; one split writes dW itself.
+// dW[g] = sum over the group's rows of dz^T x: both operands k-major.  Several workgroups share the rows of a tile; what is not
+// the whole sum is left in fp32 and added in order by pj_finish_kernel.  Without groups: `splits` shares of the rows, partial sums
+// [split][N][K].  With groups: pieces of at most so many rows, made from the groups' sizes on the device (a group may hold any
+// part of the batch); a group of one piece, or none, is written at once, the pieces of the others are numbered through.
 struct DwArgs {
     RowArgs rows;
     const void *dz, *x;
-    void* dw;                   // T [G][N][K], or float partial sums if splits > 1
+    void* dw;                   // T [G][N][K]
+    float* part;                // [splits or pieces][N][K]
+    const int4* pieces;         // (group, first list entry, end, number among the partial sums or -1); group -1: unused entry
     int64_t lddz, ldx;
     int K, Kp, N, Np, n_ti, n_tj, splits;
+};
+struct PieceArgs {
+    const int* offsets;
+    int4* pieces;               // [n_pieces]
+    int* slots;                 // [G + 1]: a group's first partial sum
+    int G, rows, n_pieces;      // rows: of a piece, at most
+    unsigned blocks;            // 1, or 0: no groups
 };
 template <typename O> struct DwEmit {
     struct Pre {};
@@ -330,18 +341,19 @@ template <typename O> struct DwEmit {
 };
 template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_dw_kernel(DwArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    // blockIdx.y: group and split
-    const int s = blockIdx.y % a.splits, g = blockIdx.y / a.splits;
     int ti, tj;
     if (!tile_of_block(blockIdx.x, a.n_ti, a.n_tj, ti, tj)) return;
-    int begin = a.rows.offsets ? a.rows.offsets[g] : 0, end = a.rows.offsets ? a.rows.offsets[g + 1] : a.rows.M;
-    if (a.splits > 1) {                                             // whole steps per split
-        const int step = S::KS * Elem<T>::KG;
-        const int steps = (end - begin + step - 1) / step;
-        const int per = (steps + a.splits - 1) / a.splits * step;
-        const int64_t b0 = (int64_t)begin + (int64_t)s * per, e0 = b0 + per;
+    int begin = 0, end = a.rows.M, g = 0, slot = -1;
+    if (a.pieces) {
+        const int4 e = a.pieces[blockIdx.y];
+        if (e.x < 0) return;
+        g = e.x; begin = e.y; end = e.z; slot = e.w;
+    } else if (a.splits > 1) {                                      // whole steps per split
+        const int step = S::KS * Elem<T>::KG, steps = (end + step - 1) / step;
+        const int64_t per = (int64_t)((steps + a.splits - 1) / a.splits) * step, b0 = blockIdx.y * per;
         begin = b0 < end ? (int)b0 : end;
-        end = e0 < end ? (int)e0 : end;
+        end = b0 + per < end ? (int)(b0 + per) : end;
+        slot = blockIdx.y;
     }
     const int n0 = ti * S::BI, k0 = tj * S::BJ;
     typedef Product<T, true, true, S, true> P;
@@ -352,8 +364,8 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
     p.start(end - begin, lds);
     p.run(lds, acc);
     const int64_t plane = (int64_t)a.N * a.K;
-    if (a.splits > 1) {
-        DwEmit<float> f = {(float*)a.dw + ((int64_t)s * a.rows.G + g) * plane, a.N, a.K, n0, k0};
+    if (slot >= 0) {
+        DwEmit<float> f = {a.part + slot * plane, a.N, a.K, n0, k0};
         tile_emit<float, S>(acc, lds, f);
     } else {
         DwEmit<T> f = {(T*)a.dw + (int64_t)g * plane, a.N, a.K, n0, k0};
@@ -480,25 +492,78 @@ template <typename T> __device__ __forceinline__ void pack_rows(const PackArgs& 
 struct PrepArgs {
     DzArgs dz;
     PackArgs x, w;
+    PieceArgs pieces;
     unsigned dz_blocks;
 };
+// exclusive sums over the workgroup's values; returns this thread's, `total` to every thread
+__device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d, 64);
+        if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) tmp[wave] = x;
+    __syncthreads();
+    int base = 0;
+    total = 0;
+    for (int w = 0; w < nw; ++w) {
+        base += w < wave ? tmp[w] : 0;
+        total += tmp[w];
+    }
+    return base + x - v;
+}
+// cuts the groups' rows into pieces (one workgroup)
+__device__ __forceinline__ void cut_pieces(const PieceArgs& a, int* tmp) {
+    int base = 0, sbase = 0;
+    for (int g0 = 0; g0 < a.G; g0 += 256) {
+        const int g = g0 + threadIdx.x;
+        const int first = g < a.G ? a.offsets[g] : 0, end = g < a.G ? a.offsets[g + 1] : 0;
+        const int n = g < a.G ? (end - first > a.rows ? (end - first + a.rows - 1) / a.rows : 1) : 0, multi = n > 1 ? n : 0;
+        int total, stotal;
+        const int at = base + block_scan(n, tmp, total), slot = sbase + block_scan(multi, tmp, stotal);
+        if (g < a.G) a.slots[g] = slot;
+        for (int i = 0; i < n; ++i) {
+            const int b = first + i * a.rows;
+            int4 e = {g, b, end - b > a.rows ? b + a.rows : end, multi ? slot + i : -1};
+            a.pieces[at + i] = e;
+        }
+        base += total;
+        sbase += stotal;
+    }
+    if (threadIdx.x == 0) a.slots[a.G] = sbase;
+    for (int i = base + threadIdx.x; i < a.n_pieces; i += 256) {
+        const int4 none = {-1, 0, 0, -1};
+        a.pieces[i] = none;
+    }
+}
 template <typename T> __global__ __launch_bounds__(256) void pj_prep_kernel(PrepArgs a) {
     __shared__ float sums[256][Elem<T>::EPC + 1];
-    if (blockIdx.x < a.dz_blocks) dz_tile<T>(a.dz, blockIdx.x, sums);
-    else if (blockIdx.x < a.dz_blocks + a.x.blocks) pack_rows<T>(a.x, blockIdx.x - a.dz_blocks);
-    else pack_rows<T>(a.w, blockIdx.x - a.dz_blocks - a.x.blocks);
+    unsigned b = blockIdx.x;
+    if (b < a.pieces.blocks) {
+        cut_pieces(a.pieces, reinterpret_cast<int*>(sums));
+        return;
+    }
+    b -= a.pieces.blocks;
+    if (b < a.dz_blocks) dz_tile<T>(a.dz, b, sums);
+    else if (b < a.dz_blocks + a.x.blocks) pack_rows<T>(a.x, b - a.dz_blocks);
+    else pack_rows<T>(a.w, b - a.dz_blocks - a.x.blocks);
 }
 
 // The sums that the passes before left in parts, in one launch:
-//   workgroups 0 .. n_join:  dw[e] = sum over splits of part[s][e], s ascending;
+//   workgroups 0 .. n_join:  dw[e] = sum over splits of part[s][e], s ascending; with groups dw[g][e] = sum over the group's
+//                            pieces, for groups of more than one (a workgroup belongs to one group, join_each to each);
 //   the others:              out[g][n] = sum of part[t][n] over the group's tiles, for bias and slope: 16 waves take every sixteenth
 //                            tile of 64 columns, their sums are added in order.
 struct FinishArgs {
     const float* dw_part;
     void* dw;
-    int64_t n_dw;
+    int64_t n_dw;               // N K
+    const int* slots;           // nullptr: no groups
     int splits;
-    unsigned n_join;
+    unsigned n_join, join_each;
     const float* part[2];
     void* out[2];
     int out_f32[2];
@@ -508,18 +573,20 @@ struct FinishArgs {
 template <typename T> __global__ __launch_bounds__(1024) void pj_finish_kernel(FinishArgs a) {
     __shared__ float sums[16][64];
     if (blockIdx.x < a.n_join) {
-        const int64_t e = ((int64_t)blockIdx.x * 1024 + threadIdx.x) * 4;
-        if (e >= a.n_dw) return;
+        const unsigned g = blockIdx.x / a.join_each;
+        const int64_t e = ((int64_t)(blockIdx.x - g * a.join_each) * 1024 + threadIdx.x) * 4;
+        const int first = a.slots ? a.slots[g] : 0, end = a.slots ? a.slots[g + 1] : a.splits;
+        if (first == end || e >= a.n_dw) return;
         float v[4] = {0, 0, 0, 0};
         const int left = a.n_dw - e < 4 ? (int)(a.n_dw - e) : 4;
 #pragma unroll 4
-        for (int s = 0; s < a.splits; ++s) {
+        for (int s = first; s < end; ++s) {
             float o[4];
             load_four<float>(a.dw_part + (int64_t)s * a.n_dw + e, left, o);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] += o[i];
         }
-        store_four<T>((T*)a.dw + e, left, v);
+        store_four<T>((T*)a.dw + g * a.n_dw + e, left, v);
         return;
     }
     unsigned b = blockIdx.x - a.n_join;
@@ -588,26 +655,6 @@ __device__ __forceinline__ void group_rank(const GroupArgs& a, int64_t first, in
         if (in && below == 0) cnt[key[i]] = at + __popcll(same);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the next rows' lanes read what this row's leader wrote
     }
-}
-// exclusive sums over the workgroup's values; returns this thread's, `total` to every thread
-__device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) tmp[wave] = x;
-    __syncthreads();
-    int base = 0;
-    total = 0;
-    for (int w = 0; w < nw; ++w) {
-        base += w < wave ? tmp[w] : 0;
-        total += tmp[w];
-    }
-    return base + x - v;
 }
 // totals[key] -> every key's first list entry (in place), tofs[key] its first tile; WRITE: offsets, tile_offsets and the tiles
 template <bool WRITE> __device__ __forceinline__ void group_tables(const GroupArgs& a, int* totals, int* tofs, int* tmp) {
@@ -842,15 +889,23 @@ template <typename T, int MT> static int launch_few_rows(const fra_linear_desc* 
 }
 template <typename T> static int forward_t(const fra_linear_desc* d, void* z, void* y, hipStream_t s) {
     FwdArgs a;
-    // up to 64 rows: the kernel for few rows; then by the number of tiles
-    const bool few = d->groups ? d->groups->tile_rows == 16 : d->M <= 64;
+    // Few rows have a kernel of their own, then it goes by the number of tiles.  fp32: up to 64 rows (K = 512, N = 512: 8.3 us against
+    // 9.6 of tiles; N = 40961: 66 against 76).  16 bits: up to 32 (K = 2048, N = 4096: 8.7 against 10.5; 64 rows 13.0 against 10.7),
+    // or 16 where N alone fills the chip with tiles (K = 512, N = 40961: 1 row 11.8 against 14.2, 32 rows 20.5 against 14.4)
+    const bool few = d->groups ? d->groups->tile_rows == 16 : d->M <= (sizeof(T) == 4 ? 64 : cdiv(d->N, 64) < 256 ? 32 : 16);
     const int bi = few ? (d->groups || d->M <= 16 ? 16 : d->M <= 32 ? 32 : 64)
                        : tile_side(d->M, d->N, sizeof(T) == 4, d->groups ? d->groups->tile_rows : 256);
     a.rows = row_args(d, bi);
     a.x = d->x; a.w = d->w; a.bias = d->bias; a.slope = d->slope; a.resid = d->resid; a.z = z; a.y = y;
     a.ldx = d->ldx; a.ldw = d->ldw; a.wg = d->w_group_stride; a.ldr = d->ldr;
     a.K = d->K; a.N = d->N; a.act = d->act; a.bias_f32 = d->bias_dtype == FRA_F32; a.slope_f32 = d->slope_dtype == FRA_F32;
-    if (few) return bi == 16 ? launch_few_rows<T, 1>(d, a, s) : bi == 32 ? launch_few_rows<T, 2>(d, a, s) : launch_few_rows<T, 4>(d, a, s);
+    if (few) {
+        if (bi == 16) return launch_few_rows<T, 1>(d, a, s);
+        if constexpr (sizeof(T) == 4) {
+            if (bi == 64) return launch_few_rows<T, 4>(d, a, s);
+        }
+        return launch_few_rows<T, 2>(d, a, s);
+    }
     if constexpr (sizeof(T) == 2) {
         if (bi == 256) return launch_forward<T, Huge>(d, a, s);
     }
@@ -860,8 +915,8 @@ template <typename T> static int forward_t(const fra_linear_desc* d, void* z, vo
 // ---- backward: what goes where in the workspace
 struct BackwardPlan {
     bool need_dz, need_sums, pack_x, pack_w;
-    int dz_rows, n_tiles, splits, dw_side, Np, Kp;
-    size_t off_dz, off_x, off_w, off_b, off_s, off_part, bytes;
+    int dz_rows, n_tiles, splits, piece_rows, n_pieces, n_parts, dw_side, Np, Kp;
+    size_t off_dz, off_x, off_w, off_b, off_s, off_part, off_pieces, off_slots, bytes;
 };
 template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc* d, bool dx, bool dw, bool db, bool ds) {
     BackwardPlan p;
@@ -879,21 +934,36 @@ template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc*
     p.pack_w = dx && !dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
     p.dz_rows = g ? g->tile_rows : 64;
     p.n_tiles = g ? g->n_tiles : cdiv(d->M, p.dz_rows);
-    // dW: enough workgroups to fill the chip twice, each with at least 128 rows of its group's average share; tiles of 64 where
-    // tiles of 128 cannot be that many
+    // dW: enough workgroups to fill the chip twice, each with at least 128 rows; tiles of 64 where tiles of 128 cannot be that many.
+    // With groups a piece has at most four times the average group's rows as well, so that a batch whose rows are nearly all of one
+    // group does not leave the chip to that group's tiles.
     const int64_t share = d->M / G / 128 > 1 ? d->M / G / 128 : 1;
     p.dw_side = (int64_t)cdiv(d->N, 128) * cdiv(d->K, 128) * G * share >= 256 ? 128 : 64;
-    const int64_t tiles = (int64_t)cdiv(d->N, p.dw_side) * cdiv(d->K, p.dw_side) * G;
+    const int64_t tiles = (int64_t)cdiv(d->N, p.dw_side) * cdiv(d->K, p.dw_side);
     int64_t sp = (512 + tiles - 1) / tiles;
-    if (sp > share) sp = share;
-    p.splits = dw && sp > 1 ? (int)sp : 1;
+    p.splits = 1;
+    p.piece_rows = p.n_pieces = p.n_parts = 0;
+    if (dw && g) {
+        const int64_t want = sp > (G + 3) / 4 ? sp : (G + 3) / 4;
+        int64_t rows = (d->M + want - 1) / want;
+        rows = rows < 128 ? 128 : (rows + 63) / 64 * 64;
+        p.piece_rows = (int)rows;
+        p.n_pieces = (int)(d->M / rows) + G;
+        p.n_parts = (int)(2 * d->M / rows);     // a group of n > 1 pieces has more than n / 2 pieces' rows
+    } else if (dw) {
+        if (sp > share) sp = share;
+        if (sp > 1) p.splits = (int)sp;
+        if (sp > 1) p.n_parts = (int)sp;
+    }
     size_t at = 0;
     p.off_dz = at; if (p.need_dz) at += up((size_t)d->M * p.Np * es);
     p.off_x = at; if (p.pack_x) at += up((size_t)d->M * p.Kp * es);
     p.off_w = at; if (p.pack_w) at += up((size_t)G * d->N * p.Kp * es);
     p.off_b = at; if (db) at += up((size_t)p.n_tiles * d->N * 4);
     p.off_s = at; if (ds) at += up((size_t)p.n_tiles * d->N * 4);
-    p.off_part = at; if (p.splits > 1) at += up((size_t)p.splits * G * d->N * d->K * 4);
+    p.off_part = at; at += up((size_t)p.n_parts * d->N * d->K * 4);
+    p.off_pieces = at; at += up((size_t)p.n_pieces * 16);
+    p.off_slots = at; if (p.n_pieces) at += up((size_t)(G + 1) * 4);
     p.bytes = at;
     return p;
 }
@@ -951,6 +1021,12 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         k.blocks = pack_blocks(k.rows, k.cpr);
         prep_blocks += k.blocks;
     }
+    if (p.n_pieces) {
+        PieceArgs& k = prep.pieces;
+        k.offsets = g->offsets; k.pieces = (int4*)(ws + p.off_pieces); k.slots = (int*)(ws + p.off_slots);
+        k.G = G; k.rows = p.piece_rows; k.n_pieces = p.n_pieces; k.blocks = 1;
+        prep_blocks += 1;
+    }
     if (prep_blocks > 0) {
         if (int rc = check_grid(prep_blocks, "fra_linear_backward")) return rc;
         hipLaunchKernelGGL((pj_prep_kernel<T>), dim3((unsigned)prep_blocks), dim3(256), 0, s, prep);
@@ -981,22 +1057,27 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
             a.x = ws + p.off_x; a.ldx = p.Kp;
         }
         a.rows = row_args(d, 128);
-        a.dz = dz; a.dw = p.splits > 1 ? (void*)(ws + p.off_part) : dw; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
+        a.dz = dz; a.dw = dw; a.part = (float*)(ws + p.off_part); a.pieces = g ? (const int4*)(ws + p.off_pieces) : nullptr; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
         a.n_ti = cdiv(d->N, p.dw_side); a.n_tj = cdiv(d->K, p.dw_side); a.splits = p.splits;
         const int64_t blocks = ((int64_t)a.n_ti * a.n_tj + 7) / 8 * 8;
-        if (int rc = check_grid(blocks * a.splits * G, "fra_linear_backward")) return rc;
-        const dim3 grid((unsigned)blocks, a.splits * G);
+        const int shares = g ? p.n_pieces : p.splits;
+        FRA_REQUIRE(shares <= 65535, FRA_ERR_ARG, "fra_linear_backward: %d shares", shares);
+        if (int rc = check_grid(blocks * shares, "fra_linear_backward")) return rc;
+        const dim3 grid((unsigned)blocks, shares);
         if (p.dw_side == 128) PJ_LAUNCH((pj_dw_kernel<T, Big>), grid, Big::NT, Big::LDS, s, a);
         else PJ_LAUNCH((pj_dw_kernel<T, Small>), grid, Small::NT, Small::LDS, s, a);
     }
-    if (p.need_sums || p.splits > 1) {
+    if (p.need_sums || p.n_parts) {
         FinishArgs a = {};
         int64_t blocks = 0;
-        if (p.splits > 1) {
+        if (p.n_parts) {
             a.dw_part = (const float*)(ws + p.off_part); a.dw = dw; a.splits = p.splits;
-            a.n_dw = (int64_t)G * d->N * d->K;
-            blocks = (a.n_dw + 4095) / 4096;
+            a.slots = g ? (const int*)(ws + p.off_slots) : nullptr;
+            a.n_dw = (int64_t)d->N * d->K;
+            const int64_t each = (a.n_dw + 4095) / 4096;
+            blocks = each * G;
             if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
+            a.join_each = (unsigned)each;
             a.n_join = (unsigned)blocks;
         }
         if (p.need_sums) {

@@ -163,6 +163,17 @@ def test_grouped_linear_and_gradients(device, m, k, n, groups, act, dt):
     check(run(t, act, rg), reference(t, act, torch.where((ids >= 0) & (ids < groups), ids, torch.full_like(ids, -1))))
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shares", [(0, 5000, 0, 300, 129, 128, 1, 2000), (3000,), (0, 0, 6000), (257, 255, 256, 1024, 1)], ids=str)
+def test_groups_of_very_different_sizes(device, shares, dt):
+    """A group's rows come in pieces whose sums are joined; groups of one piece or none are written at once."""
+    k, n, groups = 72, 40, len(shares)
+    ids = torch.repeat_interleave(torch.arange(groups), torch.tensor(shares))
+    ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(1))]
+    t = make(len(ids), k, n, dt, device, 17, lead=(groups,), act="silu")
+    check(run(t, "silu", projection.group_rows(ids.to(device), groups)), reference(t, "silu", ids))
+
+
 @pytest.mark.parametrize("kind", ["all_one", "none", "last_only"])
 def test_grouped_extremes(device, kind):
     m, k, n, groups = 333, 48, 56, 6
