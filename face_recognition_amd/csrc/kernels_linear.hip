@@ -614,11 +614,12 @@ template <typename T> __global__ __launch_bounds__(1024) void pj_finish_kernel(F
     }
 }
 // ---- rows by group: a stable counting sort --------------------------------------------------------------------------
-// key = id, or G where id is outside [0, G).  A workgroup of NW waves owns NW * 512 consecutive rows, a wave 512 of them, kept
-// as eight keys per lane.  Lanes with the same key find each other by ballots over the key's bits, so a row's rank among its
+// key = id, or G where id is outside [0, G).  A workgroup of NW waves owns NW * 64 KEYS consecutive rows, a wave 64 KEYS of them,
+// kept as KEYS keys per lane: four, or eight where that makes it one workgroup (and one launch: 8192 rows 12.6 us against 8.3 + 4.8;
+// 30001 rows take 8.7 + 5.0 us with four and 12.3 + 7.6 with eight).  Lanes with the same key find each other by ballots over the key's bits, so a row's rank among its
 // wave's rows of the key is the wave's running count plus the equal lanes below: no atomics, and the order does not depend on
 // timing.  One launch for one workgroup; else the counts of all workgroups first.
-constexpr int GR_MAX_GROUPS = 4096, GR_KEYS = 8, GR_WAVE_ROWS = 64 * GR_KEYS;
+constexpr int GR_MAX_GROUPS = 4096;
 constexpr int GR_WIDE_KEYS = 1025;          // up to this many keys sixteen waves' counters fit in LDS, beyond it four waves'
 constexpr int GR_INLINE_SCAN = 8192;        // counters up to which every workgroup adds the others' counts itself
 struct GroupArgs {
@@ -629,9 +630,9 @@ struct GroupArgs {
     int4* tiles;
 };
 // ranks the wave's rows among its rows of the same key; cnt[key] ends as the count
-__device__ __forceinline__ void group_rank(const GroupArgs& a, int64_t first, int* cnt, int lane, int (&key)[GR_KEYS], int (&rank)[GR_KEYS]) {
+template <int KEYS> __device__ __forceinline__ void group_rank(const GroupArgs& a, int64_t first, int* cnt, int lane, int (&key)[KEYS], int (&rank)[KEYS]) {
 #pragma unroll
-    for (int i = 0; i < GR_KEYS; ++i) {
+    for (int i = 0; i < KEYS; ++i) {
         const int64_t row = first + 64 * i + lane;
         key[i] = -1;
         if (row < a.M) {
@@ -640,7 +641,7 @@ __device__ __forceinline__ void group_rank(const GroupArgs& a, int64_t first, in
         }
     }
 #pragma unroll
-    for (int i = 0; i < GR_KEYS; ++i) {
+    for (int i = 0; i < KEYS; ++i) {
         const bool in = key[i] >= 0;
         unsigned long long same = __ballot(in);
         if (!same) break;
@@ -699,12 +700,12 @@ template <bool WRITE> __device__ __forceinline__ void group_tables(const GroupAr
     }
 }
 // COUNT: a workgroup's counts; else place (the only workgroup, or after the counts, or after pj_group_scan_kernel)
-template <int NW, bool COUNT> __global__ __launch_bounds__(64 * NW) void pj_group_kernel(GroupArgs a) {
+template <int NW, int KEYS, bool COUNT> __global__ __launch_bounds__(64 * NW) void pj_group_kernel(GroupArgs a) {
     extern __shared__ int cnt[];                                    // [NW][keys]; place: + totals[keys], before[keys] (= tofs), not scanned: + counts[nb][keys]
     __shared__ int tmp[NW];
     const int keys = a.G + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = 64 * NW;
-    int key[GR_KEYS], rank[GR_KEYS];
-    const int64_t first = ((int64_t)blockIdx.x * NW + wave) * GR_WAVE_ROWS;
+    int key[KEYS], rank[KEYS];
+    const int64_t first = ((int64_t)blockIdx.x * NW + wave) * (64 * KEYS);
     for (int i = threadIdx.x; i < NW * keys; i += nt) cnt[i] = 0;
     __syncthreads();
     group_rank(a, first, cnt + wave * keys, lane, key, rank);
@@ -760,7 +761,7 @@ template <int NW, bool COUNT> __global__ __launch_bounds__(64 * NW) void pj_grou
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < GR_KEYS; ++i)
+    for (int i = 0; i < KEYS; ++i)
         if (key[i] >= 0) a.order[cnt[wave * keys + key[i]] + rank[i]] = (int)(first + 64 * i + lane);
 }
 // counts[b][key] -> exclusive sums over b; totals -> tables
@@ -1096,26 +1097,32 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
 }
 
 static bool group_wide(int n_groups) { return n_groups + 1 <= GR_WIDE_KEYS; }
+static int group_keys(int64_t M, int n_groups) {
+    const int waves = group_wide(n_groups) ? 16 : 4;
+    return M > waves * 256 && M <= waves * 512 ? 8 : 4;
+}
 static int group_blocks(int64_t M, int n_groups) {
-    const int per = (group_wide(n_groups) ? 16 : 4) * GR_WAVE_ROWS;
+    const int per = (group_wide(n_groups) ? 16 : 4) * 64 * group_keys(M, n_groups);
     return M > per ? cdiv(M, per) : 1;
 }
-template <int NW> static int launch_groups(GroupArgs& a, hipStream_t s) {
+template <int NW, int KEYS> static int launch_groups(GroupArgs& a, hipStream_t s) {
     const int keys = a.G + 1, most = (NW == 16 ? GR_WIDE_KEYS : GR_MAX_GROUPS + 1) * 4, lds = (NW + 2) * keys * 4;
     static std::atomic<uint64_t> done_count{0}, done_place{0};
-    if (int rc = raise_lds(pj_group_kernel<NW, false>, (NW + 2) * most + GR_INLINE_SCAN * 4, done_place)) return rc;
-    if (a.nb > 1) {
-        if (int rc = raise_lds(pj_group_kernel<NW, true>, NW * most, done_count)) return rc;
-        hipLaunchKernelGGL((pj_group_kernel<NW, true>), dim3(a.nb), dim3(64 * NW), NW * keys * 4, s, a);
-        FRA_HIP(hipGetLastError());
-        a.scanned = (int64_t)a.nb * keys > GR_INLINE_SCAN;
-        if (a.scanned) {
-            hipLaunchKernelGGL(pj_group_scan_kernel, dim3(1), dim3(1024), 2 * keys * 4, s, a);
+    if (int rc = raise_lds(pj_group_kernel<NW, KEYS, false>, (NW + 2) * most + GR_INLINE_SCAN * 4, done_place)) return rc;
+    if constexpr (KEYS == 4) {
+        if (a.nb > 1) {
+            if (int rc = raise_lds(pj_group_kernel<NW, KEYS, true>, NW * most, done_count)) return rc;
+            hipLaunchKernelGGL((pj_group_kernel<NW, KEYS, true>), dim3(a.nb), dim3(64 * NW), NW * keys * 4, s, a);
             FRA_HIP(hipGetLastError());
+            a.scanned = (int64_t)a.nb * keys > GR_INLINE_SCAN;
+            if (a.scanned) {
+                hipLaunchKernelGGL(pj_group_scan_kernel, dim3(1), dim3(1024), 2 * keys * 4, s, a);
+                FRA_HIP(hipGetLastError());
+            }
         }
     }
     const int counts = a.nb > 1 && !a.scanned ? a.nb * keys * 4 : 0;
-    hipLaunchKernelGGL((pj_group_kernel<NW, false>), dim3(a.nb), dim3(64 * NW), lds + counts, s, a);
+    hipLaunchKernelGGL((pj_group_kernel<NW, KEYS, false>), dim3(a.nb), dim3(64 * NW), lds + counts, s, a);
     FRA_HIP(hipGetLastError());
     return FRA_OK;
 }
@@ -1196,7 +1203,9 @@ int fra_group_rows(const void* ids, int ids_are_64bit, const fra_row_groups* g, 
     a.scanned = 0;
     a.bits = 0;
     while ((1 << a.bits) < a.G + 1) ++a.bits;
-    return group_wide(a.G) ? launch_groups<16>(a, (hipStream_t)stream) : launch_groups<4>(a, (hipStream_t)stream);
+    hipStream_t s = (hipStream_t)stream;
+    if (group_keys(a.M, a.G) == 8) return group_wide(a.G) ? launch_groups<16, 8>(a, s) : launch_groups<4, 8>(a, s);
+    return group_wide(a.G) ? launch_groups<16, 4>(a, s) : launch_groups<4, 4>(a, s);
 }
 
 }  // extern "C"

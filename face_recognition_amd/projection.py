@@ -247,7 +247,9 @@ def _check(what, x, weight, bias, activation, slope, residual, lead):
 
 
 def _apply(x, weight, bias, slope, residual, act, groups):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, slope, residual)):
+    if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+            or (slope is not None and slope.requires_grad) or (residual is not None and residual.requires_grad)) \
+            and torch.is_grad_enabled():
         return _Linear.apply(x, weight, bias, slope, residual, act, groups)
     return _forward(x, weight, bias, slope, residual, act, groups, False)[0]
 

@@ -188,7 +188,7 @@ def test_grouped_extremes(device, kind):
         assert torch.equal(out["y"].detach(), t["r"]) and not out["dx"].any()
 
 
-@pytest.mark.parametrize("m", [0, 1, 63, 64, 65, 1000, 4095, 4096, 4097, 20000, 300001])
+@pytest.mark.parametrize("m", [0, 1, 63, 64, 65, 1000, 1025, 4095, 4096, 4097, 8192, 8193, 20000, 300001])
 @pytest.mark.parametrize("groups", [1, 2, 37, 4096])
 @pytest.mark.parametrize("it", [torch.int32, torch.int64], ids=str)
 def test_group_rows_is_a_stable_sort(device, m, groups, it):
