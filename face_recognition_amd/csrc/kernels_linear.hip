@@ -166,6 +166,13 @@ __device__ __forceinline__ bool next_tile(const RowArgs& a, unsigned b, int n_co
     return true;
 }
 
+// z = x W^T + b, y = act(z) + r.  One tile per workgroup.  Bound, by size: large K by the matrix cores (8192^3 in bf16 826 us, 1.33
+// PFLOP/s; the library's plain product 1.45); K = 512 by what surrounds a tile's eight steps -- of the 12.7 us of a 128 x 128 tile
+// two such workgroups on a compute unit spend 7.4 in the steps, 2.8 before the first one's data are there and 2.5 on the results
+// (4.2 with a residual and a sigmoid), and neither walking over tiles with the next one's data ahead (the registers do not hold it)
+// nor a deeper pipeline shortened that.  262144 x 512 x 512 f16 with silu and residual 241 us (3.3 TB/s of its 806 MB), 1024 x 40961
+// x 512 bf16 70 us (613 TFLOP/s), 4096 x 2048 x 1024 bf16 with gelu 23.8 us (721 TFLOP/s), 30001 x 768 x 512 in 37 groups 44 us,
+// fp32 4096^3 1.07 ms (128 TFLOP/s of the library's 141).
 template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_forward_kernel(FwdArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef Product<T, false, false, S, DMA> P;
@@ -202,7 +209,8 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT, 
 }
 
 // The same for few rows (tiles of 16 MT): a workgroup takes 16 columns, its eight waves every eighth group of k (K = 512 is one
-// trip to memory), and their sums meet in LDS, added in a fixed order.  Bound by the latency of one trip to memory, or by W's bytes: a column's weights are read once,
+// trip to memory), and their sums meet in LDS, added in a fixed order.  Bound by the latency of one trip to memory (1 x 512 x 512
+// f16: 3.1 us in a graph, of tiles 4.7), or by W's bytes (1 x 40961 x 512: 11.8 us, 3.6 TB/s): a column's weights are read once,
 // straight into MFMA operands, in pieces of 64 bytes of sixteen rows whose neighbours the other waves take.
 template <typename T, int MT> __global__ __launch_bounds__(512) void pj_few_rows_kernel(FwdArgs a) {
     typedef typename Elem<T>::Frag Frag;
@@ -267,7 +275,8 @@ template <typename T, int MT> __global__ __launch_bounds__(512) void pj_few_rows
 
 // ---- backward: everything the products read lies in rows of whole aligned chunks, in list order
 
-// dx = dz W, scattered back to the rows
+// dx = dz W, scattered back to the rows.  W is read as it lies (its rows are the contraction): the fragments come out of LDS through
+// the transposing read.  4096 x 1024 x 2048 bf16 26 us (660 TFLOP/s; the library's plain product 28.6).
 struct DxArgs {
     RowArgs rows;
     const void *dz, *w;
@@ -308,6 +317,8 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
 // the whole sum is left in fp32 and added in order by pj_finish_kernel.  Without groups: `splits` shares of the rows, partial sums
 // [split][N][K].  With groups: pieces of at most so many rows, made from the groups' sizes on the device (a group may hold any
 // part of the batch); a group of one piece, or none, is written at once, the pieces of the others are numbered through.
+// 2048 x 1024 x 4096 bf16 25 us with 5 for the joining (the library's plain product 39); 16 groups of 8192 rows, 1024 x 512 each,
+// 24 us (37 with whole groups: the largest one's tiles ran alone).
 struct DwArgs {
     RowArgs rows;
     const void *dz, *x;
@@ -374,7 +385,9 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
 }
 // dz = dy act'(z) in list order and, per row tile, the column sums of dz and of dy min(z, 0).  A workgroup takes one row tile x
 // `lpr` 16-byte pieces of columns (lpr lanes side by side, a power of two up to 16, so that narrow pieces make many workgroups;
-// 256 / lpr rows at a time); four rows per lane are requested together.  Bound by HBM: dy and z in, dz out.
+// 256 / lpr rows at a time); four rows per lane are requested together.  Bound by HBM and, with a sigmoid, by the vector ALU
+// nearly as much: 4096 x 2048 bf16 with gelu 11 us, 4.6 TB/s of dy and z in and dz out (27 us with a workgroup per 256 columns and
+// a guard around every access).
 struct DzArgs {
     RowArgs rows;
     const void *dy, *z, *slope;
@@ -557,6 +570,7 @@ template <typename T> __global__ __launch_bounds__(256) void pj_prep_kernel(Prep
 //                            pieces, for groups of more than one (a workgroup belongs to one group, join_each to each);
 //   the others:              out[g][n] = sum of part[t][n] over the group's tiles, for bias and slope: 16 waves take every sixteenth
 //                            tile of 64 columns, their sums are added in order.
+// 4 us where only the latter is to do, 7 us with four partial sums of 2048 x 1024.
 struct FinishArgs {
     const float* dw_part;
     void* dw;
@@ -616,9 +630,10 @@ template <typename T> __global__ __launch_bounds__(1024) void pj_finish_kernel(F
 // ---- rows by group: a stable counting sort --------------------------------------------------------------------------
 // key = id, or G where id is outside [0, G).  A workgroup of NW waves owns NW * 64 KEYS consecutive rows, a wave 64 KEYS of them,
 // kept as KEYS keys per lane: four, or eight where that makes it one workgroup (and one launch: 8192 rows 12.6 us against 8.3 + 4.8;
-// 30001 rows take 8.7 + 5.0 us with four and 12.3 + 7.6 with eight).  Lanes with the same key find each other by ballots over the key's bits, so a row's rank among its
-// wave's rows of the key is the wave's running count plus the equal lanes below: no atomics, and the order does not depend on
-// timing.  One launch for one workgroup; else the counts of all workgroups first.
+// 30001 rows take 8.7 + 5.0 us with four and 12.3 + 7.6 with eight).  Lanes with the same key find each other by ballots over the
+// key's bits, so a row's rank among its wave's rows of the key is the wave's running count plus the equal lanes below: no atomics,
+// and the order does not depend on timing.  One launch for one workgroup; else the counts of all workgroups first.  Bound by
+// latency: a dozen rows take 4 us, of which a launch is two.
 constexpr int GR_MAX_GROUPS = 4096;
 constexpr int GR_WIDE_KEYS = 1025;          // up to this many keys sixteen waves' counters fit in LDS, beyond it four waves'
 constexpr int GR_INLINE_SCAN = 8192;        // counters up to which every workgroup adds the others' counts itself

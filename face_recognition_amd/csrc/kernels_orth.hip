@@ -6,7 +6,13 @@
 // rounding error with them, so sixteen bits are too few between the products.  Every value is held as TWO f16, hi + lo, of
 // 2^8 times itself: 22 significant bits down to 2^-10, an absolute step of 2^-32 below, range +-255.  A product is
 // hi hi + hi lo + lo hi on the f16 matrix cores (lo lo is below 2^-22), accumulated in fp32: a third of their rate, which is
-// over three times that of the fp32 matrix instructions.
+// over three times that of the fp32 matrix instructions.  Against 64 bits the results are as near as the same iteration with
+// fp32 products (512 x 512: 1.4e-6 of the norm, fp32 2.1e-6).
+//
+// 17 launches for five steps.  Small matrices are bound by the launches' latency (512 x 512 fp32 107 us, 6.1 us each), large ones by
+// the matrix cores: eight of 2048 x 1024 1.27 ms (1.0 PFLOP/s of f16 products), one of 4096 x 4096 4.9 ms (1.25).  P and Q are
+// symmetric, which is not used: with tiles of 128 the lower half of 1024 x 1024 is 36 of 64 tiles, for a batch of eight 288 on 256
+// compute units, two rounds like all 512.
 #include "pj_tile.h"
 
 namespace fra {
