@@ -171,12 +171,11 @@ def _backward(ctx, dy):
             db = x.new_empty(weight.shape[:-1], dtype=ctx.bias_dtype)
         if need[3]:
             ds = x.new_empty(weight.shape[:-1], dtype=slope.dtype)
-        if x.data_ptr() != d.x or weight.data_ptr() != d.w or (slope is not None and slope.data_ptr() != d.slope):
-            # what was saved came back as other tensors (saved-tensor hooks)
-            x, d.ldx = _rows(x)
-            weight, d.ldw, d.w_group_stride = _weight(weight)
-            slope = slope.contiguous() if slope is not None else None
-            d.x, d.w, d.slope = x.data_ptr(), weight.data_ptr(), slope.data_ptr() if slope is not None else None
+        # saved-tensor hooks may bring back other tensors, or the same memory laid out otherwise
+        x, d.ldx = _rows(x)
+        weight, d.ldw, d.w_group_stride = _weight(weight)
+        slope = slope.contiguous() if slope is not None else None
+        d.x, d.w, d.slope = x.data_ptr(), weight.data_ptr(), slope.data_ptr() if slope is not None else None
         if z is not None:
             z = z.contiguous()
         lib = _lib.load()

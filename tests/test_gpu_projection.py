@@ -387,6 +387,25 @@ def test_once_differentiable_and_saved_tensor_hooks(device):
         torch.autograd.grad(y, w, t["dy"])
 
 
+def test_saved_tensors_back_at_their_address_in_another_layout(device):
+    # an allocator may hand the address of a freed view out again, to the packed copy that a hook brings back
+    m, k, n = 48, 40, 56
+    t = make(m, k, n, torch.float16, device, 56, bias=False, residual=False)
+    memory = torch.zeros(m, 2 * k, dtype=torch.float16, device=device)
+    x = memory[:, :k].copy_(t["x"])
+    want = run(t, None)["dw"]
+
+    def unpack(v):
+        if v.shape != (m, k):
+            return v.to(device)
+        return memory.view(-1)[:m * k].view(m, k).copy_(v)
+
+    w = t["w"].clone().requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), unpack):
+        y = projection.linear(x, w)
+    assert torch.equal(torch.autograd.grad(y, w, t["dy"])[0], want)
+
+
 def test_captured_and_replayed(device):
     m, k, n, groups = 500, 136, 72, 5
     t = make(m, k, n, torch.bfloat16, device, 61, lead=(groups,), act="prelu")
