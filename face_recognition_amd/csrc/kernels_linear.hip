@@ -38,13 +38,15 @@ template <typename T> __device__ __forceinline__ float pj_act_grad(int act, floa
     switch (act) {
         case PJ_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case PJ_PRELU: return z > 0.0f ? 1.0f : s;
+        // beyond +-200 the sigmoid q is 0 or 1 exactly and the derivative with it; the other factors are held back there, so that
+        // they meet the zero (of q or 1 - q) finite.  A NaN comes through q.
         case PJ_SILU: {
-            const float q = pj_sigmoid2<T>(LOG2E * z);
-            return q * (1.0f + z * (1.0f - q));
+            const float q = pj_sigmoid2<T>(LOG2E * z), c = __builtin_amdgcn_fmed3f(z, -200.0f, 200.0f);
+            return q * (1.0f + c * (1.0f - q));
         }
         case PJ_GELU_TANH: {
-            const float q = pj_sigmoid2<T>(z * (LOG2E * GELU_C + LOG2E * GELU_C * GELU_A * (z * z)));
-            return q * (1.0f + z * (1.0f - q) * (GELU_C + 3.0f * GELU_A * GELU_C * (z * z)));
+            const float q = pj_sigmoid2<T>(z * (LOG2E * GELU_C + LOG2E * GELU_C * GELU_A * (z * z))), c = __builtin_amdgcn_fmed3f(z, -200.0f, 200.0f);
+            return q * (1.0f + c * (1.0f - q) * (GELU_C + 3.0f * GELU_A * GELU_C * (c * c)));
         }
         default: return 1.0f;
     }

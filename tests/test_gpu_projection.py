@@ -366,6 +366,21 @@ def test_parameters_in_fp32_and_partial_gradients(device):
         assert not call(t, "prelu").requires_grad
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_far_outside_the_activation_bends(device, act, dt):
+    # one product per value: z = 300 x is far below or above, in f16 past the type's range (where what is kept of z is an infinity)
+    far = torch.tensor([1e3, 60000.0] if dt == torch.float16 else [1e3, 1e17, 1e25], dtype=dt)
+    x = torch.cat([-far, far, torch.tensor([float("nan")], dtype=dt)])[:, None].to(device).requires_grad_(True)
+    w = torch.full((1, 1), 300.0, dtype=dt, device=device)
+    y = projection.linear(x, w, activation=act)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    k = len(far)
+    assert torch.equal(y[:k], torch.zeros_like(y[:k])) and torch.equal(dx[:k], torch.zeros_like(y[:k]))
+    assert torch.equal(y[k:2 * k], (300.0 * x[k:2 * k].float()).to(dt)) and torch.equal(dx[k:2 * k], torch.full_like(y[:k], 300.0))
+    assert y[2 * k].isnan() and dx[2 * k].isnan()
+
+
 def test_once_differentiable_and_saved_tensor_hooks(device):
     t = make(50, 24, 40, torch.float32, device, 55, act="prelu")
     full = run(t, "prelu")
