@@ -853,6 +853,7 @@ static int check_desc(const fra_linear_desc* d, const char* what) {
         FRA_REQUIRE(g->tile_rows == fra_group_tile_rows(g->rows, g->n_groups) && g->n_tiles == fra_group_tiles(g->rows, g->n_groups),
                     FRA_ERR_ARG, "%s: a tile table of %d entries of %d rows is not fra_group_rows' own", what, g->n_tiles, g->tile_rows);
         FRA_REQUIRE(g->offsets && g->tiles && g->tile_offsets && (g->order || d->M == 0), FRA_ERR_ARG, "%s: null pointer in the groups", what);
+        FRA_REQUIRE(((uintptr_t)g->tiles & 15) == 0, FRA_ERR_ARG, "%s: the groups' tiles are not 16-byte aligned", what);
         FRA_REQUIRE(d->w_group_stride >= 0, FRA_ERR_ARG, "%s: group stride %lld", what, (long long)d->w_group_stride);
     }
     return FRA_OK;
@@ -1178,6 +1179,7 @@ int fra_linear_backward(const fra_linear_desc* d, const void* preact, const void
     const BackwardPlan p = backward_plan(d, dx, dw, dbias, dslope);
     FRA_REQUIRE(workspace_bytes >= p.bytes && (workspace || p.bytes == 0), FRA_ERR_WORKSPACE,
                 "fra_linear_backward: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
+    FRA_REQUIRE(((uintptr_t)workspace & 15) == 0, FRA_ERR_ARG, "fra_linear_backward: workspace not 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;
     if (d->dtype == FRA_F32) return backward_t<float>(d, p, preact, dy, lddy, dx, dw, dbias, dslope, ws, s);
@@ -1208,6 +1210,7 @@ int fra_group_rows(const void* ids, int ids_are_64bit, const fra_row_groups* g, 
     if (int rc = fra_group_rows_workspace_bytes(g->rows, g->n_groups, &need)) return rc;
     FRA_REQUIRE((ids && g->order) || g->rows == 0, FRA_ERR_ARG, "fra_group_rows: null pointer");
     FRA_REQUIRE(g->offsets && g->tiles && g->tile_offsets, FRA_ERR_ARG, "fra_group_rows: null pointer");
+    FRA_REQUIRE(((uintptr_t)g->tiles & 15) == 0 && ((uintptr_t)workspace & 15) == 0, FRA_ERR_ARG, "fra_group_rows: tiles or workspace not 16-byte aligned");
     FRA_REQUIRE(g->tile_rows == fra_group_tile_rows(g->rows, g->n_groups) && g->n_tiles == fra_group_tiles(g->rows, g->n_groups), FRA_ERR_ARG,
                 "fra_group_rows: tile_rows / n_tiles are not those of fra_group_tile_rows / fra_group_tiles");
     FRA_REQUIRE(workspace_bytes >= need && (workspace || need == 0), FRA_ERR_WORKSPACE, "fra_group_rows: workspace of %zu bytes, %zu needed",

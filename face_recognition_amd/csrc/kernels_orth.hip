@@ -439,6 +439,7 @@ int fra_orthogonalize(int dtype, const void* g, int64_t ldg, int64_t batch_strid
     FRA_REQUIRE(g && out, FRA_ERR_ARG, "fra_orthogonalize: null pointer");
     const OrthPlan p = orth_plan(batch, rows, cols);
     FRA_REQUIRE(workspace && workspace_bytes >= p.bytes, FRA_ERR_WORKSPACE, "fra_orthogonalize: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
+    FRA_REQUIRE(((uintptr_t)workspace & 15) == 0, FRA_ERR_ARG, "fra_orthogonalize: workspace not 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     char* ws = (char*)workspace;
     if (dtype == FRA_F32) return orth_t<float>(p, (const float*)g, ldg, batch_stride, steps, a, b, c, (float*)out, ws, s);

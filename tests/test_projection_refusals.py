@@ -115,3 +115,15 @@ def test_orthogonalize_refusals():
     assert call(nbytes=n.value - 1) == 5 and call(ws=None) == 5
     assert call(batch=0, g=None, out=None, ws=None, nbytes=0) == 0
     assert lib.fra_orthogonalize_workspace_bytes(1, 0, 8, C.byref(n)) == 1 and lib.fra_orthogonalize_workspace_bytes(1, 4, 8, None) == 1
+
+
+def test_scratch_and_tables_have_to_be_aligned():
+    lib = _lib.load()
+    n = C.c_size_t()
+    d = desc(act=1)
+    assert lib.fra_linear_backward_workspace_bytes(C.byref(d), 1, 1, 0, 0, C.byref(n)) == 0
+    assert lib.fra_linear_backward(C.byref(d), 64, 64, 5, 64, 64, None, None, 72, n.value, None) == 1 and b"aligned" in lib.fra_last_error()
+    g = _lib.RowGroupsDesc(8, 4, lib.fra_group_tile_rows(8, 4), lib.fra_group_tiles(8, 4), 64, 64, 68, 64)
+    assert lib.fra_group_rows(64, 0, C.byref(g), None, 0, None) == 1 and b"aligned" in lib.fra_last_error()
+    assert lib.fra_linear(C.byref(desc(M=8, groups=C.pointer(g))), None, 64, None) == 1 and b"aligned" in lib.fra_last_error()
+    assert lib.fra_orthogonalize(_lib.FRA_F32, 64, 8, 0, 1, 4, 8, 5, 1.5, -0.5, 0.0, 64, 68, 1 << 40, None) == 1 and b"aligned" in lib.fra_last_error()
