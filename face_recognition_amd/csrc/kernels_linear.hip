@@ -871,8 +871,9 @@ static RowArgs row_args(const fra_linear_desc* d, int tile_rows) {
     r.G = g ? g->n_groups : 1;
     return r;
 }
-static int check_grid(int64_t blocks, const char* what) {
-    FRA_REQUIRE(blocks < 2147483647LL, FRA_ERR_ARG, "%s: %lld workgroups", what, (long long)blocks);
+// a launch's threads are counted in 32 bits
+static int check_grid(int64_t blocks, int threads, const char* what) {
+    FRA_REQUIRE(blocks <= 4294967295LL / threads, FRA_ERR_ARG, "%s: %lld workgroups of %d are more than one launch", what, (long long)blocks, threads);
     return FRA_OK;
 }
 // The side of a product's tiles.  256 x 256 moves half the bytes per product of 128 x 128 through the caches (8192 x 8192 x 8192:
@@ -891,7 +892,7 @@ static int tile_side(int64_t rows, int64_t cols, bool f32, int most = 256) {
 template <typename T, typename S> static int launch_forward(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
     a.n_col_tiles = cdiv(d->N, S::BJ);
     const int64_t blocks = ((int64_t)a.rows.n_tiles * a.n_col_tiles + 7) / 8 * 8;
-    if (int rc = check_grid(blocks, "fra_linear")) return rc;
+    if (int rc = check_grid(blocks, S::NT, "fra_linear")) return rc;
     if (dma_ok<T>(d->x, d->ldx, d->K) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K))
         PJ_LAUNCH((pj_forward_kernel<T, S, true>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
     else
@@ -901,7 +902,7 @@ template <typename T, typename S> static int launch_forward(const fra_linear_des
 template <typename T, int MT> static int launch_few_rows(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
     a.n_col_tiles = cdiv(d->N, 16);
     const int64_t blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
-    if (int rc = check_grid(blocks, "fra_linear")) return rc;
+    if (int rc = check_grid(blocks, 512, "fra_linear")) return rc;
     hipLaunchKernelGGL((pj_few_rows_kernel<T, MT>), dim3((unsigned)blocks), dim3(512), 0, s, a);
     FRA_HIP(hipGetLastError());
     return FRA_OK;
@@ -993,7 +994,7 @@ static BackwardPlan backward_plan(const fra_linear_desc* d, bool dx, bool dw, bo
 template <typename T, typename S> static int launch_dx(DxArgs& a, hipStream_t s) {
     a.n_col_tiles = cdiv(a.K, S::BJ);
     const int64_t blocks = ((int64_t)a.rows.n_tiles * a.n_col_tiles + 7) / 8 * 8;
-    if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
+    if (int rc = check_grid(blocks, S::NT, "fra_linear_backward")) return rc;
     PJ_LAUNCH((pj_dx_kernel<T, S>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
     return FRA_OK;
 }
@@ -1021,7 +1022,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         while (a.lpr_log2 < 4 && (1 << a.lpr_log2) < pieces) ++a.lpr_log2;
         a.n_col_tiles = cdiv(pieces, 1 << a.lpr_log2);
         prep_blocks = (int64_t)a.rows.n_tiles * a.n_col_tiles;
-        if (int rc = check_grid(prep_blocks, "fra_linear_backward")) return rc;
+        if (int rc = check_grid(prep_blocks, 256, "fra_linear_backward")) return rc;
         prep.dz_blocks = (unsigned)prep_blocks;
     }
     auto pack_blocks = [](int64_t rows, int cpr) { const int64_t b = (rows * cpr + 255) / 256; return (unsigned)(b < 2048 ? b : 2048); };
@@ -1047,7 +1048,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         prep_blocks += 1;
     }
     if (prep_blocks > 0) {
-        if (int rc = check_grid(prep_blocks, "fra_linear_backward")) return rc;
+        if (int rc = check_grid(prep_blocks, 256, "fra_linear_backward")) return rc;
         hipLaunchKernelGGL((pj_prep_kernel<T>), dim3((unsigned)prep_blocks), dim3(256), 0, s, prep);
         FRA_HIP(hipGetLastError());
     }
@@ -1081,7 +1082,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
         const int64_t blocks = ((int64_t)a.n_ti * a.n_tj + 7) / 8 * 8;
         const int shares = g ? p.n_pieces : p.splits;
         FRA_REQUIRE(shares <= 65535, FRA_ERR_ARG, "fra_linear_backward: %d shares", shares);
-        if (int rc = check_grid(blocks * shares, "fra_linear_backward")) return rc;
+        if (int rc = check_grid(blocks, Big::NT, "fra_linear_backward")) return rc;
         const dim3 grid((unsigned)blocks, shares);
         if (p.dw_side == 128) PJ_LAUNCH((pj_dw_kernel<T, Big>), grid, Big::NT, Big::LDS, s, a);
         else PJ_LAUNCH((pj_dw_kernel<T, Small>), grid, Small::NT, Small::LDS, s, a);
@@ -1095,7 +1096,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
             a.n_dw = (int64_t)d->N * d->K;
             const int64_t each = (a.n_dw + 4095) / 4096;
             blocks = each * G;
-            if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
+            if (int rc = check_grid(blocks, 1024, "fra_linear_backward")) return rc;
             a.join_each = (unsigned)each;
             a.n_join = (unsigned)blocks;
         }
@@ -1106,7 +1107,7 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
             a.tile_offsets = g ? (const int*)g->tile_offsets : nullptr;
             a.n_tiles = p.n_tiles; a.N = d->N; a.n_col_tiles = cdiv(d->N, 64); a.both = db && ds;
             blocks += (int64_t)a.n_col_tiles * G * (a.both ? 2 : 1);
-            if (int rc = check_grid(blocks, "fra_linear_backward")) return rc;
+            if (int rc = check_grid(blocks, 1024, "fra_linear_backward")) return rc;
         }
         hipLaunchKernelGGL((pj_finish_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, s, a);
         FRA_HIP(hipGetLastError());

@@ -322,7 +322,7 @@ template <typename T, bool BK, bool LAST, typename S, bool TOGETHER> static int 
     a.n_col_tiles = (a.Jp + S::BJ - 1) / S::BJ;
     a.batch = batch;
     const int64_t blocks = ((int64_t)a.n_row_tiles * a.n_col_tiles * batch + 7) / 8 * 8;
-    FRA_REQUIRE(blocks < 2147483647LL, FRA_ERR_ARG, "fra_orthogonalize: %lld workgroups", (long long)blocks);
+    FRA_REQUIRE(blocks <= 4294967295LL / S::NT, FRA_ERR_ARG, "fra_orthogonalize: %lld workgroups", (long long)blocks);    // threads of a launch: 32 bits
     hipLaunchKernelGGL((orth_product_kernel<T, BK, LAST, S, TOGETHER>), dim3((unsigned)blocks), dim3(S::NT), lds, s, a);
     FRA_HIP(hipGetLastError());
     return FRA_OK;

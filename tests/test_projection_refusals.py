@@ -127,3 +127,10 @@ def test_scratch_and_tables_have_to_be_aligned():
     assert lib.fra_group_rows(64, 0, C.byref(g), None, 0, None) == 1 and b"aligned" in lib.fra_last_error()
     assert lib.fra_linear(C.byref(desc(M=8, groups=C.pointer(g))), None, 64, None) == 1 and b"aligned" in lib.fra_last_error()
     assert lib.fra_orthogonalize(_lib.FRA_F32, 64, 8, 0, 1, 4, 8, 5, 1.5, -0.5, 0.0, 64, 68, 1 << 40, None) == 1 and b"aligned" in lib.fra_last_error()
+
+
+def test_more_threads_than_a_launch_takes():
+    lib = _lib.load()
+    g = _lib.RowGroupsDesc(8, 4096, lib.fra_group_tile_rows(8, 4096), lib.fra_group_tiles(8, 4096), 64, 64, 64, 64)
+    d = desc(M=8, N=1 << 16, groups=C.pointer(g))                   # 4097 row tiles x 4096 column tiles of 512 threads
+    assert lib.fra_linear(C.byref(d), None, 64, None) == 1 and b"launch" in lib.fra_last_error()
