@@ -21,6 +21,7 @@ from functools import lru_cache
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -65,6 +66,8 @@ class RowGroups:
 
     ``order`` int32 [rows]: row numbers by group, ascending inside a group, rows of no group last; ``offsets`` int32
     [n_groups + 1]: group g's rows are ``order[offsets[g]:offsets[g + 1]]``.  Serves any number of products of these rows.
+    For use on another stream than it was made on it is a tensor like any other: wait for it there, and before it is dropped
+    call ``groups.order.record_stream(stream)`` (all its parts are one allocation).
     """
 
     def __init__(self, rows: int, n_groups: int, ids: torch.Tensor):
@@ -248,7 +251,7 @@ def _check(what, x, weight, bias, activation, slope, residual, lead):
 def _apply(x, weight, bias, slope, residual, act, groups):
     if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
             or (slope is not None and slope.requires_grad) or (residual is not None and residual.requires_grad)) \
-            and torch.is_grad_enabled():
+            and torch.is_grad_enabled() or forward_ad._current_level >= 0:      # torch refuses a tangent there; it would be lost below
         return _Linear.apply(x, weight, bias, slope, residual, act, groups)
     return _forward(x, weight, bias, slope, residual, act, groups, False)[0]
 
@@ -293,7 +296,8 @@ def orthogonalize(matrix: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4
     X = matrix / |matrix|_F, then ``steps`` times X <- a X + (b P + c P P) X with P = X X^T (of the transposed matrix where it
     is taller than wide).  The default coefficients take every singular value of an update into about [0.7, 1.2] in five
     steps; (1.5, -0.5, 0) or (1.875, -1.25, 0.375) converge to the nearest orthogonal matrix in more.  A matrix of zeros gives
-    zeros.  Between the products values keep 22 bits.  Not differentiable: it sees the values only.
+    zeros.  Between the products values keep 22 bits in a range of +-255 (1 to 100 steps, coefficients within +-16: such that the
+    singular values stay near one).  Not differentiable: it sees the values only.
     """
     if not isinstance(matrix, torch.Tensor) or matrix.dim() < 2 or matrix.dtype not in _DTYPES:
         raise RuntimeError("orthogonalize: [..., rows, cols] in float32, float16 or bfloat16")

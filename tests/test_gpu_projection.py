@@ -402,6 +402,15 @@ def test_once_differentiable_and_saved_tensor_hooks(device):
         torch.autograd.grad(y, w, t["dy"])
 
 
+def test_forward_mode_is_refused(device):
+    t = make(5, 8, 6, torch.float32, device, 57)
+    with torch.autograd.forward_ad.dual_level():
+        x = torch.autograd.forward_ad.make_dual(t["x"], torch.ones_like(t["x"]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            call(dict(t, x=x), None)
+        assert torch.equal(call(t, None), call(t, None))            # no tangent, nothing to lose
+
+
 def test_saved_tensors_back_at_their_address_in_another_layout(device):
     # an allocator may hand the address of a freed view out again, to the packed copy that a hook brings back
     m, k, n = 48, 40, 56
