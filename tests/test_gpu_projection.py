@@ -497,3 +497,28 @@ def test_nothing_is_written_beside_the_outputs(device):
         for v in (y, dx, dw):
             assert (v[:64] == 7).all() and (v[-64:] == 7).all()
         assert (ws[need.value:] == 9).all()
+
+
+@pytest.mark.parametrize("act", [None, "gelu_tanh"])
+def test_rows_behind_two_to_the_31_elements(device, act):
+    # the last rows, and the group that only they belong to, lie behind 2^31 elements (2^32 bytes) of every operand
+    n_last, k, n = 300, 512, 520
+    m = 2 ** 31 // k + 5000
+    t = make(n_last, k, n, torch.bfloat16, device, 81, lead=(2,), act=act)
+    ids = torch.zeros(m, dtype=torch.int32, device=device)
+    ids[-n_last:] = 1
+    rg = projection.group_rows(ids, 2)
+    big = {}
+    for name, c in (("x", k), ("r", n), ("dy", n)):
+        big[name] = torch.zeros(m, c, dtype=torch.bfloat16, device=device)
+        big[name][-n_last:] = t[name]
+    out = run(dict(t, **big), act, rg)
+    want = reference(t, act, torch.ones(n_last, dtype=torch.int32))
+    got = {name: v[-n_last:] if name in ("y", "dx") else v for name, v in out.items()}
+    check({name: v if name in ("y", "dx") else v[1] for name, v in got.items()},
+          {name: want[name] if name in ("y", "dx") else tuple(p[1] for p in want[name]) for name in want})
+    assert not out["dx"][:1000].any() and not out["dw"][0].any()
+    # the same without groups: rows beyond the border, and gradients summed over all of them
+    one = dict(t, w=t["w"][1], b=t["b"][1])
+    plain = run(dict(one, **big), act)
+    check({"y": plain["y"][-n_last:], "dx": plain["dx"][-n_last:], "dw": plain["dw"]}, reference(one, act))
