@@ -286,8 +286,7 @@ struct DxArgs {
     int64_t lddz, ldw, wg;
     int K, Kp, N, Np, n_col_tiles;      // Np, Kp: columns of dz and W, zeros past N and K
 };
-template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_dx_kernel(DxArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+template <typename T, typename S> __device__ __forceinline__ void dx_tile(const DxArgs& a, unsigned block, char* lds) {
     typedef Product<T, false, true, S, true> P;
     struct Emit {
         struct Pre {};
@@ -307,12 +306,16 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
     f32x4 acc[S::MI][S::MJ];
     P p;
     Tile t;
-    if (!next_tile(a.rows, blockIdx.x, a.n_col_tiles, S::BI, S::BJ, t)) return;
+    if (!next_tile(a.rows, block, a.n_col_tiles, S::BI, S::BJ, t)) return;
     p.A.base = (const T*)a.dz; p.A.order = nullptr; p.A.ld = a.lddz; p.A.row0 = t.begin; p.A.rows = t.end - t.begin; p.A.klen = a.Np; p.A.cols = 0;
     p.B.base = (const T*)a.w + (t.live ? (int64_t)t.g * a.wg : 0) + t.c0; p.B.order = nullptr; p.B.ld = a.ldw; p.B.row0 = 0; p.B.rows = 0; p.B.klen = a.N; p.B.cols = a.Kp - t.c0;
     p.start(t.live ? a.Np : 0, lds);
     p.run(lds, acc);
     tile_emit<T, S>(acc, lds, Emit{a, t});
+}
+template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_dx_kernel(DxArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    dx_tile<T, S>(a, blockIdx.x, lds);
 }
 
 // dW[g] = sum over the group's rows of dz^T x: both operands k-major.  Several workgroups share the rows of a tile; what is not
@@ -352,21 +355,20 @@ template <typename O> struct DwEmit {
         store_chunk<O>(out + (int64_t)n * K + k0 + j, left, o);
     }
 };
-template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_dw_kernel(DwArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+template <typename T, typename S> __device__ __forceinline__ void dw_tile(const DwArgs& a, unsigned block, unsigned share, char* lds) {
     int ti, tj;
-    if (!tile_of_block(blockIdx.x, a.n_ti, a.n_tj, ti, tj)) return;
+    if (!tile_of_block(block, a.n_ti, a.n_tj, ti, tj)) return;
     int begin = 0, end = a.rows.M, g = 0, slot = -1;
     if (a.pieces) {
-        const int4 e = a.pieces[blockIdx.y];
+        const int4 e = a.pieces[share];
         if (e.x < 0) return;
         g = e.x; begin = e.y; end = e.z; slot = e.w;
     } else if (a.splits > 1) {                                      // whole steps per split
         const int step = S::KS * Elem<T>::KG, steps = (end + step - 1) / step;
-        const int64_t per = (int64_t)((steps + a.splits - 1) / a.splits) * step, b0 = blockIdx.y * per;
+        const int64_t per = (int64_t)((steps + a.splits - 1) / a.splits) * step, b0 = share * per;
         begin = b0 < end ? (int)b0 : end;
         end = b0 + per < end ? (int)(b0 + per) : end;
-        slot = blockIdx.y;
+        slot = share;
     }
     const int n0 = ti * S::BI, k0 = tj * S::BJ;
     typedef Product<T, true, true, S, true> P;
@@ -385,6 +387,22 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
         tile_emit<T, S>(acc, lds, f);
     }
 }
+// Both gradients' products in one launch: neither waits for the other, and one's last tiles run beside the other's.
+struct GradArgs {
+    DxArgs dx;
+    DwArgs dw;
+    unsigned dx_blocks, dw_blocks;          // dx's, then those of every share of dW: multiples of 8 (tile_of_block)
+};
+template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_grads_kernel(GradArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if (blockIdx.x < a.dx_blocks) {
+        dx_tile<T, S>(a.dx, blockIdx.x, lds);
+    } else {
+        const unsigned b = blockIdx.x - a.dx_blocks, share = b / a.dw_blocks;
+        dw_tile<T, S>(a.dw, b - share * a.dw_blocks, share, lds);
+    }
+}
+
 // dz = dy act'(z) in list order and, per row tile, the column sums of dz and of dy min(z, 0).  A workgroup takes one row tile x
 // `lpr` 16-byte pieces of columns (lpr lanes side by side, a power of two up to 16, so that narrow pieces make many workgroups;
 // 256 / lpr rows at a time); four rows per lane are requested together.  Bound by HBM and, with a sigmoid, by the vector ALU
@@ -998,6 +1016,26 @@ template <typename T, typename S> static int launch_dx(DxArgs& a, hipStream_t s)
     PJ_LAUNCH((pj_dx_kernel<T, S>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
     return FRA_OK;
 }
+// dx: its row tiles, or none; shares of dW, or none
+template <typename T, typename S> static int launch_grads(GradArgs& a, bool dx, int shares, hipStream_t s) {
+    int64_t blocks = 0;
+    a.dx_blocks = a.dw_blocks = 0;
+    if (dx) {
+        a.dx.n_col_tiles = cdiv(a.dx.K, S::BJ);
+        blocks = ((int64_t)a.dx.rows.n_tiles * a.dx.n_col_tiles + 7) / 8 * 8;
+        if (int rc = check_grid(blocks, S::NT, "fra_linear_backward")) return rc;
+        a.dx_blocks = (unsigned)blocks;
+    }
+    if (shares) {
+        a.dw.n_ti = cdiv(a.dw.N, S::BI); a.dw.n_tj = cdiv(a.dw.K, S::BJ);
+        const int64_t each = ((int64_t)a.dw.n_ti * a.dw.n_tj + 7) / 8 * 8;
+        blocks += each * shares;
+        if (int rc = check_grid(blocks, S::NT, "fra_linear_backward")) return rc;
+        a.dw_blocks = (unsigned)each;
+    }
+    PJ_LAUNCH((pj_grads_kernel<T, S>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
+    return FRA_OK;
+}
 template <typename T>
 static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const void* z, const void* dy, int64_t lddy, void* dx, void* dw,
                       void* db, void* ds, char* ws, hipStream_t s) {
@@ -1054,38 +1092,38 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
     }
     const void* dz = p.need_dz ? ws + p.off_dz : dy;
     const int64_t lddz = p.need_dz ? p.Np : lddy;
+    GradArgs a = {};
+    int dx_side = 0;
     if (dx && d->M > 0) {
-        DxArgs a;
-        a.w = d->w; a.ldw = d->ldw; a.wg = d->w_group_stride;
+        a.dx.w = d->w; a.dx.ldw = d->ldw; a.dx.wg = d->w_group_stride;
         if (p.pack_w) {
-            a.w = ws + p.off_w; a.ldw = p.Kp; a.wg = (int64_t)d->N * p.Kp;
+            a.dx.w = ws + p.off_w; a.dx.ldw = p.Kp; a.dx.wg = (int64_t)d->N * p.Kp;
         }
-        const int bi = tile_side(d->M, d->K, sizeof(T) == 4, g ? g->tile_rows : 256);
-        a.rows = row_args(d, bi);
-        a.dz = dz; a.dx = dx; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
-        int rc = FRA_OK;
-        if constexpr (sizeof(T) == 2) {
-            if (bi == 256) rc = launch_dx<T, Huge>(a, s);
-        }
-        if (bi != 256) rc = bi == 128 ? launch_dx<T, Big>(a, s) : bi == 64 ? launch_dx<T, Small>(a, s) : launch_dx<T, Tiny>(a, s);
-        if (rc != FRA_OK) return rc;
+        dx_side = tile_side(d->M, d->K, sizeof(T) == 4, g ? g->tile_rows : 256);
+        a.dx.rows = row_args(d, dx_side);
+        a.dx.dz = dz; a.dx.dx = dx; a.dx.lddz = lddz; a.dx.K = d->K; a.dx.Kp = p.Kp; a.dx.N = d->N; a.dx.Np = p.Np;
     }
+    const int shares = !dw ? 0 : g ? p.n_pieces : p.splits;
     if (dw) {
-        DwArgs a;
-        a.x = d->x; a.ldx = d->ldx;
+        a.dw.x = d->x; a.dw.ldx = d->ldx;
         if (p.pack_x) {
-            a.x = ws + p.off_x; a.ldx = p.Kp;
+            a.dw.x = ws + p.off_x; a.dw.ldx = p.Kp;
         }
-        a.rows = row_args(d, 128);
-        a.dz = dz; a.dw = dw; a.part = (float*)(ws + p.off_part); a.pieces = g ? (const int4*)(ws + p.off_pieces) : nullptr; a.lddz = lddz; a.K = d->K; a.Kp = p.Kp; a.N = d->N; a.Np = p.Np;
-        a.n_ti = cdiv(d->N, p.dw_side); a.n_tj = cdiv(d->K, p.dw_side); a.splits = p.splits;
-        const int64_t blocks = ((int64_t)a.n_ti * a.n_tj + 7) / 8 * 8;
-        const int shares = g ? p.n_pieces : p.splits;
-        FRA_REQUIRE(shares <= 65535, FRA_ERR_ARG, "fra_linear_backward: %d shares", shares);
-        if (int rc = check_grid(blocks, Big::NT, "fra_linear_backward")) return rc;
-        const dim3 grid((unsigned)blocks, shares);
-        if (p.dw_side == 128) PJ_LAUNCH((pj_dw_kernel<T, Big>), grid, Big::NT, Big::LDS, s, a);
-        else PJ_LAUNCH((pj_dw_kernel<T, Small>), grid, Small::NT, Small::LDS, s, a);
+        a.dw.rows = row_args(d, 128);
+        a.dw.dz = dz; a.dw.dw = dw; a.dw.part = (float*)(ws + p.off_part); a.dw.pieces = g ? (const int4*)(ws + p.off_pieces) : nullptr;
+        a.dw.lddz = lddz; a.dw.K = d->K; a.dw.Kp = p.Kp; a.dw.N = d->N; a.dw.Np = p.Np; a.dw.splits = p.splits;
+    }
+    // dx by its own kernel where its tiles have a side that dW's never have, else with dW if the sides agree
+    if constexpr (sizeof(T) == 2) {
+        if (dx_side == 256)
+            if (int rc = launch_dx<T, Huge>(a.dx, s)) return rc;
+    }
+    if (dx_side == 32)
+        if (int rc = launch_dx<T, Tiny>(a.dx, s)) return rc;
+    for (int side = 128; side >= 64; side /= 2) {
+        const int sh = p.dw_side == side ? shares : 0;
+        if (dx_side != side && !sh) continue;
+        if (int rc = side == 128 ? launch_grads<T, Big>(a, dx_side == side, sh, s) : launch_grads<T, Small>(a, dx_side == side, sh, s)) return rc;
     }
     if (p.need_sums || p.n_parts) {
         FinishArgs a = {};
