@@ -320,10 +320,10 @@ template <typename T, typename S> __global__ __launch_bounds__(S::NT, S::WAVES) 
 
 // dW[g] = sum over the group's rows of dz^T x: both operands k-major.  Several workgroups share the rows of a tile; what is not
 // the whole sum is left in fp32 and added in order by pj_finish_kernel.  Without groups: `splits` shares of the rows, partial sums
-// [split][N][K].  With groups: pieces of at most so many rows, made from the groups' sizes on the device (a group may hold any
-// part of the batch); a group of one piece, or none, is written at once, the pieces of the others are numbered through.
-// 2048 x 1024 x 4096 bf16 25 us with 5 for the joining (the library's plain product 39); 16 groups of 8192 rows, 1024 x 512 each,
-// 24 us (37 with whole groups: the largest one's tiles ran alone).
+// [split][N][K].  With groups: pieces of about so many rows, made from the groups' sizes on the device (a group may hold any part of
+// the batch), equal ones of a group so that none is a remainder (with remainders 16 groups of about 512 rows, pieces of 512: the whole
+// backward pass 60 us, 53 without); a group of one piece, or none, is written at once, the pieces of the others are numbered through.
+// By itself 2048 x 1024 x 4096 bf16 25 us with 5 for the joining (the library's plain product 39).
 struct DwArgs {
     RowArgs rows;
     const void *dz, *x;
@@ -337,7 +337,7 @@ struct PieceArgs {
     const int* offsets;
     int4* pieces;               // [n_pieces]
     int* slots;                 // [G + 1]: a group's first partial sum
-    int G, rows, n_pieces;      // rows: of a piece, at most
+    int G, rows, n_pieces;      // rows: of a piece, up to half as many more
     unsigned blocks;            // 1, or 0: no groups
 };
 template <typename O> struct DwEmit {
@@ -387,7 +387,9 @@ template <typename T, typename S> __device__ __forceinline__ void dw_tile(const 
         tile_emit<T, S>(acc, lds, f);
     }
 }
-// Both gradients' products in one launch: neither waits for the other, and one's last tiles run beside the other's.
+// Both gradients' products in one launch: neither waits for the other, and one's last tiles run beside the other's (4096 x 2048 x 1024
+// bf16 44 us, 52 one after the other; 8192 rows of 16 groups, 1024 x 512: 34 and 45; 1000 x 301 x 500 fp32 15.4 and 21).
+// dx first, whose tiles' sums (over N) are the longer ones more often than not: fp32 2999 x 513 x 250 41 us in all, 45 behind dW.
 struct GradArgs {
     DxArgs dx;
     DwArgs dw;
@@ -548,20 +550,21 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
     }
     return base + x - v;
 }
-// cuts the groups' rows into pieces (one workgroup)
+// cuts the groups' rows into pieces, a group into equal ones (one workgroup)
 __device__ __forceinline__ void cut_pieces(const PieceArgs& a, int* tmp) {
     int base = 0, sbase = 0;
     for (int g0 = 0; g0 < a.G; g0 += 256) {
         const int g = g0 + threadIdx.x;
         const int first = g < a.G ? a.offsets[g] : 0, end = g < a.G ? a.offsets[g + 1] : 0;
-        const int n = g < a.G ? (end - first > a.rows ? (end - first + a.rows - 1) / a.rows : 1) : 0, multi = n > 1 ? n : 0;
+        const int rows = end - first, n = g < a.G ? (rows > a.rows + a.rows / 2 ? (rows + a.rows / 2) / a.rows : 1) : 0, multi = n > 1 ? n : 0;
         int total, stotal;
         const int at = base + block_scan(n, tmp, total), slot = sbase + block_scan(multi, tmp, stotal);
         if (g < a.G) a.slots[g] = slot;
+        const int len = n > 1 ? (rows + n - 1) / n : rows;
         for (int i = 0; i < n; ++i) {
-            const int b = first + i * a.rows;
-            int4 e = {g, b, end - b > a.rows ? b + a.rows : end, multi ? slot + i : -1};
-            a.pieces[at + i] = e;
+            const int64_t b = (int64_t)i * len, e = b + len;
+            int4 v = {g, first + (int)(b < rows ? b : rows), first + (int)(e < rows ? e : rows), multi ? slot + i : -1};
+            a.pieces[at + i] = v;
         }
         base += total;
         sbase += stotal;
@@ -953,7 +956,7 @@ template <typename T> static int forward_t(const fra_linear_desc* d, void* z, vo
 // ---- backward: what goes where in the workspace
 struct BackwardPlan {
     bool need_dz, need_sums, pack_x, pack_w;
-    int dz_rows, n_tiles, splits, piece_rows, n_pieces, n_parts, dw_side, Np, Kp;
+    int dz_rows, n_tiles, splits, piece_rows, n_pieces, n_parts, dx_side, dw_side, Np, Kp;
     size_t off_dz, off_x, off_w, off_b, off_s, off_part, off_pieces, off_slots, bytes;
 };
 template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc* d, bool dx, bool dw, bool db, bool ds) {
@@ -979,6 +982,20 @@ template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc*
     p.dw_side = (int64_t)cdiv(d->N, 128) * cdiv(d->K, 128) * G * share >= 256 ? 128 : 64;
     const int64_t tiles = (int64_t)cdiv(d->N, p.dw_side) * cdiv(d->K, p.dw_side);
     int64_t sp = (512 + tiles - 1) / tiles;
+    // dx's tiles as the forward product's; 64 instead of 32 if that lets them into dW's launch (200 x 300 x 250 bf16: 12.5 us for the
+    // whole backward pass, 15.6 apart; fp32 64 x 512 x 512: 19.5 against 19.1)
+    p.dx_side = dx && d->M > 0 ? tile_side(d->M, d->K, sizeof(T) == 4, g ? g->tile_rows : 256) : 0;
+    if (p.dx_side == 32 && dw && p.dw_side == 64 && (!g || g->tile_rows >= 64)) p.dx_side = 64;
+    // where one round of workgroups holds dx and dW together, as many shares of dW as fill it, if they are no longer than dx's sums:
+    // 4096 x 1024 x 1024 bf16 36.9 us (dW in twice as many shares 46.4), fp32 165 (202).  A group adds half a tile of rows to dx and
+    // half a piece to dW on average (8192 rows of 2 groups, 512 x 512, bf16 33 us, fp32 111; 43 and 124 without; without the allowance
+    // 37 and 134)
+    if (dw && p.dx_side == p.dw_side) {
+        const int side = p.dx_side, half = g ? G / 2 : 0;
+        const int64_t dx_tiles = (int64_t)(cdiv(d->M, side) + half) * cdiv(d->K, side);
+        const int64_t fit = (256 * (side == 128 ? Big::PER_CU : Small::PER_CU) - dx_tiles) / tiles - half;
+        if (fit >= 1 && d->M <= fit * d->N * 5 / 4) sp = fit;
+    }
     p.splits = 1;
     p.piece_rows = p.n_pieces = p.n_parts = 0;
     if (dw && g) {
@@ -987,7 +1004,7 @@ template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc*
         rows = rows < 128 ? 128 : (rows + 63) / 64 * 64;
         p.piece_rows = (int)rows;
         p.n_pieces = (int)(d->M / rows) + G;
-        p.n_parts = (int)(2 * d->M / rows);     // a group of n > 1 pieces has more than n / 2 pieces' rows
+        p.n_parts = (int)(2 * d->M / rows);     // a group of n > 1 pieces has more than n / 2 times as many
     } else if (dw) {
         if (sp > share) sp = share;
         if (sp > 1) p.splits = (int)sp;
@@ -1093,14 +1110,13 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
     const void* dz = p.need_dz ? ws + p.off_dz : dy;
     const int64_t lddz = p.need_dz ? p.Np : lddy;
     GradArgs a = {};
-    int dx_side = 0;
-    if (dx && d->M > 0) {
+    const int dx_side = p.dx_side;
+    if (dx_side) {
         a.dx.w = d->w; a.dx.ldw = d->ldw; a.dx.wg = d->w_group_stride;
         if (p.pack_w) {
             a.dx.w = ws + p.off_w; a.dx.ldw = p.Kp; a.dx.wg = (int64_t)d->N * p.Kp;
         }
-        dx_side = tile_side(d->M, d->K, sizeof(T) == 4, g ? g->tile_rows : 256);
-        a.dx.rows = row_args(d, dx_side);
+        a.dx.rows = row_args(d, p.dx_side);
         a.dx.dz = dz; a.dx.dx = dx; a.dx.lddz = lddz; a.dx.K = d->K; a.dx.Kp = p.Kp; a.dx.N = d->N; a.dx.Np = p.Np;
     }
     const int shares = !dw ? 0 : g ? p.n_pieces : p.splits;
