@@ -652,13 +652,15 @@ template <typename T> __global__ __launch_bounds__(1024) void pj_finish_kernel(F
 }
 // ---- rows by group: a stable counting sort --------------------------------------------------------------------------
 // key = id, or G where id is outside [0, G).  A workgroup of NW waves owns NW * 64 KEYS consecutive rows, a wave 64 KEYS of them,
-// kept as KEYS keys per lane: four, or eight where that makes it one workgroup (and one launch: 8192 rows 12.6 us against 8.3 + 4.8;
-// 30001 rows take 8.7 + 5.0 us with four and 12.3 + 7.6 with eight).  Lanes with the same key find each other by ballots over the
+// kept as KEYS keys per lane: four, or eight where that makes it one workgroup (and one launch).  Eight waves, whose barriers and
+// sums over waves are short (9 rows 4.2 us, with sixteen 5.3; 12000 rows of 16 groups 10.0 and 12.5; 30001 of 37 11.0 and 13.3), but
+// sixteen for very many rows, whose workgroups' counts are added up (1000000 rows of 100 groups 33 us, with eight 41).  Lanes with the same key find each other by ballots over the
 // key's bits, so a row's rank among its wave's rows of the key is the wave's running count plus the equal lanes below: no atomics,
 // and the order does not depend on timing.  One launch for one workgroup; else the counts of all workgroups first.  Bound by
-// latency: a dozen rows take 4 us, of which a launch is two.
+// latency: a launch alone is two of the 4.2 us.
 constexpr int GR_MAX_GROUPS = 4096;
-constexpr int GR_WIDE_KEYS = 1025;          // up to this many keys sixteen waves' counters fit in LDS, beyond it four waves'
+constexpr int GR_WIDE_KEYS = 1025;          // up to this many keys eight and sixteen waves' counters fit in LDS, beyond it four waves'
+constexpr int GR_MANY_ROWS = 1 << 18;       // sixteen waves beyond this
 constexpr int GR_INLINE_SCAN = 8192;        // counters up to which every workgroup adds the others' counts itself
 struct GroupArgs {
     const void* ids;
@@ -1169,17 +1171,21 @@ static int backward_t(const fra_linear_desc* d, const BackwardPlan& plan, const 
     return FRA_OK;
 }
 
-static bool group_wide(int n_groups) { return n_groups + 1 <= GR_WIDE_KEYS; }
+// sixteen waves where they make it one launch, too: 8192 rows of 16 groups 11.4 us, in two 10.1, but a launch costs the host 3
+static int group_waves(int64_t M, int n_groups) {
+    if (n_groups + 1 > GR_WIDE_KEYS) return 4;
+    return M > GR_MANY_ROWS || (M > 4096 && M <= 8192) ? 16 : 8;
+}
 static int group_keys(int64_t M, int n_groups) {
-    const int waves = group_wide(n_groups) ? 16 : 4;
+    const int waves = group_waves(M, n_groups);
     return M > waves * 256 && M <= waves * 512 ? 8 : 4;
 }
 static int group_blocks(int64_t M, int n_groups) {
-    const int per = (group_wide(n_groups) ? 16 : 4) * 64 * group_keys(M, n_groups);
+    const int per = group_waves(M, n_groups) * 64 * group_keys(M, n_groups);
     return M > per ? cdiv(M, per) : 1;
 }
 template <int NW, int KEYS> static int launch_groups(GroupArgs& a, hipStream_t s) {
-    const int keys = a.G + 1, most = (NW == 16 ? GR_WIDE_KEYS : GR_MAX_GROUPS + 1) * 4, lds = (NW + 2) * keys * 4;
+    const int keys = a.G + 1, most = (NW > 4 ? GR_WIDE_KEYS : GR_MAX_GROUPS + 1) * 4, lds = (NW + 2) * keys * 4;
     static std::atomic<uint64_t> done_count{0}, done_place{0};
     if (int rc = raise_lds(pj_group_kernel<NW, KEYS, false>, (NW + 2) * most + GR_INLINE_SCAN * 4, done_place)) return rc;
     if constexpr (KEYS == 4) {
@@ -1279,8 +1285,9 @@ int fra_group_rows(const void* ids, int ids_are_64bit, const fra_row_groups* g, 
     a.bits = 0;
     while ((1 << a.bits) < a.G + 1) ++a.bits;
     hipStream_t s = (hipStream_t)stream;
-    if (group_keys(a.M, a.G) == 8) return group_wide(a.G) ? launch_groups<16, 8>(a, s) : launch_groups<4, 8>(a, s);
-    return group_wide(a.G) ? launch_groups<16, 4>(a, s) : launch_groups<4, 4>(a, s);
+    const int waves = group_waves(a.M, a.G);
+    if (group_keys(a.M, a.G) == 8) return waves == 16 ? launch_groups<16, 8>(a, s) : waves == 8 ? launch_groups<8, 8>(a, s) : launch_groups<4, 8>(a, s);
+    return waves == 16 ? launch_groups<16, 4>(a, s) : waves == 8 ? launch_groups<8, 4>(a, s) : launch_groups<4, 4>(a, s);
 }
 
 }  // extern "C"

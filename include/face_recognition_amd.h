@@ -324,8 +324,8 @@ typedef struct {
     const fra_row_groups* groups;                   /* NULL: one matrix for all rows */
 } fra_linear_desc;
 /* ids: dev int32 or int64 [g->rows]; fills order, offsets, tiles and tile_offsets of *g (whose sizes the caller has set).  A
- * stable counting sort: one launch up to 8192 rows (2048 with more than 1024 groups), else two or three.  At most 4096 groups.  Scratch: dev,
- * fra_group_rows_workspace_bytes(). */
+ * stable counting sort: one launch up to 8192 rows (2048 with more than 1024 groups), else two or three.  At most 4096 groups.
+ * Scratch: dev, fra_group_rows_workspace_bytes(). */
 int fra_group_tile_rows(int64_t rows, int n_groups);
 int fra_group_tiles(int64_t rows, int n_groups);
 int fra_group_rows_workspace_bytes(int64_t rows, int n_groups, size_t* bytes);
