@@ -174,6 +174,25 @@ def test_groups_of_very_different_sizes(device, shares, dt):
     check(run(t, "silu", projection.group_rows(ids.to(device), groups)), reference(t, "silu", ids))
 
 
+# the gradients' products on tiles of one side in one launch (with as many shares as fill a round, and without), of different sides
+# apart, dx on the largest tiles and on the smallest
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("m,k,n,act", [(4096, 1024, 600, "gelu_tanh"), (4100, 1020, 130, None), (2000, 1024, 520, "silu"), (1000, 100, 5000, "relu"),
+                                       (16384, 2048, 24, None)])
+def test_gradients_of_many_tiles(device, m, k, n, act, dt):
+    t = make(m, k, n, dt, device, k + n, act=act, residual=False)
+    check(run(t, act), reference(t, act))
+
+
+# 38401 rows in 300 equal pieces of 129 leave the last two empty; 192 rows are one piece, 193 two
+@pytest.mark.parametrize("shares", [(38401, 11599), (192, 193, 191, 1, 500)], ids=str)
+def test_pieces_of_a_group(device, shares):
+    ids = torch.repeat_interleave(torch.arange(len(shares)), torch.tensor(shares))
+    ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(2))]
+    t = make(len(ids), 24, 16, torch.float16, device, 18, lead=(len(shares),))
+    check(run(t, None, projection.group_rows(ids.to(device), len(shares))), reference(t, None, ids))
+
+
 @pytest.mark.parametrize("kind", ["all_one", "none", "last_only"])
 def test_grouped_extremes(device, kind):
     m, k, n, groups = 333, 48, 56, 6
