@@ -903,20 +903,26 @@ static int check_grid(int64_t blocks, int threads, const char* what) {
 // 826 against 977 us) but holds one workgroup per compute unit, so it takes rounds that are nearly full (4096 x 2048 x 1024, half a
 // round: 37 against 24 us), and 16-bit operands: fp32 tiles are bound by the matrix cores at any size.  128 from one tile per unit
 // on, 64 from half of that on (2999 x 513 x 250 in fp32: 423 tiles of 64 15.5 us, 1598 of 32 21.3), below it 32 (1000 x 301 x 500 is
-// 80 tiles of 64 on 256 units).  Rows in groups: at most the table's tiles (`most`).
+// 80 tiles of 64 on 256 units).  The columns have to fill the tiles: 256 to seven eighths (262144 x 300 x 512 bf16 161 us on 128 x 128,
+// 217 on 256 x 256; 262144 x 512 x 512 219 and 185), 128 to more than half (262144 x 64 x 512 bf16 59 us on 64 x 64; fp32 171, on
+// 128 x 128 289), and for fp32, which the matrix cores bound, 64 it is where they are a twentieth fewer (262144 x 130 x 512: 452 us
+// against 587).  Rows in groups: at most the table's tiles (`most`).
 static int tile_side(int64_t rows, int64_t cols, bool f32, int most = 256) {
     auto tiles = [&](int side) { return (int64_t)cdiv(rows, side) * cdiv(cols, side); };
     const int64_t huge = tiles(256);
-    if (most >= 256 && !f32 && huge >= 512 && huge * 10 >= (huge + 255) / 256 * 256 * 9) return 256;
-    if (most >= 128 && tiles(128) >= 256) return 128;
+    if (most >= 256 && !f32 && cols * 8 >= (int64_t)cdiv(cols, 256) * 256 * 7 && huge >= 512 && huge * 10 >= (huge + 255) / 256 * 256 * 9) return 256;
+    if (most >= 128 && cols > 64 && tiles(128) >= 256 && !(f32 && cdiv(cols, 64) * 21 <= cdiv(cols, 128) * 40)) return 128;
     return most >= 64 && tiles(64) >= 128 ? 64 : 32;
 }
 
+template <typename T> static bool forward_dma(const fra_linear_desc* d) {
+    return dma_ok<T>(d->x, d->ldx, d->K) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
+}
 template <typename T, typename S> static int launch_forward(const fra_linear_desc* d, FwdArgs& a, hipStream_t s) {
     a.n_col_tiles = cdiv(d->N, S::BJ);
     const int64_t blocks = ((int64_t)a.rows.n_tiles * a.n_col_tiles + 7) / 8 * 8;
     if (int rc = check_grid(blocks, S::NT, "fra_linear")) return rc;
-    if (dma_ok<T>(d->x, d->ldx, d->K) && dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K))
+    if (forward_dma<T>(d))
         PJ_LAUNCH((pj_forward_kernel<T, S, true>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
     else
         PJ_LAUNCH((pj_forward_kernel<T, S, false>), dim3((unsigned)blocks), S::NT, S::LDS, s, a);
@@ -932,22 +938,27 @@ template <typename T, int MT> static int launch_few_rows(const fra_linear_desc* 
 }
 template <typename T> static int forward_t(const fra_linear_desc* d, void* z, void* y, hipStream_t s) {
     FwdArgs a;
-    // Few rows have a kernel of their own, then it goes by the number of tiles.  fp32: up to 64 rows (K = 512, N = 512: 8.3 us against
-    // 9.6 of tiles; N = 40961: 66 against 76).  16 bits: up to 32 (K = 2048, N = 4096: 8.7 against 10.5; 64 rows 13.0 against 10.7),
-    // or 16 where N alone fills the chip with tiles (K = 512, N = 40961: 1 row 11.8 against 14.2, 32 rows 20.5 against 14.4)
-    const bool few = d->groups ? d->groups->tile_rows == 16 : d->M <= (sizeof(T) == 4 ? 64 : cdiv(d->N, 64) < 256 ? 32 : 16);
-    const int bi = few ? (d->groups || d->M <= 16 ? 16 : d->M <= 32 ? 32 : 64)
-                       : tile_side(d->M, d->N, sizeof(T) == 4, d->groups ? d->groups->tile_rows : 256);
+    // Few rows, or so few columns that tiles would be empty, have a kernel of their own.  (Its sums are in another order, so beyond 64
+    // rows a value does not depend on the number of rows beside it: there the columns alone decide.)  Columns: up to 16, the kernel's
+    // own (262144 x 16 x 512 bf16 53 us, on tiles 116; fp32 125 and 289).  Rows: fp32 up to 64 (64 x 40961 x 512 66 us, on tiles 76).
+    // 16 bits up to 16 (1 x 40961 x 512 11.8 and 14.2), and up to 64 by what a compute unit fetches, in rows of k: this kernel's tiles
+    // are smaller, the others' read a wide product's operands less often (50 x 333 x 512 3.4 us, on tiles 5.2; 64 x 4096 x 2048 13.0
+    // and 10.4).  What DMA cannot take stays longer in the tiles' steps, for which it gets two rows of sixteen in advance.
+    const int most = d->groups ? d->groups->tile_rows : 256, side = tile_side(d->M, d->N, sizeof(T) == 4, most);
+    auto fetched = [&](int bi, int bj) { return ((int64_t)cdiv(d->M, bi) * cdiv(d->N, bj) + 255) / 256 * ((bi + bj) / 16); };
+    int mt = 1;                                                     // tiles of 16 rows: as many as fetch least
+    for (int i = 2; i <= 4; i *= 2)
+        if (16 * i <= most && fetched(16 * i, 16) < fetched(16 * mt, 16)) mt = i;
+    const bool few = most == 16 || d->N <= 16 || d->M <= (sizeof(T) == 4 ? 64 : 16) ||
+                     (d->M <= 64 && fetched(16 * mt, 16) < fetched(side, side) + (forward_dma<T>(d) ? 0 : 2));
+    const int bi = few ? 16 * mt : side;
     a.rows = row_args(d, bi);
     a.x = d->x; a.w = d->w; a.bias = d->bias; a.slope = d->slope; a.resid = d->resid; a.z = z; a.y = y;
     a.ldx = d->ldx; a.ldw = d->ldw; a.wg = d->w_group_stride; a.ldr = d->ldr;
     a.K = d->K; a.N = d->N; a.act = d->act; a.bias_f32 = d->bias_dtype == FRA_F32; a.slope_f32 = d->slope_dtype == FRA_F32;
     if (few) {
         if (bi == 16) return launch_few_rows<T, 1>(d, a, s);
-        if constexpr (sizeof(T) == 4) {
-            if (bi == 64) return launch_few_rows<T, 4>(d, a, s);
-        }
-        return launch_few_rows<T, 2>(d, a, s);
+        return bi == 32 ? launch_few_rows<T, 2>(d, a, s) : launch_few_rows<T, 4>(d, a, s);
     }
     if constexpr (sizeof(T) == 2) {
         if (bi == 256) return launch_forward<T, Huge>(d, a, s);
