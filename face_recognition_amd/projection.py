@@ -35,21 +35,16 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-class _on_device:
-    """``torch.cuda.device`` that costs nothing when the device is the current one already."""
-    __slots__ = ("index", "prev")
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+def _on_device(device: torch.device, call, *args):
+    """``call(*args)`` with `device` as the current one; nothing to do if it is (``torch.cuda.device`` costs 1 us either way)."""
+    prev = torch._C._cuda_getDevice()
+    if prev == device.index:
+        return call(*args)
+    torch.cuda.set_device(device.index)
+    try:
+        return call(*args)
+    finally:
+        torch.cuda.set_device(prev)
 
 
 @lru_cache(maxsize=256)
@@ -102,11 +97,10 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
     ids = ids.contiguous()
     rows = ids.shape[0]
     need = _group_sizes(rows, n_groups)[2]
-    with _on_device(ids.device):
-        g = RowGroups(rows, n_groups, ids)
-        ws = ids.new_empty(need, dtype=torch.uint8) if need else None
-        _lib.check(_lib.load().fra_group_rows(ids.data_ptr(), ids.dtype == torch.int64, C.byref(g._desc),
-                                              ws.data_ptr() if need else None, need, _stream(ids.device)), "fra_group_rows")
+    g = RowGroups(rows, n_groups, ids)
+    ws = ids.new_empty(need, dtype=torch.uint8) if need else None
+    _lib.check(_on_device(ids.device, _lib.load().fra_group_rows, ids.data_ptr(), ids.dtype == torch.int64, C.byref(g._desc),
+                          ws.data_ptr() if need else None, need, _stream(ids.device)), "fra_group_rows")
     return g
 
 
@@ -154,9 +148,8 @@ def _forward(x, weight, bias, slope, residual, act, groups, want_preact):
     z = torch.empty_like(out) if want_preact else None
     d = _desc(x, ldx, weight, ldw, wg, bias, slope, residual, ldr, act, groups)
     if out.shape[0]:
-        with _on_device(x.device):
-            _lib.check(_lib.load().fra_linear(C.byref(d), z.data_ptr() if z is not None else None, out.data_ptr(),
-                                              _stream(x.device)), "fra_linear")
+        _lib.check(_on_device(x.device, _lib.load().fra_linear, C.byref(d), z.data_ptr() if z is not None else None,
+                              out.data_ptr(), _stream(x.device)), "fra_linear")
     return out, z, d, (x, weight, slope)
 
 
@@ -183,15 +176,14 @@ def _backward(ctx, dy):
             z = z.contiguous()
         lib = _lib.load()
         g, lddy = _rows(dy)
-        with _on_device(x.device):
-            nbytes = C.c_size_t()
-            _lib.check(lib.fra_linear_backward_workspace_bytes(C.byref(d), need[0], need[1], need[2], need[3], C.byref(nbytes)),
-                       "fra_linear_backward_workspace_bytes")
-            ws = x.new_empty(nbytes.value, dtype=torch.uint8)
-            _lib.check(lib.fra_linear_backward(C.byref(d), z.data_ptr() if z is not None else None, g.data_ptr(), lddy,
-                                               dx.data_ptr() if need[0] else None, dw.data_ptr() if need[1] else None,
-                                               db.data_ptr() if need[2] else None, ds.data_ptr() if need[3] else None,
-                                               ws.data_ptr(), nbytes.value, _stream(x.device)), "fra_linear_backward")
+        nbytes = C.c_size_t()
+        _lib.check(lib.fra_linear_backward_workspace_bytes(C.byref(d), need[0], need[1], need[2], need[3], C.byref(nbytes)),
+                   "fra_linear_backward_workspace_bytes")
+        ws = x.new_empty(nbytes.value, dtype=torch.uint8)
+        _lib.check(_on_device(x.device, lib.fra_linear_backward, C.byref(d), z.data_ptr() if z is not None else None,
+                              g.data_ptr(), lddy, dx.data_ptr() if need[0] else None, dw.data_ptr() if need[1] else None,
+                              db.data_ptr() if need[2] else None, ds.data_ptr() if need[3] else None,
+                              ws.data_ptr(), nbytes.value, _stream(x.device)), "fra_linear_backward")
     return dx, dw, db, ds, (dy if need[4] else None), None, None
 
 
@@ -214,6 +206,13 @@ class _Linear(torch.autograd.Function):
         return _Linear._once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
+def _check_parameter(what, name, t, shape, dt, device):
+    if t.shape != shape or (t.dtype != dt and t.dtype != torch.float32):
+        raise RuntimeError(f"{what}: {name} must be {list(shape)} in {dt} or float32, got {list(t.shape)} {t.dtype}")
+    if t.device != device:
+        raise RuntimeError(f"{what}: {name} is on {t.device}, x on {device}")
+
+
 def _check(what, x, weight, bias, activation, slope, residual, lead):
     act = ACTIVATIONS.get(activation, -1) if activation is None or isinstance(activation, str) else -1
     if act < 0:
@@ -223,28 +222,29 @@ def _check(what, x, weight, bias, activation, slope, residual, lead):
         raise RuntimeError(f"{what}: {dt} is not supported (float32, float16, bfloat16)")
     if not x.is_cuda:
         raise RuntimeError(f"{what}: tensors live on the HIP device ('cuda'); there is no CPU path")
-    ws = weight.shape
-    if len(ws) != 2 + len(lead) or ws[:-2] != lead:
+    ws, xs, dev = weight.shape, x.shape, x.device
+    if len(ws) != 2 + len(lead) or (lead and ws[:-2] != lead):
         raise RuntimeError(f"{what}: weight must be [{', '.join([str(v) for v in lead] + ['N', 'K'])}], got {tuple(ws)}")
-    n, k = ws[-2:]
-    xs = x.shape
-    if n == 0 or k == 0 or len(xs) < 1 or xs[-1] != k:
+    n, k = ws[-2], ws[-1]
+    if n == 0 or k == 0 or not xs or xs[-1] != k:
         raise RuntimeError(f"{what}: x {tuple(xs)} does not go with weight {tuple(ws)}")
+    if weight.dtype != dt:
+        raise RuntimeError(f"{what}: weight is {weight.dtype}, x is {dt}")
+    if weight.device != dev:
+        raise RuntimeError(f"{what}: weight is on {weight.device}, x on {dev}")
     if (act == 2) != (slope is not None):
         raise RuntimeError(f"{what}: slope goes with activation 'prelu', and only with it")
-    par = lead + (n,)
-    for name, t in (("bias", bias), ("slope", slope)):
-        if t is not None and (t.shape != par or (t.dtype != dt and t.dtype != torch.float32)):
-            raise RuntimeError(f"{what}: {name} must be {list(par)} in {dt} or float32, got {list(t.shape)} {t.dtype}")
-    if residual is not None and residual.shape != xs[:-1] + (n,):
-        raise RuntimeError(f"{what}: residual must be {list(xs[:-1]) + [n]}, got {list(residual.shape)}")
-    for name, t in (("weight", weight), ("residual", residual)):
-        if t is not None and t.dtype != dt:
-            raise RuntimeError(f"{what}: {name} is {t.dtype}, x is {dt}")
-    dev = x.device
-    for name, t in (("weight", weight), ("bias", bias), ("slope", slope), ("residual", residual)):
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, x on {dev}")
+    if bias is not None:
+        _check_parameter(what, "bias", bias, lead + (n,), dt, dev)
+    if slope is not None:
+        _check_parameter(what, "slope", slope, lead + (n,), dt, dev)
+    if residual is not None:
+        if residual.shape != xs[:-1] + (n,):
+            raise RuntimeError(f"{what}: residual must be {list(xs[:-1]) + [n]}, got {list(residual.shape)}")
+        if residual.dtype != dt:
+            raise RuntimeError(f"{what}: residual is {residual.dtype}, x is {dt}")
+        if residual.device != dev:
+            raise RuntimeError(f"{what}: residual is on {residual.device}, x on {dev}")
     return act
 
 
@@ -320,10 +320,8 @@ def orthogonalize(matrix: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4
     out = torch.empty(matrix.shape, dtype=matrix.dtype, device=matrix.device)
     need = C.c_size_t()
     _lib.check(lib.fra_orthogonalize_workspace_bytes(batch, rows, cols, C.byref(need)), "fra_orthogonalize_workspace_bytes")
-    with _on_device(matrix.device):
-        ws = torch.empty(need.value, dtype=torch.uint8, device=matrix.device)
-        _lib.check(lib.fra_orthogonalize(_DTYPES[g.dtype], g.data_ptr(), s0 if rows > 1 else cols,
-                                         g.stride(0) if g.dim() == 3 else 0, batch, rows, cols, int(steps),
-                                         *[float(v) for v in coefficients], out.data_ptr(), ws.data_ptr(), need.value,
-                                         _stream(matrix.device)), "fra_orthogonalize")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=matrix.device)
+    _lib.check(_on_device(matrix.device, lib.fra_orthogonalize, _DTYPES[g.dtype], g.data_ptr(), s0 if rows > 1 else cols,
+                          g.stride(0) if g.dim() == 3 else 0, batch, rows, cols, int(steps), *[float(v) for v in coefficients],
+                          out.data_ptr(), ws.data_ptr(), need.value, _stream(matrix.device)), "fra_orthogonalize")
     return out
