@@ -77,12 +77,12 @@ class RowGroups:
     @property
     def order(self) -> torch.Tensor:
         at = 4 * self._desc.n_tiles
-        return self._buf[at:at + self.rows]
+        return self._buf.narrow(0, at, self.rows)
 
     @property
     def offsets(self) -> torch.Tensor:
         at = 4 * self._desc.n_tiles + self.rows
-        return self._buf[at:at + self.n_groups + 1]
+        return self._buf.narrow(0, at, self.n_groups + 1)
 
 
 def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
@@ -104,9 +104,8 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
     return g
 
 
-def _rows(t: torch.Tensor):
-    """(tensor, pitch): 2-D with contiguous rows, copied only if it is not."""
-    r, c = t.shape
+def _rows(t: torch.Tensor, r: int, c: int):
+    """(tensor, pitch) of [r,c]: contiguous rows, copied only if they are not."""
     s0, s1 = t.stride()
     if (s1 != 1 and c > 1) or (r > 1 and s0 < c):
         t = t.contiguous()
@@ -114,77 +113,80 @@ def _rows(t: torch.Tensor):
     return t, (s0 if r > 1 else c)
 
 
-def _desc(x, ldx, weight, ldw, wg, bias, slope, residual, ldr, act, groups):
-    return _lib.LinearDesc(_DTYPES[x.dtype], act, _DTYPES[bias.dtype] if bias is not None else 0,
-                           _DTYPES[slope.dtype] if slope is not None else 0, x.shape[0], x.shape[1], weight.shape[-2],
-                           x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
-                           slope.data_ptr() if slope is not None else None,
-                           residual.data_ptr() if residual is not None else None, ldx, ldw, ldr, wg,
-                           C.pointer(groups._desc) if groups is not None else None)
-
-
-def _weight(weight):
+def _weight(weight: torch.Tensor, n: int, k: int):
     """(tensor, row pitch, group pitch) of [N,K] or [G,N,K] with contiguous rows."""
-    n, k = weight.shape[-2:]
-    s0, s1 = weight.stride()[-2:]
-    if (s1 != 1 and k > 1) or (n > 1 and s0 < k) or (weight.dim() == 3 and weight.stride(0) < 0):
+    if weight.dim() == 2:
+        return *_rows(weight, n, k), 0
+    sg, s0, s1 = weight.stride()
+    if (s1 != 1 and k > 1) or (n > 1 and s0 < k):
         weight = weight.contiguous()
-        s0 = k
-    return weight, (s0 if n > 1 else k), (weight.stride(0) if weight.dim() == 3 else 0)
+        sg, s0 = n * k, k
+    return weight, (s0 if n > 1 else k), sg
 
 
 def _forward(x, weight, bias, slope, residual, act, groups, want_preact):
-    """(out, preact, descriptor, (x, weight, slope) as the kernels read them)."""
-    x, ldx = _rows(x)
-    weight, ldw, wg = _weight(weight)
+    """(out, preact, descriptor, (x, weight, slope) as the kernels read them).  Sizes are taken apart once, and `new_empty` gets
+    plain numbers: a shape costs 1 us more."""
+    m, k = x.shape
+    n = weight.shape[-2]
+    dt = _DTYPES[x.dtype]
+    x, ldx = _rows(x, m, k)
+    weight, ldw, wg = _weight(weight, n, k)
     ldr = 0
     if residual is not None:
-        residual, ldr = _rows(residual)
+        residual, ldr = _rows(residual, m, n)
     if bias is not None:
         bias = bias.contiguous()
     if slope is not None:
         slope = slope.contiguous()
-    out = x.new_empty((x.shape[0], weight.shape[-2]))
+    out = x.new_empty(m, n)
     z = torch.empty_like(out) if want_preact else None
-    d = _desc(x, ldx, weight, ldw, wg, bias, slope, residual, ldr, act, groups)
-    if out.shape[0]:
-        _lib.check(_on_device(x.device, _lib.load().fra_linear, C.byref(d), z.data_ptr() if z is not None else None,
-                              out.data_ptr(), _stream(x.device)), "fra_linear")
+    d = _lib.LinearDesc(dt, act, _DTYPES[bias.dtype] if bias is not None else 0, _DTYPES[slope.dtype] if slope is not None else 0,
+                        m, k, n, x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
+                        slope.data_ptr() if slope is not None else None, residual.data_ptr() if residual is not None else None,
+                        ldx, ldw, ldr, wg, C.pointer(groups._desc) if groups is not None else None)
+    if m:
+        device = x.device
+        _lib.check(_on_device(device, _lib.load().fra_linear, C.byref(d), z.data_ptr() if z is not None else None,
+                              out.data_ptr(), _stream(device)), "fra_linear")
     return out, z, d, (x, weight, slope)
 
 
 def _backward(ctx, dy):
-    x, weight, slope, z = ctx.saved_tensors
-    need = ctx.needs_input_grad
-    d = ctx.desc
+    need_x, need_w, need_b, need_s, need_r, _, _ = ctx.needs_input_grad
     dx = dw = db = ds = None
-    if need[0] or need[1] or need[2] or need[3]:
-        if need[0]:
-            dx = x.new_empty(x.shape)
-        if need[1]:
-            dw = x.new_empty(weight.shape)
-        if need[2]:
-            db = x.new_empty(weight.shape[:-1], dtype=ctx.bias_dtype)
-        if need[3]:
-            ds = x.new_empty(weight.shape[:-1], dtype=slope.dtype)
+    if need_x or need_w or need_b or need_s:
+        x, weight, slope, z = ctx.saved_tensors
+        d, groups = ctx.desc, ctx.groups
+        m, k, n = d.M, d.K, d.N
+        lead = (groups.n_groups,) if groups is not None else ()
+        if need_x:
+            dx = x.new_empty(m, k)
+        if need_w:
+            dw = x.new_empty(*lead, n, k)
+        if need_b:
+            db = x.new_empty(*lead, n, dtype=ctx.bias_dtype)
+        if need_s:
+            ds = x.new_empty(*lead, n, dtype=slope.dtype)
         # saved-tensor hooks may bring back other tensors, or the same memory laid out otherwise
-        x, d.ldx = _rows(x)
-        weight, d.ldw, d.w_group_stride = _weight(weight)
-        slope = slope.contiguous() if slope is not None else None
-        d.x, d.w, d.slope = x.data_ptr(), weight.data_ptr(), slope.data_ptr() if slope is not None else None
+        x, d.ldx = _rows(x, m, k)
+        weight, d.ldw, d.w_group_stride = _weight(weight, n, k)
+        d.x, d.w = x.data_ptr(), weight.data_ptr()
+        if slope is not None:
+            slope = slope.contiguous()
+            d.slope = slope.data_ptr()
         if z is not None:
             z = z.contiguous()
-        lib = _lib.load()
-        g, lddy = _rows(dy)
-        nbytes = C.c_size_t()
-        _lib.check(lib.fra_linear_backward_workspace_bytes(C.byref(d), need[0], need[1], need[2], need[3], C.byref(nbytes)),
+        lib, device, nbytes = _lib.load(), x.device, C.c_size_t()
+        g, lddy = _rows(dy, m, n)
+        _lib.check(lib.fra_linear_backward_workspace_bytes(C.byref(d), need_x, need_w, need_b, need_s, C.byref(nbytes)),
                    "fra_linear_backward_workspace_bytes")
         ws = x.new_empty(nbytes.value, dtype=torch.uint8)
-        _lib.check(_on_device(x.device, lib.fra_linear_backward, C.byref(d), z.data_ptr() if z is not None else None,
-                              g.data_ptr(), lddy, dx.data_ptr() if need[0] else None, dw.data_ptr() if need[1] else None,
-                              db.data_ptr() if need[2] else None, ds.data_ptr() if need[3] else None,
-                              ws.data_ptr(), nbytes.value, _stream(x.device)), "fra_linear_backward")
-    return dx, dw, db, ds, (dy if need[4] else None), None, None
+        _lib.check(_on_device(device, lib.fra_linear_backward, C.byref(d), z.data_ptr() if z is not None else None,
+                              g.data_ptr(), lddy, dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                              db.data_ptr() if need_b else None, ds.data_ptr() if need_s else None,
+                              ws.data_ptr(), nbytes.value, _stream(device)), "fra_linear_backward")
+    return dx, dw, db, ds, (dy if need_r else None), None, None
 
 
 class _Linear(torch.autograd.Function):
