@@ -91,9 +91,9 @@ SIGNATURES = {
     "fra_group_tiles": (_I, [_L, _I]),
     "fra_group_rows_workspace_bytes": (_I, [_L, _I, C.POINTER(C.c_size_t)]),
     "fra_group_rows": (_I, [_P, _I, C.POINTER(RowGroupsDesc), _P, C.c_size_t, _P]),
-    "fra_linear": (_I, [C.POINTER(LinearDesc), _P, _P, _P]),
-    "fra_linear_backward_workspace_bytes": (_I, [C.POINTER(LinearDesc), _I, _I, _I, _I, C.POINTER(C.c_size_t)]),
-    "fra_linear_backward": (_I, [C.POINTER(LinearDesc), _P, _P, _L, _P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "fra_linear": (_I, [_P, _P, _P, _P]),
+    "fra_linear_backward_workspace_bytes": (_I, [_P, _I, _I, _I, _I, C.POINTER(C.c_size_t)]),
+    "fra_linear_backward": (_I, [_P, _P, _P, _L, _P, _P, _P, _P, _P, C.c_size_t, _P]),
     "fra_orthogonalize_workspace_bytes": (_I, [_L, _I, _I, C.POINTER(C.c_size_t)]),
     "fra_orthogonalize": (_I, [_I, _P, _L, _L, _L, _I, _I, _I, C.c_float, C.c_float, C.c_float, _P, _P, C.c_size_t, _P]),
     "fa_align_warp": (_I, [_P, _I, _I, _P, _I, _P, _I, _I, _P]),

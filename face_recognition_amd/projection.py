@@ -17,6 +17,7 @@ captured into a graph.  Capture a backward pass as ``torch.autograd.grad`` on le
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from functools import lru_cache
 from typing import Optional
 
@@ -65,14 +66,14 @@ class RowGroups:
     call ``groups.order.record_stream(stream)`` (all its parts are one allocation).
     """
 
-    def __init__(self, rows: int, n_groups: int, ids: torch.Tensor):
+    def __init__(self, rows: int, n_groups: int, ids: torch.Tensor, tile_rows: int, n_tiles: int):
         self.rows, self.n_groups, self.device = rows, n_groups, ids.device
-        tile_rows, n_tiles, _ = _group_sizes(rows, n_groups)
         # one allocation: tiles (16-byte aligned) | order | offsets | tile_offsets
         self._buf = ids.new_empty(4 * n_tiles + rows + 2 * n_groups + 3, dtype=torch.int32)
         base, at = self._buf.data_ptr(), 4 * n_tiles
         self._desc = _lib.RowGroupsDesc(rows, n_groups, tile_rows, n_tiles, base + 4 * at, base + 4 * (at + rows), base,
                                         base + 4 * (at + rows + n_groups + 1))
+        self._address = C.addressof(self._desc)
 
     @property
     def order(self) -> torch.Tensor:
@@ -96,12 +97,16 @@ def group_rows(ids: torch.Tensor, n_groups: int) -> RowGroups:
         raise RuntimeError(f"group_rows: {n_groups} groups (1 to {MAX_GROUPS})")
     ids = ids.contiguous()
     rows = ids.shape[0]
-    need = _group_sizes(rows, n_groups)[2]
-    g = RowGroups(rows, n_groups, ids)
+    tile_rows, n_tiles, need = _group_sizes(rows, n_groups)
+    g = RowGroups(rows, n_groups, ids, tile_rows, n_tiles)
     ws = ids.new_empty(need, dtype=torch.uint8) if need else None
-    _lib.check(_on_device(ids.device, _lib.load().fra_group_rows, ids.data_ptr(), ids.dtype == torch.int64, C.byref(g._desc),
-                          ws.data_ptr() if need else None, need, _stream(ids.device)), "fra_group_rows")
+    _lib.check(_on_device(g.device, _lib.load().fra_group_rows, ids.data_ptr(), ids.dtype == torch.int64, C.byref(g._desc),
+                          ws.data_ptr() if need else None, need, _stream(g.device)), "fra_group_rows")
     return g
+
+
+# a _lib.LinearDesc as bytes, in C's layout: filling a ctypes structure costs 1 us more
+_DESC = struct.Struct("@4iq2i5P4qP")
 
 
 def _rows(t: torch.Tensor, r: int, c: int):
@@ -125,8 +130,8 @@ def _weight(weight: torch.Tensor, n: int, k: int):
 
 
 def _forward(x, weight, bias, slope, residual, act, groups, want_preact):
-    """(out, preact, descriptor, (x, weight, slope) as the kernels read them).  Sizes are taken apart once, and `new_empty` gets
-    plain numbers: a shape costs 1 us more."""
+    """(out, preact, the descriptor's types and sizes, (x, weight, slope) as the kernels read them).  Sizes are taken apart once, and
+    `new_empty` gets plain numbers: a shape costs 1 us more."""
     m, k = x.shape
     n = weight.shape[-2]
     dt = _DTYPES[x.dtype]
@@ -141,15 +146,15 @@ def _forward(x, weight, bias, slope, residual, act, groups, want_preact):
         slope = slope.contiguous()
     out = x.new_empty(m, n)
     z = torch.empty_like(out) if want_preact else None
-    d = _lib.LinearDesc(dt, act, _DTYPES[bias.dtype] if bias is not None else 0, _DTYPES[slope.dtype] if slope is not None else 0,
-                        m, k, n, x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
-                        slope.data_ptr() if slope is not None else None, residual.data_ptr() if residual is not None else None,
-                        ldx, ldw, ldr, wg, C.pointer(groups._desc) if groups is not None else None)
+    sizes = (dt, act, _DTYPES[bias.dtype] if bias is not None else 0, _DTYPES[slope.dtype] if slope is not None else 0, m, k, n)
+    d = _DESC.pack(*sizes, x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else 0,
+                   slope.data_ptr() if slope is not None else 0, residual.data_ptr() if residual is not None else 0,
+                   ldx, ldw, ldr, wg, groups._address if groups is not None else 0)
     if m:
         device = x.device
-        _lib.check(_on_device(device, _lib.load().fra_linear, C.byref(d), z.data_ptr() if z is not None else None,
+        _lib.check(_on_device(device, _lib.load().fra_linear, d, z.data_ptr() if z is not None else None,
                               out.data_ptr(), _stream(device)), "fra_linear")
-    return out, z, d, (x, weight, slope)
+    return out, z, sizes, (x, weight, slope)
 
 
 def _backward(ctx, dy):
@@ -157,8 +162,8 @@ def _backward(ctx, dy):
     dx = dw = db = ds = None
     if need_x or need_w or need_b or need_s:
         x, weight, slope, z = ctx.saved_tensors
-        d, groups = ctx.desc, ctx.groups
-        m, k, n = d.M, d.K, d.N
+        sizes, groups = ctx.sizes, ctx.groups
+        m, k, n = sizes[4:]
         lead = (groups.n_groups,) if groups is not None else ()
         if need_x:
             dx = x.new_empty(m, k)
@@ -169,20 +174,20 @@ def _backward(ctx, dy):
         if need_s:
             ds = x.new_empty(*lead, n, dtype=slope.dtype)
         # saved-tensor hooks may bring back other tensors, or the same memory laid out otherwise
-        x, d.ldx = _rows(x, m, k)
-        weight, d.ldw, d.w_group_stride = _weight(weight, n, k)
-        d.x, d.w = x.data_ptr(), weight.data_ptr()
+        x, ldx = _rows(x, m, k)
+        weight, ldw, wg = _weight(weight, n, k)
         if slope is not None:
             slope = slope.contiguous()
-            d.slope = slope.data_ptr()
         if z is not None:
             z = z.contiguous()
-        lib, device, nbytes = _lib.load(), x.device, C.c_size_t()
         g, lddy = _rows(dy, m, n)
-        _lib.check(lib.fra_linear_backward_workspace_bytes(C.byref(d), need_x, need_w, need_b, need_s, C.byref(nbytes)),
+        d = _DESC.pack(*sizes, x.data_ptr(), weight.data_ptr(), 0, slope.data_ptr() if slope is not None else 0, 0, ldx, ldw, 0, wg,
+                       groups._address if groups is not None else 0)
+        lib, device, nbytes = _lib.load(), x.device, C.c_size_t()
+        _lib.check(lib.fra_linear_backward_workspace_bytes(d, need_x, need_w, need_b, need_s, C.byref(nbytes)),
                    "fra_linear_backward_workspace_bytes")
         ws = x.new_empty(nbytes.value, dtype=torch.uint8)
-        _lib.check(_on_device(device, lib.fra_linear_backward, C.byref(d), z.data_ptr() if z is not None else None,
+        _lib.check(_on_device(device, lib.fra_linear_backward, d, z.data_ptr() if z is not None else None,
                               g.data_ptr(), lddy, dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
                               db.data_ptr() if need_b else None, ds.data_ptr() if need_s else None,
                               ws.data_ptr(), nbytes.value, _stream(device)), "fra_linear_backward")
@@ -193,10 +198,10 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, slope, residual, act, groups):
         need = ctx.needs_input_grad
-        out, z, d, kept = _forward(x, weight, bias, slope, residual, act, groups,
-                                   act != 0 and (need[0] or need[1] or need[2] or need[3]))
+        out, z, sizes, kept = _forward(x, weight, bias, slope, residual, act, groups,
+                                       act != 0 and (need[0] or need[1] or need[2] or need[3]))
         ctx.save_for_backward(*kept, z)
-        ctx.desc, ctx.groups = d, groups
+        ctx.sizes, ctx.groups = sizes, groups
         ctx.bias_dtype = bias.dtype if bias is not None else None
         return out
 
@@ -251,9 +256,9 @@ def _check(what, x, weight, bias, activation, slope, residual, lead):
 
 
 def _apply(x, weight, bias, slope, residual, act, groups):
-    if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-            or (slope is not None and slope.requires_grad) or (residual is not None and residual.requires_grad)) \
-            and torch.is_grad_enabled() or forward_ad._current_level >= 0:      # torch refuses a tangent there; it would be lost below
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (slope is not None and slope.requires_grad) or (residual is not None and residual.requires_grad)) \
+            or forward_ad._current_level >= 0:      # torch refuses a tangent there; it would be lost below
         return _Linear.apply(x, weight, bias, slope, residual, act, groups)
     return _forward(x, weight, bias, slope, residual, act, groups, False)[0]
 

@@ -134,3 +134,10 @@ def test_more_threads_than_a_launch_takes():
     g = _lib.RowGroupsDesc(8, 4096, lib.fra_group_tile_rows(8, 4096), lib.fra_group_tiles(8, 4096), 64, 64, 64, 64)
     d = desc(M=8, N=1 << 16, groups=C.pointer(g))                   # 4097 row tiles x 4096 column tiles of 512 threads
     assert lib.fra_linear(C.byref(d), None, 64, None) == 1 and b"launch" in lib.fra_last_error()
+
+
+def test_packed_descriptor_is_the_structure():
+    values = (1, 2, 3, 4, 5 << 40, 6, 7, 8 << 40, 9 << 40, 10 << 40, 11 << 40, 12 << 40, 13 << 40, 14 << 40, 15 << 40, 16 << 40, 0)
+    d = _lib.LinearDesc.from_buffer_copy(projection._DESC.pack(*values))
+    assert projection._DESC.size == C.sizeof(_lib.LinearDesc) and not d.groups
+    assert tuple(getattr(d, name) for name, _ in d._fields_[:-1]) == values[:-1]
