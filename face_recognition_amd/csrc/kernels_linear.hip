@@ -56,7 +56,6 @@ template <typename T> __device__ __forceinline__ float pj_act_grad(int act, floa
 struct RowArgs {
     const int* order;           // nullptr: the rows themselves
     const int4* tiles;          // (group, first list entry, end, -) per row tile; nullptr: one group, tiles of BI rows
-    const int* offsets;         // [G + 1] list entries of a group (grouped only)
     const int* tile_offsets;    // [G + 2], the last one the number of tiles in use (grouped only)
     int n_tiles, M, G;
     int sub;                    // tiles a table entry is cut into (a kernel's tiles may be shorter than the table's)
@@ -886,7 +885,6 @@ static RowArgs row_args(const fra_linear_desc* d, int tile_rows) {
     const fra_row_groups* g = d->groups;
     r.order = g ? g->order : nullptr;
     r.tiles = g ? (const int4*)g->tiles : nullptr;
-    r.offsets = g ? g->offsets : nullptr;
     r.tile_offsets = g ? g->tile_offsets : nullptr;
     r.sub = g && g->tile_rows > tile_rows ? g->tile_rows / tile_rows : 1;
     r.n_tiles = g ? g->n_tiles * r.sub : cdiv(d->M, tile_rows);
@@ -940,8 +938,8 @@ template <typename T> static int forward_t(const fra_linear_desc* d, void* z, vo
     FwdArgs a;
     // Few rows, or so few columns that tiles would be empty, have a kernel of their own.  (Its sums are in another order, so beyond 64
     // rows a value does not depend on the number of rows beside it: there the columns alone decide.)  Columns: up to 16, the kernel's
-    // own (262144 x 16 x 512 bf16 53 us, on tiles 116; fp32 125 and 289).  Rows: fp32 up to 64 (64 x 40961 x 512 66 us, on tiles 76).
-    // 16 bits up to 16 (1 x 40961 x 512 11.8 and 14.2), and up to 64 by what a compute unit fetches, in rows of k: this kernel's tiles
+    // own, as far as its launch goes (262144 x 16 x 512 bf16 53 us, on tiles 116; fp32 125 and 289).  Rows: fp32 up to 64 (64 x 40961
+    // x 512 66 us, on tiles 76), 16 bits up to 16 (1 x 40961 x 512 11.8 and 14.2), and up to 64 by what a compute unit fetches, in rows of k: this kernel's tiles
     // are smaller, the others' read a wide product's operands less often (50 x 333 x 512 3.4 us, on tiles 5.2; 64 x 4096 x 2048 13.0
     // and 10.4).  What DMA cannot take stays longer in the tiles' steps, for which it gets two rows of sixteen in advance.
     const int most = d->groups ? d->groups->tile_rows : 256, side = tile_side(d->M, d->N, sizeof(T) == 4, most);
@@ -949,7 +947,7 @@ template <typename T> static int forward_t(const fra_linear_desc* d, void* z, vo
     int mt = 1;                                                     // tiles of 16 rows: as many as fetch least
     for (int i = 2; i <= 4; i *= 2)
         if (16 * i <= most && fetched(16 * i, 16) < fetched(16 * mt, 16)) mt = i;
-    const bool few = most == 16 || d->N <= 16 || d->M <= (sizeof(T) == 4 ? 64 : 16) ||
+    const bool few = most == 16 || (d->N <= 16 && d->M <= 1 << 28) || d->M <= (sizeof(T) == 4 ? 64 : 16) ||
                      (d->M <= 64 && fetched(16 * mt, 16) < fetched(side, side) + (forward_dma<T>(d) ? 0 : 2));
     const int bi = few ? 16 * mt : side;
     a.rows = row_args(d, bi);

@@ -89,11 +89,6 @@ template <typename T> __device__ __forceinline__ void store_four(T* p, int n, co
             if (e < n) p[e] = (T)v[e];
     }
 }
-// a parameter vector that is float or of the product's own type
-template <typename T> __device__ __forceinline__ void load_param4(const void* p, bool is_f32, int64_t at, int n, float (&o)[4]) {
-    if (is_f32) load_four<float>(reinterpret_cast<const float*>(p) + at, n, o);
-    else load_four<T>(reinterpret_cast<const T*>(p) + at, n, o);
-}
 
 template <int KS> __device__ __forceinline__ int swz_row_major(int row, int c) { return KS == 2 ? c ^ (row & 7) : c ^ ((row >> 1) & 3); }
 template <typename T, int CPR> __device__ __forceinline__ int swz_k_major(int k, int c) {

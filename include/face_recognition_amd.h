@@ -295,9 +295,11 @@ int fa_align_warp(const uint8_t* frame, int H, int W, const double* matrices, in
  *
  *     z = x w^T + bias;   out = act(z) + resid          x [M,K], w [N,K], bias / slope [N], resid / out [M,N]
  *
- * Any M >= 0, K, N >= 1 up to 2^24.  dtype is the type of x, w, resid, preact, out and their gradients; bias and slope are of
- * that type or fp32.  Sums are fp32 (fp32 products on the fp32 matrix instructions).  Rows are contiguous, at a pitch of ldx /
- * ldw / ldr elements; any element alignment works, 16-byte aligned rows are the fast ones.  Results do not depend on timing.
+ * Any M >= 0, K, N >= 1 up to 2^24, as far as one launch's 2^32 threads go (10^9 rows of 64 columns do).  dtype is the type of x,
+ * w, resid, preact, out and their gradients; bias and slope are of that type or fp32.  Sums are fp32 (fp32 products on the fp32
+ * matrix instructions).  Rows are contiguous, at a pitch of ldx / ldw / ldr elements; any element alignment works, 16-byte aligned
+ * rows are the fast ones.  Results do not depend on timing, nor, beyond 64 rows, a row's on the number of rows beside it (without
+ * groups).
  * Nothing here allocates; scratch is the caller's, 16-byte aligned. */
 enum fra_activation {
     FRA_ACT_NONE = 0, FRA_ACT_RELU = 1,
