@@ -309,6 +309,80 @@ template <typename T, bool BK, bool LAST, typename S, bool TOGETHER> __global__ 
     }
 }
 
+// ---- C = C^T (X X^T, and P P for a symmetric P): the lower triangle's tiles, each handed on to both sides of the diagonal
+
+// hands the transposed results on: f as tile_emit's, whose rows are the tile's columns.  A wave's part, 32 of its rows at a time, goes
+// through its own LDS as [column][row].
+template <typename S, int LDS, typename F> __device__ __forceinline__ void mirror_emit(const f32x4 (&acc)[S::MI][S::MJ], char* lds, const F& f) {
+    constexpr int MG = S::MI < 2 ? S::MI : 2, V = 8, ROWS = MG * 16, LPR = ROWS / V, RPP = 64 / LPR, PITCH = ROWS + 4;
+    static_assert(S::WI * S::WJ * S::MJ * 16 * PITCH * 4 <= LDS && S::MI % MG == 0 && (S::MJ * 16) % RPP == 0, "the waves' parts fit");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wi = (wave % S::WI) * (S::BI / S::WI), wj = (wave / S::WI) * (S::BJ / S::WJ);
+    float* strip = reinterpret_cast<float*>(lds) + wave * (S::MJ * 16 * PITCH);
+#pragma unroll
+    for (int m0 = 0; m0 < S::MI; m0 += MG) {
+#pragma unroll
+        for (int mi = 0; mi < MG; ++mi)
+#pragma unroll
+            for (int mj = 0; mj < S::MJ; ++mj)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) strip[(16 * mj + 4 * (lane >> 4) + e) * PITCH + 16 * mi + (lane & 15)] = acc[m0 + mi][mj][e];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int jl = 0; jl < S::MJ * 16; jl += RPP) {
+            const int jr = jl + lane / LPR, il = (lane % LPR) * V, row = f.row(wj + jr), col = wi + 16 * m0 + il;
+            const typename F::Pre pre = f.pre(row, col);
+            float v[V];
+#pragma unroll
+            for (int q = 0; q < V; q += 4) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(strip + jr * PITCH + il + q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[q + e] = x[e];
+            }
+            f.emit(row, col, pre, v);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+template <typename S, int LDS> __device__ __forceinline__ void symmetric_tile(const OrthArgs& a, int64_t b, int i0, int j0, char* lds) {
+    f32x4 acc[S::MI][S::MJ];
+    PairProduct<false, S, true> p;
+    p.A.order = p.B.order = nullptr; p.A.ld = a.lda; p.B.ld = a.ldb; p.A.klen = p.B.klen = a.K; p.A.cols = p.B.cols = 0;
+    p.A.row0 = i0; p.A.rows = a.I - i0; p.A.base = a.ah + b * a.sa;
+    p.B.row0 = j0; p.B.rows = a.J - j0; p.B.base = a.bh + b * a.sb;
+    p.a_lo = a.al - a.ah; p.b_lo = a.bl - a.bh;
+    p.run(a.K, lds, acc);
+    tile_emit<f16, S>(acc, lds, OrthEmit<f16>{a, b, i0, j0});
+    if (i0 == j0) return;
+    __syncthreads();                                                // another wave's part of LDS lies elsewhere now
+    mirror_emit<S, LDS>(acc, lds, OrthEmit<f16>{a, b, j0, i0});
+}
+// A die takes consecutive tiles (of one matrix, or of neighbours).  `big` of them are 128 x 128, full rounds of one per compute
+// unit; the rest would leave most units idle for a whole round and are cut into four, of 64 x 64.
+typedef Shape<128, 128, 4, 2, 2, 2> SymBig;
+typedef Shape<64, 64, 4, 2, 2, 2> SymQuarter;
+__global__ __launch_bounds__(SymBig::NT) void orth_symmetric_kernel(OrthArgs a, int side, int big) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int LDS = PairProduct<false, SymBig, true>::LDS;
+    static_assert(PairProduct<false, SymQuarter, true>::LDS <= LDS && SymQuarter::NT == SymBig::NT, "");
+    const int each = side * (side + 1) / 2, all = each * a.batch, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+    const int first = (int)((int64_t)all * x / 8), count = (int)((int64_t)all * (x + 1) / 8) - first;
+    const int n_big = count < big ? count : big, at = i < n_big ? i : n_big + ((i - n_big) >> 2), quarter = (i - n_big) & 3;
+    if (at >= count) return;
+    const int mat = (first + at) / each, t = first + at - mat * each;
+    int r = (int)((__builtin_sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);       // the last r with r (r + 1) / 2 <= t
+    while (r > 0 && r * (r + 1) / 2 > t) --r;
+    while ((r + 1) * (r + 2) / 2 <= t) ++r;
+    const int i0 = r * 128, j0 = (t - r * (r + 1) / 2) * 128;
+    if (i < n_big) {
+        symmetric_tile<SymBig, LDS>(a, mat, i0, j0, lds);
+    } else {
+        const int qi = i0 + (quarter >> 1) * 64, qj = j0 + (quarter & 1) * 64;
+        if (qi < qj || qi >= a.I) return;                           // above the diagonal, or past the last row (columns are no more)
+        symmetric_tile<SymQuarter, LDS>(a, mat, qi, qj, lds);
+    }
+}
+
 typedef Shape<256, 256, 2, 4, 2, 2> OrthHuge;       // three products in a chain
 typedef Shape<128, 128, 4, 2, 2, 2> OrthBig;
 typedef Shape<64, 64, 2, 2, 2, 2> OrthSmall;
@@ -329,8 +403,40 @@ template <typename T, bool BK, bool LAST, typename S, bool TOGETHER> static int 
 }
 // rounds of one workgroup per compute unit that are at least nine tenths full
 static bool full_rounds(int64_t tiles) { return tiles >= 230 && tiles * 10 >= (tiles + 255) / 256 * 256 * 9; }
+// How long a product takes, in rounds of 128 x 128 tiles: a round of 256 x 256 is 3.3 of them, one of 64 x 64 beside the others 0.35
+struct SymPlan {
+    int side, big, per_die;         // tiles along a side, 128 x 128 tiles and workgroups of a die; per_die 0: not worth it
+};
+static SymPlan symmetric_plan(int m, int batch) {
+    SymPlan p = {(m + 127) / 128, 0, 0};
+    const int64_t all = (int64_t)p.side * (p.side + 1) / 2 * batch, square = (int64_t)p.side * p.side * batch;
+    const int64_t rounds = all / 256, rest = all - rounds * 256;
+    if (rounds < 1 || all > (1 << 28)) return p;
+    const double lower = rounds + (rest == 0 ? 0.0 : rest <= 64 ? 0.35 : rest <= 128 ? 0.7 : 1.0);
+    const int64_t huge = (int64_t)((m + 255) / 256) * ((m + 255) / 256) * batch;
+    const double whole = full_rounds(huge) ? 3.3 * ((huge + 255) / 256) : (double)((square + 255) / 256);
+    if (lower > 0.85 * whole) return p;
+    const int most = (int)((all + 7) / 8);                          // a die's
+    p.big = rest > 128 ? most : (int)rounds * 32;
+    p.per_die = most <= p.big ? most : p.big + 4 * (most - p.big);
+    return p;
+}
+static int product_symmetric(OrthArgs& a, const SymPlan& p, int batch, hipStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    const int lds = PairProduct<false, SymBig, true>::LDS;
+    if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(orth_symmetric_kernel), lds, done)) return rc;
+    a.batch = batch;
+    FRA_REQUIRE((int64_t)p.per_die * 8 <= 4294967295LL / SymBig::NT, FRA_ERR_ARG, "fra_orthogonalize: %d workgroups of a die", p.per_die);
+    hipLaunchKernelGGL(orth_symmetric_kernel, dim3((unsigned)p.per_die * 8), dim3(SymBig::NT), lds, s, a, p.side, p.big);
+    FRA_HIP(hipGetLastError());
+    return FRA_OK;
+}
 template <typename T, bool BK, bool LAST> static int product(OrthArgs& a, int batch, hipStream_t s) {
     auto tiles = [&](int64_t bi, int64_t bj) { return (a.I + bi - 1) / bi * ((a.Jp + bj - 1) / bj) * batch; };
+    if constexpr (!BK) {                                            // X X^T and P P
+        const SymPlan p = symmetric_plan(a.I, batch);
+        if (p.per_die) return product_symmetric(a, p, batch, s);
+    }
     if (full_rounds(tiles(256, 256))) return launch_orth<T, BK, LAST, OrthHuge, false>(a, batch, s);
     if (tiles(128, 128) >= 192) return launch_orth<T, BK, LAST, OrthBig, true>(a, batch, s);
     if (tiles(64, 64) >= 192) return launch_orth<T, BK, LAST, OrthSmall, true>(a, batch, s);

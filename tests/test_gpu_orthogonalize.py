@@ -195,3 +195,22 @@ def test_large_batches(device, shape, dt):
         err = torch.linalg.matrix_norm(y[i].double() - want).item()
         assert err <= allowed([1.0], want, USUAL, dt)
         assert (y[i].double() - want).abs().max() <= 2.0 ** -7 * want.abs().max()       # no value out of place
+
+
+# X X^T and P P by the lower triangle: whole tiles with quarters of others behind them (some past the last row), whole tiles only,
+# several rounds; every matrix of the batch
+@pytest.mark.parametrize("shape", [(8, 1024, 1024), (20, 520, 600), (20, 600, 520), (9, 1000, 1100), (60, 321, 330), (2, 2048, 2100), (3, 1930, 1930)], ids=str)
+def test_products_by_the_lower_triangle(device, shape):
+    g = matrix(shape, torch.float32, device, 4)
+    a, b, c = USUAL
+    y = projection.orthogonalize(g, steps=1)
+    for i in range(shape[0]):
+        x = g[i].double()
+        x = x / torch.linalg.matrix_norm(x)
+        tall = x.shape[0] > x.shape[1]
+        x = x.mT if tall else x
+        p = x @ x.mT
+        want = a * x + (b * p + c * (p @ p)) @ x
+        want = want.mT if tall else want
+        assert torch.linalg.matrix_norm(y[i].double() - want).item() <= allowed([1.0], want, USUAL, torch.float32)
+        assert (y[i].double() - want).abs().max() <= 2.0 ** -12 * want.abs().max()      # no value out of place
