@@ -9,10 +9,9 @@
 // over three times that of the fp32 matrix instructions.  Against 64 bits the results are as near as the same iteration with
 // fp32 products (512 x 512: 1.4e-6 of the norm, fp32 2.1e-6).
 //
-// 17 launches for five steps.  Small matrices are bound by the launches' latency (512 x 512 fp32 107 us, 6.1 us each), large ones by
-// the matrix cores: eight of 2048 x 1024 1.27 ms (1.0 PFLOP/s of f16 products), one of 4096 x 4096 4.9 ms (1.25).  P and Q are
-// symmetric, which is not used: with tiles of 128 the lower half of 1024 x 1024 is 36 of 64 tiles, for a batch of eight 288 on 256
-// compute units, two rounds like all 512.
+// 17 launches for five steps.  Small matrices are bound by the launches' latency (512 x 512 fp32 104 us, 6 us each), large ones by
+// the matrix cores: eight of 2048 x 1024 1.09 ms, one of 4096 x 4096 3.9 ms.  P and Q are symmetric: where that saves rounds of
+// workgroups, only the tiles of the lower triangle are computed (1.27 and 4.9 ms with all of them).
 #include "pj_tile.h"
 
 namespace fra {
@@ -357,35 +356,34 @@ template <typename S, int LDS> __device__ __forceinline__ void symmetric_tile(co
     __syncthreads();                                                // another wave's part of LDS lies elsewhere now
     mirror_emit<S, LDS>(acc, lds, OrthEmit<f16>{a, b, j0, i0});
 }
-// A die takes consecutive tiles (of one matrix, or of neighbours).  `big` of them are 128 x 128, full rounds of one per compute
-// unit; the rest would leave most units idle for a whole round and are cut into four, of 64 x 64.
-typedef Shape<128, 128, 4, 2, 2, 2> SymBig;
-typedef Shape<64, 64, 4, 2, 2, 2> SymQuarter;
-__global__ __launch_bounds__(SymBig::NT) void orth_symmetric_kernel(OrthArgs a, int side, int big) {
+typedef Shape<128, 128, 4, 2, 2, 2> OrthBig;
+typedef Shape<64, 64, 2, 2, 2, 2> OrthSmall;
+typedef Shape<64, 64, 4, 2, 2, 2> OrthQuarter;      // of an OrthBig tile, by as many threads
+// A die takes consecutive tiles (of one matrix, or of neighbours).  `whole` of them are W's, full rounds of one per compute unit; the
+// rest would leave most units idle for a whole round and are cut into four (of 128 x 128 only).
+template <typename W> __global__ __launch_bounds__(W::NT) void orth_symmetric_kernel(OrthArgs a, int side, int whole) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int LDS = PairProduct<false, SymBig, true>::LDS;
-    static_assert(PairProduct<false, SymQuarter, true>::LDS <= LDS && SymQuarter::NT == SymBig::NT, "");
+    constexpr int LDS = PairProduct<false, W, true>::LDS;
     const int each = side * (side + 1) / 2, all = each * a.batch, x = blockIdx.x & 7, i = blockIdx.x >> 3;
     const int first = (int)((int64_t)all * x / 8), count = (int)((int64_t)all * (x + 1) / 8) - first;
-    const int n_big = count < big ? count : big, at = i < n_big ? i : n_big + ((i - n_big) >> 2), quarter = (i - n_big) & 3;
+    const int n_whole = count < whole ? count : whole, at = i < n_whole ? i : n_whole + ((i - n_whole) >> 2), quarter = (i - n_whole) & 3;
     if (at >= count) return;
     const int mat = (first + at) / each, t = first + at - mat * each;
     int r = (int)((__builtin_sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);       // the last r with r (r + 1) / 2 <= t
     while (r > 0 && r * (r + 1) / 2 > t) --r;
     while ((r + 1) * (r + 2) / 2 <= t) ++r;
-    const int i0 = r * 128, j0 = (t - r * (r + 1) / 2) * 128;
-    if (i < n_big) {
-        symmetric_tile<SymBig, LDS>(a, mat, i0, j0, lds);
-    } else {
+    const int i0 = r * W::BI, j0 = (t - r * (r + 1) / 2) * W::BI;
+    if (i < n_whole) {
+        symmetric_tile<W, LDS>(a, mat, i0, j0, lds);
+    } else if constexpr (W::BI == 128) {
+        static_assert(PairProduct<false, OrthQuarter, true>::LDS <= LDS && OrthQuarter::NT == W::NT, "");
         const int qi = i0 + (quarter >> 1) * 64, qj = j0 + (quarter & 1) * 64;
         if (qi < qj || qi >= a.I) return;                           // above the diagonal, or past the last row (columns are no more)
-        symmetric_tile<SymQuarter, LDS>(a, mat, qi, qj, lds);
+        symmetric_tile<OrthQuarter, LDS>(a, mat, qi, qj, lds);
     }
 }
 
 typedef Shape<256, 256, 2, 4, 2, 2> OrthHuge;       // three products in a chain
-typedef Shape<128, 128, 4, 2, 2, 2> OrthBig;
-typedef Shape<64, 64, 2, 2, 2, 2> OrthSmall;
 typedef Shape<32, 32, 2, 1, 2, 3> OrthTiny;
 
 template <typename T, bool BK, bool LAST, typename S, bool TOGETHER> static int launch_orth(OrthArgs& a, int batch, hipStream_t s) {
@@ -403,31 +401,38 @@ template <typename T, bool BK, bool LAST, typename S, bool TOGETHER> static int 
 }
 // rounds of one workgroup per compute unit that are at least nine tenths full
 static bool full_rounds(int64_t tiles) { return tiles >= 230 && tiles * 10 >= (tiles + 255) / 256 * 256 * 9; }
-// How long a product takes, in rounds of 128 x 128 tiles: a round of 256 x 256 is 3.3 of them, one of 64 x 64 beside the others 0.35
+// Whether the lower triangle is worth it.  How long a product takes, in rounds of 128 x 128 tiles: a round of 256 x 256 is 3.3 of
+// them; one of 64 x 64 on a unit 0.35, two 0.6 (eight of 1024 x 1024: P from X of 2048 columns 117 -> 81 us, Q 57 -> 47; a matrix
+// of 1500 x 1500 665 -> 466 us for all steps; 24 of 512 x 512 456 -> 369).  Asked
+// to be a sixth less, except against the same tiles (four of 700 x 700 220 -> 211).
 struct SymPlan {
-    int side, big, per_die;         // tiles along a side, 128 x 128 tiles and workgroups of a die; per_die 0: not worth it
+    int tile, side, whole, per_die;     // tile: 128 or 64, 0: not worth it; tiles along a side; whole tiles and workgroups of a die
 };
-static SymPlan symmetric_plan(int m, int batch) {
-    SymPlan p = {(m + 127) / 128, 0, 0};
-    const int64_t all = (int64_t)p.side * (p.side + 1) / 2 * batch, square = (int64_t)p.side * p.side * batch;
-    const int64_t rounds = all / 256, rest = all - rounds * 256;
-    if (rounds < 1 || all > (1 << 28)) return p;
-    const double lower = rounds + (rest == 0 ? 0.0 : rest <= 64 ? 0.35 : rest <= 128 ? 0.7 : 1.0);
-    const int64_t huge = (int64_t)((m + 255) / 256) * ((m + 255) / 256) * batch;
-    const double whole = full_rounds(huge) ? 3.3 * ((huge + 255) / 256) : (double)((square + 255) / 256);
-    if (lower > 0.85 * whole) return p;
-    const int most = (int)((all + 7) / 8);                          // a die's
-    p.big = rest > 128 ? most : (int)rounds * 32;
-    p.per_die = most <= p.big ? most : p.big + 4 * (most - p.big);
+static SymPlan symmetric_plan(int m, int64_t batch) {
+    auto sides = [&](int tile) { return (int64_t)((m + tile - 1) / tile); };
+    auto square = [&](int tile) { return sides(tile) * sides(tile) * batch; };
+    auto lower = [&](int tile) { return sides(tile) * (sides(tile) + 1) / 2 * batch; };
+    auto small = [](int64_t tiles) { return tiles <= 256 ? 0.35 : 0.6 * ((tiles + 511) / 512); };
+    const bool now64 = !full_rounds(square(256)) && square(128) < 192;
+    const double now = now64 ? small(square(64)) : full_rounds(square(256)) ? 3.3 * ((square(256) + 255) / 256) : (double)((square(128) + 255) / 256);
+    const int64_t rounds = lower(128) / 256, rest = lower(128) % 256;
+    const double by128 = rounds + (rest == 0 ? 0.0 : rest <= 64 ? 0.35 : rest <= 128 ? 0.7 : 1.0), by64 = small(lower(64));
+    SymPlan p = {0, 0, 0, 0};
+    if (lower(64) > 1 << 28 || (by128 > 0.85 * now && (now64 ? square(64) <= 256 : by64 > 0.85 * now))) return p;
+    p.tile = by64 <= by128 ? 64 : 128;
+    p.side = (int)sides(p.tile);
+    const int most = (int)((lower(p.tile) + 7) / 8);                // a die's
+    p.whole = p.tile == 64 || rest > 128 ? most : (int)rounds * 32;
+    p.per_die = most <= p.whole ? most : p.whole + 4 * (most - p.whole);
     return p;
 }
-static int product_symmetric(OrthArgs& a, const SymPlan& p, int batch, hipStream_t s) {
+template <typename W> static int launch_symmetric(OrthArgs& a, const SymPlan& p, int batch, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
-    const int lds = PairProduct<false, SymBig, true>::LDS;
-    if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(orth_symmetric_kernel), lds, done)) return rc;
+    const int lds = PairProduct<false, W, true>::LDS;
+    if (int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(orth_symmetric_kernel<W>), lds, done)) return rc;
     a.batch = batch;
-    FRA_REQUIRE((int64_t)p.per_die * 8 <= 4294967295LL / SymBig::NT, FRA_ERR_ARG, "fra_orthogonalize: %d workgroups of a die", p.per_die);
-    hipLaunchKernelGGL(orth_symmetric_kernel, dim3((unsigned)p.per_die * 8), dim3(SymBig::NT), lds, s, a, p.side, p.big);
+    FRA_REQUIRE((int64_t)p.per_die * 8 <= 4294967295LL / W::NT, FRA_ERR_ARG, "fra_orthogonalize: %d workgroups of a die", p.per_die);
+    hipLaunchKernelGGL((orth_symmetric_kernel<W>), dim3((unsigned)p.per_die * 8), dim3(W::NT), lds, s, a, p.side, p.whole);
     FRA_HIP(hipGetLastError());
     return FRA_OK;
 }
@@ -435,7 +440,8 @@ template <typename T, bool BK, bool LAST> static int product(OrthArgs& a, int ba
     auto tiles = [&](int64_t bi, int64_t bj) { return (a.I + bi - 1) / bi * ((a.Jp + bj - 1) / bj) * batch; };
     if constexpr (!BK) {                                            // X X^T and P P
         const SymPlan p = symmetric_plan(a.I, batch);
-        if (p.per_die) return product_symmetric(a, p, batch, s);
+        if (p.tile == 128) return launch_symmetric<OrthBig>(a, p, batch, s);
+        if (p.tile == 64) return launch_symmetric<OrthSmall>(a, p, batch, s);
     }
     if (full_rounds(tiles(256, 256))) return launch_orth<T, BK, LAST, OrthHuge, false>(a, batch, s);
     if (tiles(128, 128) >= 192) return launch_orth<T, BK, LAST, OrthBig, true>(a, batch, s);

@@ -197,6 +197,11 @@ def test_large_batches(device, shape, dt):
         assert (y[i].double() - want).abs().max() <= 2.0 ** -7 * want.abs().max()       # no value out of place
 
 
+@pytest.mark.parametrize("shape", [(4, 700, 700), (24, 510, 512), (3, 900, 910), (1, 1500, 1530)], ids=str)
+def test_products_by_the_lower_triangle_in_small_tiles(device, shape):
+    test_products_by_the_lower_triangle(device, shape)
+
+
 # X X^T and P P by the lower triangle: whole tiles with quarters of others behind them (some past the last row), whole tiles only,
 # several rounds; every matrix of the batch
 @pytest.mark.parametrize("shape", [(8, 1024, 1024), (20, 520, 600), (20, 600, 520), (9, 1000, 1100), (60, 321, 330), (2, 2048, 2100), (3, 1930, 1930)], ids=str)
