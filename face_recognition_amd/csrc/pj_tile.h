@@ -100,12 +100,12 @@ template <typename T, int CPR> __device__ __forceinline__ int swz_k_major(int k,
 
 // 16 bytes per lane from global memory into LDS at `lds` + 16 lane, without passing through registers.  Written out (the
 // instruction has no register result) so that the compiler does not put a wait for it in front of every LDS read; the loops
-// that use it wait by count (dma_wait_barrier) before the barrier that publishes a tile.  m0 holds the LDS address; one wait
-// state lies between its write and the load.
+// that use it wait by count (dma_wait_barrier) before the barrier that publishes a tile.  m0 holds the LDS address (a clobber: the
+// compiler sets m0 for its own uses, and keeps it across what does not name it); one wait state lies between its write and the load.
 // The asm takes the LDS pointer itself: memory whose address never leaves the kernel's own loads counts as unwritten.
 typedef __attribute__((address_space(3))) char* LdsPtr;
 __device__ __forceinline__ void dma16(const void* g, LdsPtr lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "m0", "memory");
 }
 // at most N loads of this wave still on their way, all its LDS reads done; then the workgroup's barrier
 template <int N> __device__ __forceinline__ void dma_wait_barrier() {
