@@ -34,21 +34,22 @@ template <typename T> __device__ __forceinline__ float pj_act(int act, float z, 
         default: return z;
     }
 }
-template <typename T> __device__ __forceinline__ float pj_act_grad(int act, float z, float s) {
+// dy act'(z)
+template <typename T> __device__ __forceinline__ float pj_dz(int act, float dy, float z, float s) {
     switch (act) {
-        case PJ_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case PJ_PRELU: return z > 0.0f ? 1.0f : s;
+        case PJ_RELU: return z > 0.0f ? dy : 0.0f;                  // no product: an infinite dy does not reach what relu holds back
+        case PJ_PRELU: return z > 0.0f ? dy : dy * s;
         // beyond +-200 the sigmoid q is 0 or 1 exactly and the derivative with it; the other factors are held back there, so that
         // they meet the zero (of q or 1 - q) finite.  A NaN comes through q.
         case PJ_SILU: {
             const float q = pj_sigmoid2<T>(LOG2E * z), c = __builtin_amdgcn_fmed3f(z, -200.0f, 200.0f);
-            return q * (1.0f + c * (1.0f - q));
+            return dy * (q * (1.0f + c * (1.0f - q)));
         }
         case PJ_GELU_TANH: {
             const float q = pj_sigmoid2<T>(z * (LOG2E * GELU_C + LOG2E * GELU_C * GELU_A * (z * z))), c = __builtin_amdgcn_fmed3f(z, -200.0f, 200.0f);
-            return q * (1.0f + c * (1.0f - q) * (GELU_C + 3.0f * GELU_A * GELU_C * (c * c)));
+            return dy * (q * (1.0f + c * (1.0f - q) * (GELU_C + 3.0f * GELU_A * GELU_C * (c * c))));
         }
-        default: return 1.0f;
+        default: return dy;
     }
 }
 
@@ -452,7 +453,7 @@ template <typename T, int ACT, bool FULL> __device__ __forceinline__ void dz_row
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float y = (float)dy[u][e], zv = ACT != PJ_NONE ? (float)z[u][e] : 0.0f;
-                const float dz = ACT != PJ_NONE ? y * pj_act_grad<T>(ACT, zv, sl[e]) : y;
+                const float dz = pj_dz<T>(ACT, y, zv, sl[e]);
                 sb[e] += dz;
                 if (ACT == PJ_PRELU) ss[e] += zv > 0.0f ? 0.0f : y * zv;
                 if (ACT != PJ_NONE) d[e] = (T)dz;

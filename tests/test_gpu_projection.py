@@ -541,3 +541,20 @@ def test_rows_behind_two_to_the_31_elements(device, act):
     one = dict(t, w=t["w"][1], b=t["b"][1])
     plain = run(dict(one, **big), act)
     check({"y": plain["y"][-n_last:], "dx": plain["dx"][-n_last:], "dw": plain["dw"]}, reference(one, act))
+
+
+@pytest.mark.parametrize("m,k,n", [(40, 24, 33), (300, 64, 72)])
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_relu_holds_back_any_gradient(device, m, k, n, dt):
+    """Where relu's input is below zero its gradient is zero, whatever the output's is: infinities and NaN there change no bit."""
+    for groups in (0, 3):
+        lead = (groups,) if groups else ()
+        t = make(m, k, n, dt, device, 95 + groups, lead=lead, act="relu", residual=False)
+        rg = projection.group_rows(torch.arange(m, device=device) % groups, groups) if groups else None
+        base = run(t, "relu", rg)
+        off = base["y"].detach() == 0
+        spoil = torch.tensor([float("inf"), float("-inf"), float("nan")], dtype=dt, device=device)
+        dy = torch.where(off, spoil[torch.arange(m * n, device=device).view(m, n) % 3], t["dy"])
+        assert off.any() and not dy.isfinite().all()
+        for name, v in run(dict(t, dy=dy), "relu", rg).items():
+            assert torch.equal(v, base[name]), name
