@@ -297,24 +297,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, groups: RowGroups, bia
     return _apply(x, weight, bias, slope, residual, act, groups)
 
 
-def orthogonalize(matrix: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)) -> torch.Tensor:
-    """Newton-Schulz orthogonalisation of [..., rows, cols] (every leading index a matrix of its own), in its type.
-
-    X = matrix / |matrix|_F, then ``steps`` times X <- a X + (b P + c P P) X with P = X X^T (of the transposed matrix where it
-    is taller than wide).  The default coefficients take every singular value of an update into about [0.7, 1.2] in five
-    steps; (1.5, -0.5, 0) or (1.875, -1.25, 0.375) converge to the nearest orthogonal matrix in more.  A matrix of zeros gives
-    zeros.  Between the products values keep 22 bits in a range of +-255 (1 to 100 steps, coefficients within +-16: such that the
-    singular values stay near one).  Not differentiable: it sees the values only.
-    """
-    if not isinstance(matrix, torch.Tensor) or matrix.dim() < 2 or matrix.dtype not in _DTYPES:
-        raise RuntimeError("orthogonalize: [..., rows, cols] in float32, float16 or bfloat16")
-    if not matrix.is_cuda:
-        raise RuntimeError("orthogonalize: tensors live on the HIP device ('cuda'); there is no CPU path")
-    if len(coefficients) != 3:
-        raise RuntimeError("orthogonalize: three coefficients")
+def _orthogonalize(matrix, steps, coefficients):
     rows, cols = matrix.shape[-2:]
-    if rows == 0 or cols == 0:
-        raise RuntimeError(f"orthogonalize: empty matrices {tuple(matrix.shape)}")
     g = matrix.detach()
     if g.dim() > 3:
         g = g.reshape(-1, rows, cols)
@@ -329,6 +313,41 @@ def orthogonalize(matrix: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4
     _lib.check(lib.fra_orthogonalize_workspace_bytes(batch, rows, cols, C.byref(need)), "fra_orthogonalize_workspace_bytes")
     ws = torch.empty(need.value, dtype=torch.uint8, device=matrix.device)
     _lib.check(_on_device(matrix.device, lib.fra_orthogonalize, _DTYPES[g.dtype], g.data_ptr(), s0 if rows > 1 else cols,
-                          g.stride(0) if g.dim() == 3 else 0, batch, rows, cols, int(steps), *[float(v) for v in coefficients],
+                          g.stride(0) if g.dim() == 3 else 0, batch, rows, cols, steps, *[float(v) for v in coefficients],
                           out.data_ptr(), ws.data_ptr(), need.value, _stream(matrix.device)), "fra_orthogonalize")
     return out
+
+
+class _ValuesOnly(torch.autograd.Function):
+    """``_orthogonalize`` of a matrix whose derivatives are being followed, so that one that goes through it is not lost without a word."""
+
+    @staticmethod
+    def forward(ctx, matrix, steps, coefficients):
+        return _orthogonalize(matrix, steps, coefficients)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise RuntimeError("orthogonalize is not differentiable: call it on matrix.detach(), or under torch.no_grad(), for its values")
+
+
+def orthogonalize(matrix: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315)) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of [..., rows, cols] (every leading index a matrix of its own), in its type.
+
+    X = matrix / |matrix|_F, then ``steps`` times X <- a X + (b P + c P P) X with P = X X^T (of the transposed matrix where it
+    is taller than wide).  The default coefficients take every singular value of an update into about [0.7, 1.2] in five
+    steps; (1.5, -0.5, 0) or (1.875, -1.25, 0.375) converge to the nearest orthogonal matrix in more.  A matrix of zeros gives
+    zeros.  Between the products values keep 22 bits in a range of +-255 (1 to 100 steps, coefficients within +-16: such that the
+    singular values stay near one).  Not differentiable: a derivative asked of it, backward or forward mode, is an error.
+    """
+    if not isinstance(matrix, torch.Tensor) or matrix.dim() < 2 or matrix.dtype not in _DTYPES:
+        raise RuntimeError("orthogonalize: [..., rows, cols] in float32, float16 or bfloat16")
+    if not matrix.is_cuda:
+        raise RuntimeError("orthogonalize: tensors live on the HIP device ('cuda'); there is no CPU path")
+    if len(coefficients) != 3:
+        raise RuntimeError("orthogonalize: three coefficients")
+    rows, cols = matrix.shape[-2:]
+    if rows == 0 or cols == 0:
+        raise RuntimeError(f"orthogonalize: empty matrices {tuple(matrix.shape)}")
+    if torch.is_grad_enabled() and matrix.requires_grad or forward_ad._current_level >= 0:
+        return _ValuesOnly.apply(matrix, int(steps), coefficients)
+    return _orthogonalize(matrix, int(steps), coefficients)

@@ -219,3 +219,23 @@ def test_products_by_the_lower_triangle(device, shape):
         want = want.mT if tall else want
         assert torch.linalg.matrix_norm(y[i].double() - want).item() <= allowed([1.0], want, USUAL, torch.float32)
         assert (y[i].double() - want).abs().max() <= 2.0 ** -12 * want.abs().max()      # no value out of place
+
+
+def test_a_derivative_is_refused_not_lost(device):
+    w = matrix((24, 40), torch.float32, device, 23).requires_grad_(True)
+    want = projection.orthogonalize(w.detach())
+    assert not want.requires_grad
+    y = projection.orthogonalize(w)
+    assert torch.equal(y, want)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        (y.sum() + w.sum()).backward()                               # w's own path alone would be a wrong gradient
+    assert w.grad is None
+    with torch.no_grad():
+        assert torch.equal(projection.orthogonalize(w), want) and not projection.orthogonalize(w).requires_grad
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(w.detach(), torch.ones_like(w))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            projection.orthogonalize(dual)
+        assert torch.equal(projection.orthogonalize(w.detach()), want)      # no tangent, nothing to lose
+    with torch.inference_mode():
+        assert torch.equal(projection.orthogonalize(w), want)
