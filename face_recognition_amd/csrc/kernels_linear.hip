@@ -8,7 +8,8 @@
 // its rows through it and scatters its results back.  The backward pass sorts once, while it reads anyway: dz lies in list
 // order, x is copied into it for dW, and both gradients' products then run over contiguous rows.  Sums are fp32; z and dz are
 // rounded once to the product's type (they are operands of the matrix instructions / of act' only, the same half step as the
-// outputs').
+// outputs').  What that costs, bf16 with gelu, dx and dW against 64 bits: 0.0017 of the norm is the outputs' own rounding, 0.0023 with
+// dz's, 0.0024 with both; a dz in two bf16 halves would double the products, a z in fp32 the bytes kept between the passes.
 #include "pj_tile.h"
 
 namespace fra {
@@ -172,9 +173,11 @@ __device__ __forceinline__ bool next_tile(const RowArgs& a, unsigned b, int n_co
 // PFLOP/s; the library's plain product 1.45); K = 512 by what surrounds a tile's eight steps -- of the 12.7 us of a 128 x 128 tile
 // two such workgroups on a compute unit spend 7.4 in the steps, 2.8 before the first one's data are there and 2.5 on the results
 // (4.2 with a residual and a sigmoid), and neither walking over tiles with the next one's data ahead (the registers do not hold it)
-// nor a deeper pipeline shortened that.  262144 x 512 x 512 f16 with silu and residual 241 us (3.3 TB/s of its 806 MB), 1024 x 40961
-// x 512 bf16 70 us (613 TFLOP/s), 4096 x 2048 x 1024 bf16 with gelu 23.8 us (721 TFLOP/s), 30001 x 768 x 512 in 37 groups 44 us,
-// fp32 4096^3 1.07 ms (128 TFLOP/s of the library's 141).
+// nor a deeper pipeline shortened that.  Aligned 256 x 256 tiles fill the register file: 16 registers of a lane are spilled (68 bytes).
+// Calls in a row: 262144 x 512 x 512 f16 with silu and residual 242 us (3.3 TB/s of its 806 MB), 1024 x 40961 x 512 bf16 72 us (595
+// TFLOP/s; in a captured graph 63, of which 6 are the odd column's: 57 with 40960), 4096 x 2048 x 1024 bf16 with gelu 23.6 us in a graph
+// (728 TFLOP/s), 30001 x 768 x 512 in 37 groups 45 us under the profiler, fp32 4096^3 1.07 to 1.15 ms (120 to 128 TFLOP/s of the
+// library's 141).
 template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT, S::WAVES) void pj_forward_kernel(FwdArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     typedef Product<T, false, false, S, DMA> P;
@@ -212,7 +215,7 @@ template <typename T, typename S, bool DMA> __global__ __launch_bounds__(S::NT, 
 
 // The same for few rows (tiles of 16 MT): a workgroup takes 16 columns, its eight waves every eighth group of k (K = 512 is one
 // trip to memory), and their sums meet in LDS, added in a fixed order.  Bound by the latency of one trip to memory (1 x 512 x 512
-// f16: 3.1 us in a graph, of tiles 4.7), or by W's bytes (1 x 40961 x 512: 11.8 us, 3.6 TB/s): a column's weights are read once,
+// f16: 3.2 us in a captured graph, on tiles 4.9), or by W's bytes (1 x 40961 x 512: 9.6 us, 4.4 TB/s): a column's weights are read once,
 // straight into MFMA operands, in pieces of 64 bytes of sixteen rows whose neighbours the other waves take.
 template <typename T, int MT> __global__ __launch_bounds__(512) void pj_few_rows_kernel(FwdArgs a) {
     typedef typename Elem<T>::Frag Frag;
@@ -593,7 +596,8 @@ template <typename T> __global__ __launch_bounds__(256) void pj_prep_kernel(Prep
 //                            pieces, for groups of more than one (a workgroup belongs to one group, join_each to each);
 //   the others:              out[g][n] = sum of part[t][n] over the group's tiles, for bias and slope: 16 waves take every sixteenth
 //                            tile of 64 columns, their sums are added in order.
-// 4 us where only the latter is to do, 7 us with four partial sums of 2048 x 1024.
+// 4 us where only the latter is to do, 7 us with four partial sums of 2048 x 1024.  One workgroup for 64 columns' sums, whatever the
+// rows: with 262144 of them and 40 columns (4096 tiles' sums, and 128 of dW's shares) 39 us bf16, 47 fp32.
 struct FinishArgs {
     const float* dw_part;
     void* dw;
@@ -938,11 +942,12 @@ template <typename T, int MT> static int launch_few_rows(const fra_linear_desc* 
 template <typename T> static int forward_t(const fra_linear_desc* d, void* z, void* y, hipStream_t s) {
     FwdArgs a;
     // Few rows, or so few columns that tiles would be empty, have a kernel of their own.  (Its sums are in another order, so beyond 64
-    // rows a value does not depend on the number of rows beside it: there the columns alone decide.)  Columns: up to 16, the kernel's
-    // own, as far as its launch goes (262144 x 16 x 512 bf16 53 us, on tiles 116; fp32 125 and 289).  Rows: fp32 up to 64 (64 x 40961
-    // x 512 66 us, on tiles 76), 16 bits up to 16 (1 x 40961 x 512 11.8 and 14.2), and up to 64 by what a compute unit fetches, in rows of k: this kernel's tiles
-    // are smaller, the others' read a wide product's operands less often (50 x 333 x 512 3.4 us, on tiles 5.2; 64 x 4096 x 2048 13.0
-    // and 10.4).  What DMA cannot take stays longer in the tiles' steps, for which it gets two rows of sixteen in advance.
+    // rows a value does not depend on the number of rows beside it: there the columns alone decide.)  Times in a captured graph, here and
+    // on tiles.  Columns: up to 16, the kernel's own, as far as its launch goes (fp32 262144 x 16 x 512 133 us and 163, x 5 127 and 164,
+    // 1000 x 12 x 512 4.3 and 10.1; bf16 55 and 53, 51 and 59, 3.4 and 5.8).  Rows: fp32 up to 64 (64 x 40961 x 512 65 us and 76, 50 x
+    // 333 x 512 4.5 and 10.2), 16 bits up to 16 (1 x 40961 x 512 9.6 and 13.2), and up to 64 by what a compute unit fetches, in rows of
+    // k: this kernel's tiles are smaller, the others' read a wide product's operands less often (f16 50 x 333 x 512 3.6 us and 5.8; 64 x
+    // 4096 x 2048 13.1 and 10.6).  What DMA cannot take stays longer in the tiles' steps, for which it gets two rows of sixteen in advance.
     const int most = d->groups ? d->groups->tile_rows : 256, side = tile_side(d->M, d->N, sizeof(T) == 4, most);
     auto fetched = [&](int bi, int bj) { return ((int64_t)cdiv(d->M, bi) * cdiv(d->N, bj) + 255) / 256 * ((bi + bj) / 16); };
     int mt = 1;                                                     // tiles of 16 rows: as many as fetch least
@@ -987,7 +992,10 @@ template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc*
     p.pack_w = dx && !dma_ok<T>(d->w, d->ldw | d->w_group_stride, d->K);
     p.dz_rows = g ? g->tile_rows : 64;
     p.n_tiles = g ? g->n_tiles : cdiv(d->M, p.dz_rows);
-    // dW: enough workgroups to fill the chip twice, each with at least 128 rows; tiles of 64 where tiles of 128 cannot be that many.
+    // dW: enough workgroups to fill the chip twice, each with at least 128 rows; tiles of 64 where tiles of 128 cannot be that many
+    // (forward and gradients, 4096 x 2048 x 1024 bf16 87 us, with 64 98; fp32 469 and 476).  How far N and K fill the tiles is not
+    // weighed, which narrow products pay for (262144 x 40 x 512 fp32 984 us, with 64 579; bf16 268 and 253; 16384 x 130 x 512 134 and 119, 64
+    // and 52).
     // With groups a piece has at most four times the average group's rows as well, so that a batch whose rows are nearly all of one
     // group does not leave the chip to that group's tiles.
     const int64_t share = d->M / G / 128 > 1 ? d->M / G / 128 : 1;
@@ -1023,7 +1031,7 @@ template <typename T> static BackwardPlan backward_plan_t(const fra_linear_desc*
         if (sp > 1) p.n_parts = (int)sp;
     }
     size_t at = 0;
-    p.off_dz = at; if (p.need_dz) at += up((size_t)d->M * p.Np * es);
+    p.off_dz = at; if (p.need_dz) at += up((size_t)d->M * p.Np * es);      // also where an aligned dy will serve as dz: it is not known yet
     p.off_x = at; if (p.pack_x) at += up((size_t)d->M * p.Kp * es);
     p.off_w = at; if (p.pack_w) at += up((size_t)G * d->N * p.Kp * es);
     p.off_b = at; if (db) at += up((size_t)p.n_tiles * d->N * 4);

@@ -9,8 +9,8 @@
 // over three times that of the fp32 matrix instructions.  Against 64 bits the results are as near as the same iteration with
 // fp32 products (512 x 512: 1.4e-6 of the norm, fp32 2.1e-6).
 //
-// 17 launches for five steps.  Small matrices are bound by the launches' latency (512 x 512 fp32 104 us, 6 us each), large ones by
-// the matrix cores: eight of 2048 x 1024 1.09 ms, one of 4096 x 4096 3.9 ms.  P and Q are symmetric: where that saves rounds of
+// 17 launches for five steps.  Small matrices are bound by the launches' latency (512 x 512 fp32 108 us, 6 us each), large ones by
+// the matrix cores: eight of 2048 x 1024 1.09 ms, one of 4096 x 4096 4.0 ms.  P and Q are symmetric: where that saves rounds of
 // workgroups, only the tiles of the lower triangle are computed (1.27 and 4.9 ms with all of them).
 #include "pj_tile.h"
 
@@ -399,7 +399,8 @@ template <typename T, bool BK, bool LAST, typename S, bool TOGETHER> static int 
     FRA_HIP(hipGetLastError());
     return FRA_OK;
 }
-// rounds of one workgroup per compute unit that are at least nine tenths full
+// rounds of one workgroup per compute unit that are at least nine tenths full.  Counted in tiles, whatever of them the matrices fill: many
+// small ones take large tiles too (256 of 64 x 64 126 us, 250 of 100 x 100 231, 60 of 321 x 330 559)
 static bool full_rounds(int64_t tiles) { return tiles >= 230 && tiles * 10 >= (tiles + 255) / 256 * 256 * 9; }
 // Whether the lower triangle is worth it.  How long a product takes, in rounds of 128 x 128 tiles: a round of 256 x 256 is 3.3 of
 // them; one of 64 x 64 on a unit 0.35, two 0.6 (eight of 1024 x 1024: P from X of 2048 columns 117 -> 81 us, Q 57 -> 47; a matrix

@@ -3,11 +3,11 @@
     linear(x, weight, bias, activation, slope, residual)            y = act(x W^T + b) + r
     group_rows(ids, n_groups) -> RowGroups                          rows sorted by the group they name
     grouped_linear(x, weight[G], groups, ...)                       every row through its group's matrix
-    orthogonalize(matrix, steps, coefficients)                      an update (or a fitted map) made orthogonal
+    orthogonalize(matrix, steps, coefficients)                      an update made nearly orthogonal, or a fitted map wholly
 
 Uses: a head on top of the 512-wide embeddings, a map that takes one network's embeddings into another's space so that an
-existing gallery stays searchable, one such map per camera / tenant / model version, and the training of all of these (an
-orthogonal map leaves distances, and the thresholds set for them, as they are).  No counterpart in the reference.  All
+existing gallery stays searchable, one such map per camera / tenant / model version, and the training of all of these (a map
+that is wholly orthogonal leaves distances, and the thresholds set for them, as they are).  No counterpart in the reference.  All
 products run in the HIP library (``fra_linear``, ``fra_group_rows``, ``fra_orthogonalize``); there is no CPU path.
 
 Types: float32, float16, bfloat16; ``x``, ``weight`` and ``residual`` share one, ``bias`` and ``slope`` are of it or float32.
@@ -334,9 +334,10 @@ def orthogonalize(matrix: torch.Tensor, steps: int = 5, coefficients=(3.4445, -4
     """Newton-Schulz orthogonalisation of [..., rows, cols] (every leading index a matrix of its own), in its type.
 
     X = matrix / |matrix|_F, then ``steps`` times X <- a X + (b P + c P P) X with P = X X^T (of the transposed matrix where it
-    is taller than wide).  The default coefficients take every singular value of an update into about [0.7, 1.2] in five
-    steps; (1.5, -0.5, 0) or (1.875, -1.25, 0.375) converge to the nearest orthogonal matrix in more.  A matrix of zeros gives
-    zeros.  Between the products values keep 22 bits in a range of +-255 (1 to 100 steps, coefficients within +-16: such that the
+    is taller than wide).  The default coefficients (published by K. Jordan et al. with the Muon optimizer, 2024) take the singular
+    values of an update, but the smallest, into about [0.7, 1.2] in five steps and do not converge further: good for an update, not for
+    a map that is to leave distances as they are.  Those of the Newton-Schulz iteration, (1.5, -0.5, 0) or (1.875, -1.25, 0.375),
+    converge to the nearest orthogonal matrix in more steps (20 to 40, by the smallest singular value).  A matrix of zeros gives zeros.  Between the products values keep 22 bits in a range of +-255 (1 to 100 steps, coefficients within +-16: such that the
     singular values stay near one).  Not differentiable: a derivative asked of it, backward or forward mode, is an error.
     """
     if not isinstance(matrix, torch.Tensor) or matrix.dim() < 2 or matrix.dtype not in _DTYPES:

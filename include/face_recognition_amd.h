@@ -299,7 +299,7 @@ int fa_align_warp(const uint8_t* frame, int H, int W, const double* matrices, in
  * w, resid, preact, out and their gradients; bias and slope are of that type or fp32.  Sums are fp32 (fp32 products on the fp32
  * matrix instructions).  Rows are contiguous, at a pitch of ldx / ldw / ldr elements; any element alignment works, 16-byte aligned
  * rows are the fast ones.  Results do not depend on timing, nor, beyond 64 rows, a row's on the number of rows beside it (without
- * groups).
+ * groups; with up to 16 columns, up to 2^28 rows).
  * Nothing here allocates; scratch is the caller's, 16-byte aligned. */
 enum fra_activation {
     FRA_ACT_NONE = 0, FRA_ACT_RELU = 1,
@@ -338,14 +338,16 @@ int fra_group_rows(const void* ids, int ids_are_64bit, const fra_row_groups* g, 
 int fra_linear(const fra_linear_desc* d, void* preact, void* out, fra_stream stream);
 /* Gradients of the wanted (non-NULL) of: dx [M,K], dw [N,K] or [n_groups,N,K] (a group without rows: zeros), dbias / dslope
  * [N] or [n_groups,N] in bias_dtype / slope_dtype, all contiguous; the residual's gradient is dy itself.  dy dev [M,N] at a
- * pitch of lddy.  The descriptor is the forward call's; its bias and resid are not read. */
+ * pitch of lddy.  The descriptor is the forward call's; its bias and resid are not read.  FRA_ACT_RELU takes dy or leaves it: an
+ * infinite dy where z <= 0 does not count.  Scratch is sized for a dy of any alignment. */
 int fra_linear_backward_workspace_bytes(const fra_linear_desc* d, int want_dx, int want_dw, int want_dbias, int want_dslope,
                                         size_t* bytes);
 int fra_linear_backward(const fra_linear_desc* d, const void* preact, const void* dy, int64_t lddy, void* dx, void* dw,
                         void* dbias, void* dslope, void* workspace, size_t workspace_bytes, fra_stream stream);
 /* Newton-Schulz orthogonalisation of `batch` matrices g [rows][cols] (pitch ldg, batch_stride elements apart), as applied to
  * the update of a weight matrix: X = g / |g|_F, then `steps` times X <- a X + (b P + c P P) X with P = X X^T (of the transposed
- * matrix where rows > cols).  out dev [batch][rows][cols] contiguous, dtype as g.  A matrix of zeros gives zeros.  Between
+ * matrix where rows > cols).  How near to orthogonal the result is depends on a, b, c and steps.  out dev [batch][rows][cols]
+ * contiguous, dtype as g.  A matrix of zeros gives zeros.  Between
  * products values are held to 22 bits in a range of +-255: coefficients under which the singular values stay near one.
  * Scratch: dev, fra_orthogonalize_workspace_bytes(). */
 int fra_orthogonalize_workspace_bytes(int64_t batch, int rows, int cols, size_t* bytes);
